@@ -37,6 +37,12 @@ class Geom(ctypes.Structure):
     ]
 
 
+class Rotary(ctypes.Structure):
+    """Mirror of `bob_sm100_rotary`."""
+
+    _fields_ = [("pairs", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("factor", ctypes.c_double), ("turns", ctypes.c_uint64 * 64)]
+
+
 # every symbol include/bob_sm100.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "bob_sm100_version": (ctypes.c_int, []),
@@ -52,6 +58,11 @@ SYMBOLS = {
     "bob_sm100_noalloc_max_rows": (ctypes.c_size_t, []),
     "bob_sm100_noalloc_read_status": (ctypes.c_int, [ctypes.c_int, _vp]),
     "bob_sm100_bwd2_noalloc": (ctypes.c_int, [ctypes.POINTER(Geom)] + [_vp] * 17),
+    "bob_sm100_rotate": (ctypes.c_int, [_vp] * 2),
+    "bob_sm100_cache_append": (ctypes.c_int, [_vp] * 3 + [ctypes.c_int] + [_vp] * 5),
+    "bob_sm100_cache_read": (ctypes.c_int, [_vp] * 2 + [ctypes.c_int] + [_vp] * 3),
+    "bob_sm100_paged_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "bob_sm100_paged_fwd": (ctypes.c_int, [_vp] * 3),
     "bob_sm100_timeout_selftest": (ctypes.c_int, [_vp, _vp]),
     "bob_sm100_selftest": (ctypes.c_int, [_vp, _vp, ctypes.c_int, _vp, _vp, _vp]),
 }

@@ -11,7 +11,8 @@ from pathlib import Path
 from . import _lib
 
 _MODULE_PATH = Path(__file__).resolve().parent / "bob_torch.so"
-_BOUND = ("fwd", "bwd1", "bwd2", "workspace_bytes", "read_status", "last_status", "error_string")
+_BOUND = ("fwd", "bwd1", "bwd2", "workspace_bytes", "read_status", "last_status", "error_string", "rotate", "cache_append",
+          "cache_read", "paged_workspace_bytes", "paged_fwd")
 
 _module = None
 _lock = threading.Lock()

@@ -18,8 +18,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libbob_sm100.so"
 TORCH_MODULE = PKG / "bob_torch.so"
-SOURCES = ("api.cu", "selftest.cu", "noalloc.cu")
-HEADERS = ("ptx.cuh", "sweep.cuh", "decode.cuh", "tmap.h", "internal.h")
+SOURCES = ("api.cu", "selftest.cu", "noalloc.cu", "paged.cu")
+HEADERS = ("ptx.cuh", "sweep.cuh", "decode.cuh", "tmap.h", "internal.h", "rotary.cuh", "cache.cuh", "paged.cuh")
 
 
 def _nvcc() -> str:
@@ -68,7 +68,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     srcs = [str(CSRC / s) for s in SOURCES if (CSRC / s).exists()]
     cmd = [
         _nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-        "-shared", "-Xcompiler", "-fPIC", "-o", str(LIB), *srcs,
+        "-shared", "-Xcompiler", "-fPIC", "--threads", "0", "-o", str(LIB), *srcs,
     ]
     if verbose:
         cmd[1:1] = ["-Xptxas", "-v"]

@@ -384,6 +384,8 @@ extern "C" const char* bob_sm100_error_string(int code) {
         case -12: return "problem too large for the built-in scratch (B*Hq*Nq > 1048576 rows)";
         case -101: return "tensor base address must be 16-byte aligned";
         case -102: return "tensor strides unusable for TMA";
+        case 21: return "device: a page table entry within a sequence's length is outside the cache";
+        case 22: return "device: a sequence's length or number of new tokens is out of range";
         case 77: return "device: the self-test's wait ran out (as it is meant to)";
         case kStatusTimeoutLoad: return "device: a wait for a TMA load ran out";
         case kStatusTimeoutMma: return "device: a wait in the MMA issuer ran out";

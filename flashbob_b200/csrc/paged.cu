@@ -1,0 +1,344 @@
+// Host side of the C ABI for rotary positions, the paged cache and the attention over it.
+#include "internal.h"
+#include "paged.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+namespace bob {
+
+// Return codes as in api.cu.
+enum : int { kBadNull = -1, kBadGeom = -2, kBadDtype = -3, kBadHeadDim = -4, kBadStride = -5, kBadWorkspace = -6, kBadDevice = -7,
+             kBadLaunch = -8, kBadAttr = -9, kBadAlign = -10 };
+
+// B200's SMs, and not asked of the device: the workspace's size then depends on the arguments alone.
+constexpr int kPagedSms = 148;
+constexpr int kMaxDevices = 64;
+
+struct CurrentDevice {
+    int before = -1;
+    bool ok = true, changed = false;
+    explicit CurrentDevice(int device) {
+        if (device < 0 || device >= kMaxDevices || cudaGetDevice(&before) != cudaSuccess) { ok = false; return; }
+        changed = before != device;
+        if (changed && cudaSetDevice(device) != cudaSuccess) { ok = false; changed = false; }
+    }
+    ~CurrentDevice() { if (changed) cudaSetDevice(before); }
+};
+
+static int launched() { return cudaGetLastError() == cudaSuccess ? 0 : kBadLaunch; }
+
+static int check_head_dim(int D) { return D == 32 || D == 64 || D == 128 ? 0 : kBadHeadDim; }
+static int check_dtype(int dtype) { return dtype == BOB_SM100_FP16 || dtype == BOB_SM100_BF16 ? 0 : kBadDtype; }
+
+// Strides and address of a [B, H, N, D] tensor of tokens; a stride of zero repeats, as of an expanded tensor.
+static int check_tokens(const void* ptr, const int64_t* strides) {
+    if (!ptr || !strides) return kBadNull;
+    if (reinterpret_cast<uintptr_t>(ptr) % 16) return kBadAlign;
+    for (int i = 0; i < 3; ++i)
+        if (strides[i] < 0 || strides[i] % 8) return kBadStride;
+    return 0;
+}
+
+static int check_rotary(const bob_sm100_rotary& r, int D) {
+    return r.pairs >= 0 && 2 * r.pairs <= D && std::isfinite(r.factor) ? 0 : kBadGeom;
+}
+
+static int check_cache(const bob_sm100_cache* c) {
+    if (!c) return kBadNull;
+    if (int rc = check_dtype(c->dtype)) return rc;
+    if (int rc = check_head_dim(c->D)) return rc;
+    if (c->pages <= 0 || c->heads <= 0 || c->page_size < 16 || c->page_size > 4096 || (c->page_size & (c->page_size - 1))) return kBadGeom;
+    if (c->bits != 16 && c->bits != 4) return kBadGeom;
+    for (int w = 0; w < 2; ++w) {
+        if (!c->data[w] || (c->bits == 4 && !c->scales[w])) return kBadNull;
+        if (reinterpret_cast<uintptr_t>(c->data[w]) % 16 || reinterpret_cast<uintptr_t>(c->scales[w]) % 8) return kBadAlign;
+        for (int i = 0; i < 3; ++i)
+            if (c->strides[w][i] < 0 || c->strides[w][i] % 16 || (c->bits == 4 && (c->scale_strides[w][i] < 0 || c->scale_strides[w][i] % 8))) return kBadStride;
+    }
+    return 0;
+}
+
+static int check_sequences(const bob_sm100_cache* c, const bob_sm100_sequences* s) {
+    if (!s || !s->table || !s->lengths) return kBadNull;
+    if (s->B <= 0 || s->max_pages <= 0 || s->table_stride < 0 || (int64_t)s->max_pages * c->page_size > (1 << 28)) return kBadGeom;
+    return 0;
+}
+
+static SequenceParams sequences(const bob_sm100_cache* c, const bob_sm100_sequences* s) {
+    SequenceParams p = {};
+    p.table = s->table; p.table_stride = s->table_stride;
+    p.lengths = s->lengths; p.counts = s->counts;
+    p.B = s->B; p.max_pages = s->max_pages; p.pages = c->pages;
+    while ((1 << p.page_shift) < c->page_size) ++p.page_shift;
+    p.sticky = sticky_word(c->device, true);
+    return p;
+}
+
+static CacheTensor cache_tensor(const bob_sm100_cache* c, int w) {
+    CacheTensor t = {};
+    t.data = static_cast<uint8_t*>(c->data[w]); t.sp = c->strides[w][0]; t.sh = c->strides[w][1]; t.sr = c->strides[w][2];
+    t.scales = static_cast<float*>(c->scales[w]);
+    t.ssp = c->scale_strides[w][0] / 4; t.ssh = c->scale_strides[w][1] / 4; t.ssr = c->scale_strides[w][2] / 4;
+    return t;
+}
+
+template <int V> struct Int { static constexpr int value = V; };
+
+template <class F> static void with_form(int form, F f) {
+    if (form == kHalf) f(Int<kHalf>{});
+    else if (form == kInterleaved) f(Int<kInterleaved>{});
+    else f(Int<kScattered>{});
+}
+template <class F> static void with_type(int dtype, F f) {
+    if (dtype == BOB_SM100_BF16) f(std::true_type{});
+    else f(std::false_type{});
+}
+
+// Threads of a grid that has enough of them to hide the memory's latency; with more, a thread takes several heads and
+// shares its sines and cosines between them.
+constexpr int64_t kManyThreads = (int64_t)kPagedSms * 2048;
+
+static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream) {
+    RotateParams p = {};
+    p.rotary = a->rotary;
+    if (a->inverse)
+        for (uint64_t& x : p.rotary.turns) x = 0 - x;
+    for (int i = 0; i < 2; ++i) {
+        p.t[i].in = static_cast<const uint16_t*>(a->in[i]);
+        p.t[i].in_sb = a->in_strides[i][0]; p.t[i].in_sh = a->in_strides[i][1]; p.t[i].in_sn = a->in_strides[i][2];
+        p.t[i].out = static_cast<uint16_t*>(a->out[i]);
+        p.t[i].H = a->heads[i];
+    }
+    p.B = a->B; p.N = a->N; p.D = a->D;
+    p.positions = a->positions; p.wide = a->position_bits == 64;
+    p.pos_sb = a->position_strides[0]; p.pos_sn = a->position_strides[1];
+    p.first = a->first;
+    const int64_t threads = (int64_t)a->B * a->N * (a->D / 16), blocks = (threads + kRotateThreads - 1) / kRotateThreads;
+    const int heads = a->heads[0] + a->heads[1];
+    if (blocks > 0x7fffffffLL) return kBadGeom;
+    with_form(rotary_form(&a->rotary), [&](auto form) {
+        with_type(a->dtype, [&](auto bf16) {
+            constexpr int F = decltype(form)::value;
+            constexpr bool BF = decltype(bf16)::value;
+            auto go = [&](auto hpt) {
+                constexpr int HPT = decltype(hpt)::value;
+                const dim3 grid((unsigned)blocks, (heads + HPT - 1) / HPT);
+                rotate_kernel<F, BF, HPT><<<grid, kRotateThreads, 0, stream>>>(p);
+            };
+            if (threads * heads >= 4 * kManyThreads) go(Int<4>{});
+            else go(Int<1>{});
+        });
+    });
+    return launched();
+}
+
+static int run_append(const bob_sm100_cache* c, const bob_sm100_sequences* s, const bob_sm100_rotary* r, int N, const void* const* in,
+                      const int64_t* const* strides, cudaStream_t stream) {
+    AppendParams p = {};
+    p.rotary = *r;
+    p.seq = sequences(c, s);
+    for (int w = 0; w < 2; ++w) {
+        p.cache[w] = cache_tensor(c, w);
+        p.in[w] = static_cast<const uint16_t*>(in[w]);
+        p.in_sb[w] = strides[w][0]; p.in_sh[w] = strides[w][1]; p.in_sn[w] = strides[w][2];
+    }
+    p.H = c->heads; p.N = N; p.D = c->D;
+    const int64_t threads = (int64_t)s->B * N * (c->D / 16), blocks = (threads + kCacheThreads - 1) / kCacheThreads;
+    if (blocks > 0x7fffffffLL) return kBadGeom;
+    with_form(rotary_form(r), [&](auto form) {
+        with_type(c->dtype, [&](auto bf16) {
+            constexpr int F = decltype(form)::value;
+            constexpr bool BF = decltype(bf16)::value;
+            auto go = [&](auto bits, auto hpt) {
+                constexpr int HPT = decltype(hpt)::value;
+                const dim3 grid((unsigned)blocks, (c->heads + HPT - 1) / HPT);
+                append_kernel<F, BF, decltype(bits)::value, HPT><<<grid, kCacheThreads, 0, stream>>>(p);
+            };
+            const bool many = threads * c->heads >= 4 * kManyThreads;
+            if (c->bits == 16) { if (many) go(Int<16>{}, Int<4>{}); else go(Int<16>{}, Int<1>{}); }
+            else { if (many) go(Int<4>{}, Int<4>{}); else go(Int<4>{}, Int<1>{}); }
+        });
+    });
+    return launched();
+}
+
+static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int n, void* const* out, cudaStream_t stream) {
+    ReadParams p = {};
+    p.seq = sequences(c, s);
+    p.seq.counts = nullptr;
+    for (int w = 0; w < 2; ++w) { p.cache[w] = cache_tensor(c, w); p.out[w] = static_cast<uint16_t*>(out[w]); }
+    p.H = c->heads; p.N = n; p.D = c->D;
+    const int64_t threads = (int64_t)s->B * n * (c->D / 16), blocks = (threads + kCacheThreads - 1) / kCacheThreads;
+    if (blocks > 0x7fffffffLL) return kBadGeom;
+    with_type(c->dtype, [&](auto bf16) {
+        constexpr bool BF = decltype(bf16)::value;
+        auto go = [&](auto bits, auto hpt) {
+            constexpr int HPT = decltype(hpt)::value;
+            const dim3 grid((unsigned)blocks, (c->heads + HPT - 1) / HPT);
+            read_kernel<BF, decltype(bits)::value, HPT><<<grid, kCacheThreads, 0, stream>>>(p);
+        };
+        const bool many = threads * c->heads >= 4 * kManyThreads;
+        if (c->bits == 16) { if (many) go(Int<16>{}, Int<2>{}); else go(Int<16>{}, Int<1>{}); }
+        else { if (many) go(Int<4>{}, Int<2>{}); else go(Int<4>{}, Int<1>{}); }
+    });
+    return launched();
+}
+
+// ---- attention --------------------------------------------------------------------------------------------------
+static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+struct PagedPlan { int mt, groups, ctas; size_t acc_offset, bytes; };
+
+static int block_keys(int D, int bits) { return bits == 16 ? 2048 / D : (D == 128 ? 32 : 64); }
+
+static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
+    PagedPlan d = {};
+    const int64_t R = (int64_t)a->N * (a->Hq / a->cache.heads);
+    d.mt = R <= 16 ? 1 : 2;
+    d.groups = (int)((R + 16 * d.mt - 1) / (16 * d.mt));
+    // no more CTAs than the longest possible sequences have work for
+    const int64_t kb = block_keys(a->cache.D, a->cache.bits), most = ((int64_t)a->seq.max_pages * a->cache.page_size + kb - 1) / kb;
+    const int64_t line = most * a->seq.B * a->cache.heads * d.groups;
+    d.ctas = (int)std::min<int64_t>(2 * kPagedSms, std::max<int64_t>(1, line / kPagedMinBlocks));
+    const size_t rows = (size_t)d.ctas * 2 * 16 * d.mt;
+    d.acc_offset = up256(rows * 2 * sizeof(float));
+    d.bytes = d.acc_offset + rows * a->cache.D * sizeof(float);
+    return d;
+}
+
+static int check_paged(const bob_sm100_paged_args* a) {
+    if (!a) return kBadNull;
+    if (int rc = check_cache(&a->cache)) return rc;
+    if (int rc = check_sequences(&a->cache, &a->seq)) return rc;
+    if (int rc = check_rotary(a->rotary, a->cache.D)) return rc;
+    if (a->Hq <= 0 || a->Hq % a->cache.heads || a->N <= 0 || a->N > (1 << 28)) return kBadGeom;
+    if (a->window < 0 || (a->window > 0 && !a->is_causal)) return kBadGeom;
+    if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return kBadGeom;
+    const int64_t R = (int64_t)a->N * (a->Hq / a->cache.heads);
+    const int64_t blocks = ((int64_t)a->seq.max_pages * a->cache.page_size + 15) / 16 + 1;
+    // a sequence's part of the line, and the grid of the second kernel, are counted in 32 bits
+    if (R > (1 << 28) || blocks * a->cache.heads * ((R + 15) / 16) > 0x7fffffffLL || (int64_t)a->seq.B * a->cache.heads * ((R + 15) / 16) > 0x7fffffffLL) return kBadGeom;
+    if (int rc = check_tokens(a->q, a->q_strides)) return rc;
+    if (!a->out) return kBadNull;
+    return reinterpret_cast<uintptr_t>(a->out) % 16 ? kBadAlign : 0;
+}
+
+template <int D, int MT, bool BF16, int BITS>
+static int launch_paged(PagedParams& p, int device, cudaStream_t stream) {
+    using CFG = PagedConfig<D, MT, BITS>;
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = 1ull << device;
+    if (!(done.load(std::memory_order_acquire) & bit)) {
+        if (cudaFuncSetAttribute(paged_kernel<D, MT, BF16, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, CFG::SMEM) != cudaSuccess) return kBadAttr;
+        done.fetch_or(bit, std::memory_order_release);
+    }
+    paged_kernel<D, MT, BF16, BITS><<<p.ctas, kPagedThreads, CFG::SMEM, stream>>>(p);
+    if (int rc = launched()) return rc;
+    // started while paged_kernel runs, and waits for it
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    const int rows = std::min(CFG::ROWS, p.N * p.G);
+    cfg.gridDim = dim3((unsigned)(p.seq.B * p.Hkv * p.groups), (unsigned)((rows + kPagedWarps - 1) / kPagedWarps));
+    cfg.blockDim = dim3(kPagedThreads);
+    cfg.stream = stream;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, combine_kernel<D, MT, BF16, BITS>, p) == cudaSuccess ? 0 : kBadLaunch;
+}
+
+static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_t stream) {
+    const PagedPlan d = paged_plan(a);
+    PagedParams p = {};
+    p.rotary = a->rotary;
+    p.seq = sequences(&a->cache, &a->seq);
+    for (int w = 0; w < 2; ++w) p.cache[w] = cache_tensor(&a->cache, w);
+    p.q = static_cast<const uint16_t*>(a->q); p.q_sb = a->q_strides[0]; p.q_sh = a->q_strides[1]; p.q_sn = a->q_strides[2];
+    p.out = static_cast<uint16_t*>(a->out);
+    p.Hq = a->Hq; p.Hkv = a->cache.heads; p.G = a->Hq / a->cache.heads; p.N = a->N;
+    p.form = rotary_form(&a->rotary);
+    p.groups = d.groups;
+    p.causal = a->is_causal != 0;
+    p.window = std::min(a->window, 1 << 28);
+    p.scale = a->scale;
+    p.ctas = d.ctas;
+    p.part_ml = static_cast<float*>(workspace);
+    p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + d.acc_offset);
+    int rc = 0;
+    with_type(a->cache.dtype, [&](auto bf16) {
+        constexpr bool BF = decltype(bf16)::value;
+        auto dim = [&](auto mt, auto bits) {
+            constexpr int MT = decltype(mt)::value, BITS = decltype(bits)::value;
+            if (a->cache.D == 32) rc = launch_paged<32, MT, BF, BITS>(p, a->cache.device, stream);
+            else if (a->cache.D == 64) rc = launch_paged<64, MT, BF, BITS>(p, a->cache.device, stream);
+            else rc = launch_paged<128, MT, BF, BITS>(p, a->cache.device, stream);
+        };
+        if (a->cache.bits == 16) { if (d.mt == 1) dim(Int<1>{}, Int<16>{}); else dim(Int<2>{}, Int<16>{}); }
+        else { if (d.mt == 1) dim(Int<1>{}, Int<4>{}); else dim(Int<2>{}, Int<4>{}); }
+    });
+    return rc;
+}
+
+}  // namespace bob
+
+using namespace bob;
+
+extern "C" int bob_sm100_rotate(const bob_sm100_rotate_args* a, void* stream) {
+    if (!a) return kBadNull;
+    if (int rc = check_dtype(a->dtype)) return rc;
+    if (int rc = check_head_dim(a->D)) return rc;
+    if (int rc = check_rotary(a->rotary, a->D)) return rc;
+    if (a->B <= 0 || a->N <= 0 || a->N > (1 << 28) || a->heads[0] <= 0 || a->heads[1] < 0 || (int64_t)a->heads[0] + a->heads[1] > 65535) return kBadGeom;
+    if (a->positions && a->position_bits != 32 && a->position_bits != 64) return kBadGeom;
+    for (int i = 0; i < (a->heads[1] ? 2 : 1); ++i) {
+        if (int rc = check_tokens(a->in[i], a->in_strides[i])) return rc;
+        if (!a->out[i]) return kBadNull;
+        if (reinterpret_cast<uintptr_t>(a->out[i]) % 16) return kBadAlign;
+    }
+    CurrentDevice device(a->device);
+    if (!device.ok) return kBadDevice;
+    return run_rotate(a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int bob_sm100_cache_append(const bob_sm100_cache* c, const bob_sm100_sequences* s, const bob_sm100_rotary* r, int N,
+                                      const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, void* stream) {
+    if (int rc = check_cache(c)) return rc;
+    if (int rc = check_sequences(c, s)) return rc;
+    if (!r) return kBadNull;
+    if (int rc = check_rotary(*r, c->D)) return rc;
+    if (N <= 0 || N > (1 << 28) || c->heads > 65535) return kBadGeom;
+    if (int rc = check_tokens(k, k_strides)) return rc;
+    if (int rc = check_tokens(v, v_strides)) return rc;
+    CurrentDevice device(c->device);
+    if (!device.ok) return kBadDevice;
+    const void* in[2] = {k, v};
+    const int64_t* strides[2] = {k_strides, v_strides};
+    return run_append(c, s, r, N, in, strides, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int bob_sm100_cache_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int n, void* k, void* v, void* stream) {
+    if (int rc = check_cache(c)) return rc;
+    if (int rc = check_sequences(c, s)) return rc;
+    if (n <= 0 || n > (1 << 28) || c->heads > 65535) return kBadGeom;
+    if (!k || !v) return kBadNull;
+    if (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % 16) return kBadAlign;
+    CurrentDevice device(c->device);
+    if (!device.ok) return kBadDevice;
+    void* out[2] = {k, v};
+    return run_read(c, s, n, out, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t bob_sm100_paged_workspace_bytes(const bob_sm100_paged_args* a) {
+    return check_paged(a) ? 0 : paged_plan(a).bytes;
+}
+
+extern "C" int bob_sm100_paged_fwd(const bob_sm100_paged_args* a, void* workspace, void* stream) {
+    if (int rc = check_paged(a)) return rc;
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256) return kBadWorkspace;
+    CurrentDevice device(a->cache.device);
+    if (!device.ok) return kBadDevice;
+    return run_paged(a, workspace, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,699 @@
+// Attention of new tokens' queries over a paged cache, 16-bit or 4-bit: out = softmax(scale q k^T + mask) v.
+//
+// What bounds it: reading the cached rows once.  A KV head's queries (count tokens x G heads, 16 or 32 rows at a time)
+// share every row that is read, and the products run on mma.sync (m16n8k16): a step of generation needs at most 16 rows of
+// a product, where tcgen05's 128 would be padding, and its operands come straight from the registers that decode 4 bits.
+//
+// Every warp is a stream of its own: it copies blocks of KB keys into its ring in shared memory (cp.async, NST - 1 blocks
+// ahead, also across the ends of its work), waits for its own copies only, and keeps its own running maximum, sum and
+// accumulator in registers; there is no barrier in the loop.  Rows outside the item's key range are filled with zeros and
+// not read, so nothing that lies there can reach a result.
+//
+// Work: the blocks of all (sequence, KV head, row group) items form one line, cut evenly between the CTAs whatever the
+// lengths are; the four warps of a CTA take a segment's blocks in turn and add up through their free ring slots.
+// An item inside one CTA is finished there; parts of a divided one are parked and added in the order of the CTAs by
+// combine_kernel, so results do not depend on which CTA finishes first.  The host needs no lengths for any of this.
+#pragma once
+
+#include "cache.cuh"
+
+namespace bob {
+
+struct PagedParams {
+    bob_sm100_rotary rotary;      // pairs 0: queries are taken as they are
+    SequenceParams seq;
+    CacheTensor cache[2];
+    const uint16_t* q; long long q_sb, q_sh, q_sn;
+    uint16_t* out;                // contiguous [B, Hq, N, D]
+    int Hq, Hkv, G, N, form;
+    int groups;                   // row groups of ROWS query rows per KV head
+    int causal, window;
+    float scale;
+    float* part_ml;               // [CTAs][2][ROWS] (reference, sum)
+    float* part_acc;              // [CTAs][2][ROWS][D]
+    int ctas;                     // CTAs of paged_kernel
+};
+
+constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
+constexpr int kPagedMinBlocks = 4;          // blocks that are worth a CTA of their own
+
+template <int D_, int MT_, int BITS_>
+struct PagedConfig {
+    static constexpr int D = D_, MT = MT_, BITS = BITS_, ROWS = 16 * MT;
+    // 16 bits: 4 KB of keys and 4 KB of values per block.  4 bits: 2 to 2.5 KB each, where the work per block counts.
+    static constexpr int KB = BITS == 16 ? 2048 / D : (D == 128 ? 32 : 64);
+    static constexpr int ROW_BYTES = D * BITS / 8, CHUNKS = ROW_BYTES / 16;
+    // 4 bits: a thread reads a word of four rows two apart; these strides put the rows into different banks
+    static constexpr int V_STRIDE = BITS == 16 ? ROW_BYTES : (D == 128 ? 80 : (D == 64 ? 48 : 16));
+    static constexpr int OFF_V = KB * ROW_BYTES, OFF_SK = OFF_V + KB * V_STRIDE, OFF_SV = OFF_SK + (BITS == 4 ? KB * 8 : 0);
+    static constexpr int STAGE = OFF_SV + (BITS == 4 ? KB * 8 : 0);
+    static constexpr int NST = BITS == 16 ? 3 : 4;
+    // columns that 16 rows of an accumulator bring into a ring slot at a time
+    static constexpr int EX_COLS = 64 * D <= STAGE ? D : D / 2;
+    static_assert(64 * EX_COLS <= STAGE && STAGE % 16 == 0, "an accumulator passes through a slot");
+    static constexpr int Q_STRIDE = 2 * D + 16;                  // bytes of a query row; the 16 spread rows over the banks
+    static constexpr int OFF_Q = kPagedWarps * NST * STAGE, OFF_ML = OFF_Q + ROWS * Q_STRIDE;
+    static constexpr int OFF_SLOT = OFF_ML + 2 * kPagedWarps * 16 * 4;
+    static constexpr int SMEM = OFF_SLOT + 16;
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
+}
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t* w) {
+    if constexpr (WORDS == 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+    else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Blocks [first, first + n) of KB keys that the queries of sequence b attend to, of every KV head and row group.
+struct BlockRange { int first, n; };
+template <int KB>
+__device__ __forceinline__ BlockRange blocks_of(const PagedParams& p, int b) {
+    const Sequence s = sequence_of(p.seq, b, p.N);
+    int lo = 0;
+    if (p.window > 0) lo = max(0, s.start - p.window + 1);
+    if (s.count == 0 || s.length <= lo) return {0, 0};
+    const int first = lo / KB;
+    return {first, (s.length + KB - 1) / KB - first};
+}
+
+// The line of all blocks: its length, and where it is cut.
+template <int KB>
+__device__ __forceinline__ long long line_length(const PagedParams& p, int lane) {
+    long long total = 0;
+    for (int b = lane; b < p.seq.B; b += 32) total += blocks_of<KB>(p, b).n;
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    return total * p.Hkv * p.groups;
+}
+__device__ __forceinline__ int line_parts(const PagedParams& p, long long total) {
+    return static_cast<int>(min((long long)p.ctas, max(1LL, total / kPagedMinBlocks)));
+}
+__device__ __forceinline__ long long cut(long long total, int parts, int i) { return total * i / parts; }
+
+// Walks the items of a CTA's stretch of the line.
+template <int KB>
+struct Cursor {
+    long long pos, end, base;     // base: where sequence b begins on the line
+    int b, first, n;              // its blocks
+    // the segment: blocks [blk, last) of an item, reduced to those that its rows attend to
+    int kv_head, group, blk, last, lo, hi;
+    bool whole, begins;           // the segment is the whole item; ... has its first block
+
+    // Finds the sequence that `begin` lies in.
+    __device__ __forceinline__ void start(const PagedParams& p, long long begin, long long end_, int lane) {
+        pos = begin; end = end_; base = 0; b = 0; first = 0; n = 0;
+        if (begin >= end_) return;
+        const int per = p.Hkv * p.groups;
+        for (int b0 = 0;; b0 += 32) {
+            const int mine = b0 + lane < p.seq.B ? blocks_of<KB>(p, b0 + lane).n : 0;
+            int upto = mine;
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += t;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, base + (long long)upto * per > begin);
+            if (past || b0 + 32 >= p.seq.B) {
+                const int l = past ? __ffs(past) - 1 : 31;
+                b = b0 + l;
+                base += (long long)__shfl_sync(0xffffffffu, upto - mine, l) * per;
+                break;
+            }
+            base += (long long)__shfl_sync(0xffffffffu, upto, 31) * per;
+        }
+        const BlockRange r = blocks_of<KB>(p, b);
+        first = r.first; n = r.n;
+    }
+    // The next segment; false at the end.
+    template <int ROWS>
+    __device__ __forceinline__ bool next(const PagedParams& p) {
+        if (pos >= end) return false;
+        const int per = p.Hkv * p.groups;
+        while (pos >= base + (long long)n * per) {
+            base += (long long)n * per;
+            const BlockRange r = blocks_of<KB>(p, ++b);
+            first = r.first; n = r.n;
+        }
+        const int at = static_cast<int>(pos - base), item = at / n, off = at - item * n;
+        const int take = static_cast<int>(min((long long)(n - off), end - pos));
+        kv_head = item / p.groups;
+        group = item - kv_head * p.groups;
+        blk = first + off;
+        last = blk + take;
+        whole = take == n;
+        begins = off == 0;
+        pos += take;
+        const Sequence s = sequence_of(p.seq, b, p.N);
+        const int i0 = group * ROWS / p.G, i1 = min((min((group + 1) * ROWS, p.N * p.G) - 1) / p.G, s.count - 1);
+        lo = p.window > 0 ? max(0, s.start + i0 - p.window + 1) : 0;
+        hi = i0 > i1 ? 0 : (p.causal ? min(s.length, s.start + i1 + 1) : s.length);
+        blk = max(blk, lo / KB);
+        last = min(last, (hi + KB - 1) / KB);
+        return true;
+    }
+};
+
+// Row `r` of a KV head's queries (token r / G, head r % G), turned to its position, into shared memory.
+template <int D, bool BF16, int FORM>
+__device__ __forceinline__ void bring_query(const PagedParams& p, uint16_t* dst, const uint16_t* src, int c, int position) {
+    const RowPlace<FORM> place(c, p.rotary.pairs);
+    Turner<FORM, BF16, float> turn;
+    const Chunks x = place.load(src);
+    turn.set(p.rotary, c, position);
+    place.store(dst, turn(x));
+}
+
+template <int D, int MT, bool BF16, int BITS>
+__global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_constant__ PagedParams p) {
+    using CFG = PagedConfig<D, MT, BITS>;
+    constexpr int KB = CFG::KB, NT = KB / 8, KS = D / 16, ROWS = CFG::ROWS, NST = CFG::NST, STAGE = CFG::STAGE;
+    constexpr float kLog2e = 1.4426950408889634f, kNone = -1e30f;
+    extern __shared__ __align__(128) uint8_t paged_smem[];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
+    const uint32_t ring = smem_u32(paged_smem) + warp * NST * STAGE;
+    float* sm_m = reinterpret_cast<float*>(paged_smem + CFG::OFF_ML);            // [warp][16]
+    float* sm_l = sm_m + kPagedWarps * 16;
+    volatile int* sm_slot = reinterpret_cast<volatile int*>(paged_smem + CFG::OFF_SLOT);
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    if (blockIdx.x == 0 && warp == 0) {
+        for (int b = lane; b < p.seq.B; b += 32)
+            if (!sequence_of(p.seq, b, p.N).ok) report(p.seq.sticky, kStatusBadLength);
+    }
+    const long long total = line_length<KB>(p, lane);
+    const int parts = line_parts(p, total);
+    if (static_cast<int>(blockIdx.x) >= parts) return;
+    const long long begin = cut(total, parts, blockIdx.x), end = cut(total, parts, blockIdx.x + 1);
+
+    // ---- copies: block `blk` of the copying cursor, a warp's every fourth of a segment ----------------------
+    Cursor<KB> src, seg;
+    src.start(p, begin, end, lane);
+    seg = src;
+    int fill = 0;                                        // ring slot that is free
+    bool more = true;
+    src.blk = src.last = 0;
+    int page_ids = -1;                                   // lane i: page of keys 16 i ... of the block
+    auto seek = [&]() {                                  // to this warp's next block, and ask for its pages
+        while (more && src.blk >= src.last) {
+            more = src.template next<ROWS>(p);
+            src.blk += warp;
+        }
+        page_ids = -1;
+        if (more) {
+            const int key = src.blk * KB + 16 * lane;
+            if (lane < KB / 16 && key + 15 >= src.lo && key < src.hi) {
+                page_ids = page_of(p.seq, src.b, key);
+                if (page_ids < 0) report(p.seq.sticky, kStatusBadPage);
+            }
+        }
+    };
+    auto copy_block = [&]() {
+        if (more) {
+            const uint32_t dst = ring + fill * STAGE;
+            const int key0 = src.blk * KB, mask = (1 << p.seq.page_shift) - 1;
+            #pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const CacheTensor& c = p.cache[w];
+                const uint8_t* head = c.data + src.kv_head * c.sh;
+                #pragma unroll
+                for (int k = 0; k < KB * CFG::CHUNKS / 32; ++k) {
+                    const int id = k * 32 + lane, r = id / CFG::CHUNKS, ch = id % CFG::CHUNKS, key = key0 + r;
+                    const int page = __shfl_sync(0xffffffffu, page_ids, r / 16);
+                    const bool there = key >= src.lo && key < src.hi && page >= 0;
+                    const uint8_t* from = there ? head + page * c.sp + (key & mask) * c.sr + 16 * ch : c.data;
+                    uint32_t to = dst + (w ? CFG::OFF_V + r * CFG::V_STRIDE : r * CFG::ROW_BYTES);
+                    if constexpr (BITS == 16) to += 16 * (ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3));
+                    else to += 16 * ch;
+                    copy16(to, from, there);
+                }
+                if constexpr (BITS == 4) {
+                    #pragma unroll
+                    for (int k = 0; k < KB / 32; ++k) {
+                        const int r = k * 32 + lane, key = key0 + r;
+                        const int page = __shfl_sync(0xffffffffu, page_ids, r / 16);
+                        const bool there = key >= src.lo && key < src.hi && page >= 0;
+                        const float* from = there ? c.scales + page * c.ssp + src.kv_head * c.ssh + (key & mask) * c.ssr : c.scales;
+                        copy8(dst + (w ? CFG::OFF_SV : CFG::OFF_SK) + 8 * r, from, there);
+                    }
+                }
+            }
+            src.blk += kPagedWarps;
+            seek();
+        }
+        cp_async_commit();                               // (an empty group at the end keeps the count)
+        fill = fill + 1 == NST ? 0 : fill + 1;
+    };
+    seek();
+    #pragma unroll 1
+    for (int i = 0; i < NST - 1; ++i) copy_block();
+    int slot = 0;                                        // ring slot of the next block to use
+
+    const float c_exp = p.scale * kLog2e;
+    const int R = p.N * p.G;
+    #pragma unroll 1
+    while (seg.template next<ROWS>(p)) {
+        const Sequence s = sequence_of(p.seq, seg.b, p.N);
+        const int row0 = seg.group * ROWS;
+        // ---- the item's queries ---------------------------------------------------------------------------
+        __syncthreads();                                 // (the last item's are in registers, its sums written)
+        #pragma unroll 1
+        for (int id = tid; id < ROWS * (D / 16); id += kPagedThreads) {
+            const int r = row0 + id / (D / 16), c = id % (D / 16), i = r / p.G, h = seg.kv_head * p.G + r % p.G;
+            uint16_t* dst = reinterpret_cast<uint16_t*>(paged_smem + CFG::OFF_Q + (id / (D / 16)) * CFG::Q_STRIDE);
+            if (r < R && i < s.count) {
+                const uint16_t* from = p.q + seg.b * p.q_sb + h * p.q_sh + i * p.q_sn;
+                if (p.form == kHalf) bring_query<D, BF16, kHalf>(p, dst, from, c, s.start + i);
+                else if (p.form == kInterleaved) bring_query<D, BF16, kInterleaved>(p, dst, from, c, s.start + i);
+                else bring_query<D, BF16, kScattered>(p, dst, from, c, s.start + i);
+            } else {
+                RowPlace<kInterleaved>(c, 0).store(dst, Chunks{});
+            }
+        }
+        __syncthreads();
+        uint32_t qa[MT][KS][4];
+        float q_sum[MT][2];                              // 4 bits: sum of a row's elements
+        (void)q_sum;
+        #pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const uint32_t base = smem_u32(paged_smem) + CFG::OFF_Q + mt * 16 * CFG::Q_STRIDE;
+            if constexpr (BITS == 16) {
+                #pragma unroll
+                for (int ks = 0; ks < KS; ++ks) ldsm4(base + (lane % 16) * CFG::Q_STRIDE + ks * 32 + (lane / 16) * 16, qa[mt][ks]);
+            } else {
+                // the elements in the order in which a word of codes yields them: thread t holds words NWD t ... of a
+                // key row, and a word's pairs are (e, e + 4)
+                constexpr int NWD = D / 32;
+                #pragma unroll
+                for (int hr = 0; hr < 2; ++hr) {
+                    float sum = 0.f;
+                    #pragma unroll
+                    for (int j = 0; j < NWD; ++j) {
+                        uint32_t w[4];
+                        lds_words<4>(base + (g + 8 * hr) * CFG::Q_STRIDE + 16 * (NWD * t + j), w);
+                        float f[8];
+                        widen8<BF16>(make_uint4(w[0], w[1], w[2], w[3]), f);
+                        #pragma unroll
+                        for (int e = 0; e < 8; ++e) sum += f[e];
+                        #pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            qa[mt][2 * j + half][hr] = __byte_perm(w[half], w[2 + half], 0x5410);
+                            qa[mt][2 * j + half][2 + hr] = __byte_perm(w[half], w[2 + half], 0x7632);
+                        }
+                    }
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    q_sum[mt][hr] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+                }
+            }
+        }
+        int lo[MT][2], hi[MT][2];                        // keys that my rows attend to
+        int all_lo = 0, all_hi = 0x7fffffff;             // ... that every row of the item does
+        #pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            #pragma unroll
+            for (int hr = 0; hr < 2; ++hr) {
+                const int i = (row0 + mt * 16 + hr * 8 + g) / p.G;
+                hi[mt][hr] = p.causal ? min(s.length, s.start + i + 1) : s.length;
+                lo[mt][hr] = p.window > 0 ? s.start + i - p.window + 1 : 0;
+            }
+        }
+        {
+            const int i0 = row0 / p.G, i1 = (row0 + ROWS - 1) / p.G;
+            all_hi = p.causal ? min(s.length, s.start + i0 + 1) : s.length;
+            all_lo = p.window > 0 ? s.start + i1 - p.window + 1 : 0;
+        }
+        float acc[MT][D / 8][4], m[MT][2], l[MT][2], z[MT][2];       // z: 4 bits, what every column gains
+        #pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            #pragma unroll
+            for (int i = 0; i < D / 8; ++i) acc[mt][i][0] = acc[mt][i][1] = acc[mt][i][2] = acc[mt][i][3] = 0.f;
+            m[mt][0] = m[mt][1] = kNone;
+            l[mt][0] = l[mt][1] = z[mt][0] = z[mt][1] = 0.f;
+        }
+
+        #pragma unroll 1
+        for (int blk = seg.blk + warp; blk < seg.last; blk += kPagedWarps) {
+            copies_wait<NST - 2>();
+            __syncwarp();                                // every lane's copies are there, and the free slot is read
+            const uint32_t base = ring + slot * STAGE;
+            slot = slot + 1 == NST ? 0 : slot + 1;
+            copy_block();
+
+            // ---- scores -----------------------------------------------------------------------------------
+            float sc[MT][NT][4];
+            #pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                #pragma unroll
+                for (int i = 0; i < NT; ++i) sc[mt][i][0] = sc[mt][i][1] = sc[mt][i][2] = sc[mt][i][3] = 0.f;
+            }
+            if constexpr (BITS == 16) {
+                #pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    #pragma unroll
+                    for (int pr = 0; pr < NT / 2; ++pr) {
+                        const int r = pr * 16 + (lane / 16) * 8 + lane % 8, ch = 2 * ks + (lane / 8) % 2;
+                        uint32_t kf[4];
+                        ldsm4(base + r * CFG::ROW_BYTES + 16 * (ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3)), kf);
+                        #pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            mma16816<BF16>(sc[mt][2 * pr], qa[mt][ks], kf[0], kf[1]);
+                            mma16816<BF16>(sc[mt][2 * pr + 1], qa[mt][ks], kf[2], kf[3]);
+                        }
+                    }
+                }
+            } else {
+                // codes as 16-bit numbers 128 + c (bf16) or 1024 + c (fp16): one operation on a pair.  What the offset
+                // adds to a score, offset * q_sum, goes with the row's zero; in fp32 it costs 2^-24 * 1024 |q_sum| <
+                // 1e-3 of a step of the codes.
+                constexpr uint32_t kOffset = BF16 ? 0x43004300u : 0x64006400u;
+                constexpr float kOff = BF16 ? 128.f : 1024.f;
+                constexpr int NWD = D / 32;
+                #pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    uint32_t w[NWD];
+                    lds_words<NWD>(base + (8 * nt + g) * CFG::ROW_BYTES + 4 * NWD * t, w);
+                    #pragma unroll
+                    for (int j = 0; j < NWD; ++j) {
+                        #pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const uint32_t b0 = ((w[j] >> (8 * half)) & 0x000f000fu) | kOffset;
+                            const uint32_t b1 = ((w[j] >> (8 * half + 4)) & 0x000f000fu) | kOffset;
+                            #pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) mma16816<BF16>(sc[mt][nt], qa[mt][2 * j + half], b0, b1);
+                        }
+                    }
+                    uint32_t raw[4];                     // (scale, zero) of keys 2 t and 2 t + 1
+                    lds_words<4>(base + CFG::OFF_SK + 8 * (8 * nt + 2 * t), raw);
+                    #pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float scale = __uint_as_float(raw[2 * k]), add = fmaf(-kOff, scale, __uint_as_float(raw[2 * k + 1]));
+                        #pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            #pragma unroll
+                            for (int hr = 0; hr < 2; ++hr) sc[mt][nt][2 * hr + k] = fmaf(sc[mt][nt][2 * hr + k], scale, add * q_sum[mt][hr]);
+                        }
+                    }
+                }
+            }
+
+            // ---- softmax ----------------------------------------------------------------------------------
+            const int key0 = blk * KB;
+            const bool masked = key0 < all_lo || key0 + KB > all_hi;
+            if (masked) {
+                #pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    #pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        #pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + 8 * i + 2 * t + (e & 1);
+                            if (key < lo[mt][e >> 1] || key >= hi[mt][e >> 1]) sc[mt][i][e] = -INFINITY;
+                        }
+                    }
+                }
+            }
+            uint32_t pa[MT][NT / 2][4];                  // probabilities as the second product's operand
+            bool grow = false;
+            float mt_[MT][2];
+            #pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                #pragma unroll
+                for (int hr = 0; hr < 2; ++hr) {
+                    float v = fmaxf(sc[mt][0][2 * hr], sc[mt][0][2 * hr + 1]);
+                    #pragma unroll
+                    for (int i = 1; i < NT; ++i) v = fmaxf(v, fmaxf(sc[mt][i][2 * hr], sc[mt][i][2 * hr + 1]));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+                    mt_[mt][hr] = fmaxf(v * c_exp, kNone);           // (the scale is positive)
+                    grow = grow || mt_[mt][hr] > m[mt][hr] + 8.f;
+                }
+            }
+            // the reference moves only when the maximum has outgrown it by 2^8
+            if (__any_sync(0xffffffffu, grow)) {
+                #pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    #pragma unroll
+                    for (int hr = 0; hr < 2; ++hr) {
+                        const float ref = fmaxf(m[mt][hr], mt_[mt][hr]), f = exp2_ftz(m[mt][hr] - ref);
+                        m[mt][hr] = ref;
+                        l[mt][hr] *= f;
+                        if constexpr (BITS == 4) z[mt][hr] *= f;
+                        #pragma unroll
+                        for (int i = 0; i < D / 8; ++i) { acc[mt][i][2 * hr] *= f; acc[mt][i][2 * hr + 1] *= f; }
+                    }
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                uint32_t raw[4];                         // 4 bits: (scale, zero) of the values of keys 2 t, 2 t + 1
+                if constexpr (BITS == 4) lds_words<4>(base + CFG::OFF_SV + 8 * (8 * i + 2 * t), raw);
+                #pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    #pragma unroll
+                    for (int hr = 0; hr < 2; ++hr) {
+                        float pr[2];
+                        #pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            pr[k] = exp2_ftz(fmaf(sc[mt][i][2 * hr + k], c_exp, -m[mt][hr]));
+                            l[mt][hr] += pr[k];
+                            if constexpr (BITS == 4) {
+                                // value = scale (code - 8) + (zero + 8 scale): the first part goes through the product, with
+                                // the scale in the probability, the second is the same for every column.  Rounded to
+                                // bf16 in both types (2^-9, a sixtieth of what half a step of the codes is): a scale
+                                // may lie outside fp16.
+                                const float scale = __uint_as_float(raw[2 * k]), mid = fmaf(8.f, scale, __uint_as_float(raw[2 * k + 1]));
+                                if (!masked || pr[k] != 0.f) z[mt][hr] = fmaf(pr[k], mid, z[mt][hr]);
+                                pr[k] = !masked || pr[k] != 0.f ? pr[k] * scale : 0.f;
+                            }
+                        }
+                        pa[mt][i / 2][2 * (i % 2) + hr] = pack2<BITS == 4 ? true : BF16>(pr[0], pr[1]);
+                    }
+                }
+            }
+
+            // ---- values -----------------------------------------------------------------------------------
+            if constexpr (BITS == 16) {
+                #pragma unroll
+                for (int kk = 0; kk < NT / 2; ++kk) {
+                    #pragma unroll
+                    for (int dp = 0; dp < D / 16; ++dp) {
+                        const int r = kk * 16 + lane % 16, ch = 2 * dp + lane / 16;
+                        uint32_t vf[4];
+                        ldsm4_trans(base + CFG::OFF_V + r * CFG::ROW_BYTES + 16 * (ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3)), vf);
+                        #pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            mma16816<BF16>(acc[mt][2 * dp], pa[mt][kk], vf[0], vf[1]);
+                            mma16816<BF16>(acc[mt][2 * dp + 1], pa[mt][kk], vf[2], vf[3]);
+                        }
+                    }
+                }
+            } else {
+                // thread g holds words NWG g ... of a value row: column n of product (word, nibble) is element
+                // 8 (NWG n + word) + nibble.  (D = 32: four words, lanes 4 ... 7 take their upper nibbles.)
+                constexpr int NWG = D >= 64 ? D / 64 : 1, NIB = D >= 64 ? 8 : 4;
+                const __nv_bfloat162 k136 = __floats2bfloat162_rn(136.f, 136.f);
+                auto centred = [&](uint32_t x) {         // two codes as bf16 c - 8, exactly
+                    x = (x & 0x000f000fu) | 0x43004300u;
+                    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), k136);
+                    return *reinterpret_cast<const uint32_t*>(&y);
+                };
+                #pragma unroll
+                for (int kk = 0; kk < NT / 2; ++kk) {
+                    uint32_t w[4][NWG];
+                    #pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = kk * 16 + 2 * t + (k & 1) + 8 * (k >> 1);
+                        lds_words<NWG>(base + CFG::OFF_V + r * CFG::V_STRIDE + 4 * (D >= 64 ? NWG * g : g % 4), w[k]);
+                    }
+                    #pragma unroll
+                    for (int word = 0; word < NWG; ++word) {
+                        uint32_t x[2][2];                // [keys 2 t, or 2 t + 8][nibbles 0 ... 3, or 4 ... 7] of two keys
+                        #pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            x[k][0] = __byte_perm(w[2 * k][word], w[2 * k + 1][word], 0x5410);
+                            x[k][1] = __byte_perm(w[2 * k][word], w[2 * k + 1][word], 0x7632);
+                            if (D == 32 && g >= 4) x[k][0] = x[k][1];
+                        }
+                        #pragma unroll
+                        for (int i = 0; i < NIB; ++i) {
+                            const uint32_t b0 = centred(x[0][i / 4] >> (4 * (i % 4))), b1 = centred(x[1][i / 4] >> (4 * (i % 4)));
+                            #pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) mma16816<true>(acc[mt][word * NIB + i], pa[mt][kk], b0, b1);
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- the four warps' parts, through their free ring slots, 16 rows at a time -----------------------
+        // the element that column n (0 ... 7) of accumulator tile i stands for
+        auto column = [&](int i, int n) {
+            if constexpr (BITS == 16) return 8 * i + n;
+            else if constexpr (D >= 64) return 8 * ((D / 64) * n + i / 8) + i % 8;
+            else return 8 * (n % 4) + 4 * (n / 4) + i;
+        };
+        constexpr int EXC = CFG::EX_COLS;
+        __syncwarp();                                    // (the slot that is free now was read last)
+        #pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            if (mt > 0) __syncthreads();
+            #pragma unroll
+            for (int hr = 0; hr < 2; ++hr) {
+                float sum = l[mt][hr], zs = z[mt][hr];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if constexpr (BITS == 4) {
+                    zs += __shfl_xor_sync(0xffffffffu, zs, 1);
+                    z[mt][hr] = zs + __shfl_xor_sync(0xffffffffu, zs, 2);
+                }
+                if (t == 0) { sm_m[warp * 16 + hr * 8 + g] = m[mt][hr]; sm_l[warp * 16 + hr * 8 + g] = sum; }
+            }
+            if (lane == 0) sm_slot[warp] = (warp * NST + fill) * STAGE;
+            #pragma unroll
+            for (int part = 0; part < D / EXC; ++part) {
+                if (part > 0) __syncthreads();
+                float* mine = reinterpret_cast<float*>(paged_smem + (warp * NST + fill) * STAGE);
+                #pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = g + 8 * (e >> 1), col = column(i, 2 * t + (e & 1)) - part * EXC;
+                        if (EXC == D || (col >= 0 && col < EXC))
+                            mine[r * EXC + (col ^ ((r & 3) << 3))] = acc[mt][i][e] + (BITS == 4 ? z[mt][e >> 1] : 0.f);
+                    }
+                }
+                __syncthreads();
+                #pragma unroll 1
+                for (int id = tid; id < 16 * EXC / 4; id += kPagedThreads) {
+                    const int r = id / (EXC / 4), col = (id % (EXC / 4)) * 4, row = row0 + mt * 16 + r;
+                    if (row >= R) continue;
+                    float ref = sm_m[r];
+                    #pragma unroll
+                    for (int w = 1; w < kPagedWarps; ++w) ref = fmaxf(ref, sm_m[w * 16 + r]);
+                    float sum = 0.f;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    #pragma unroll
+                    for (int w = 0; w < kPagedWarps; ++w) {
+                        const float f = exp2_ftz(sm_m[w * 16 + r] - ref);
+                        const float4 x = *reinterpret_cast<const float4*>(paged_smem + sm_slot[w] + 4 * (r * EXC + (col ^ ((r & 3) << 3))));
+                        sum = fmaf(f, sm_l[w * 16 + r], sum);
+                        v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
+                    }
+                    const int i = row / p.G, h = seg.kv_head * p.G + row % p.G;
+                    if (i >= s.count) sum = 0.f;         // a row behind the sequence's new tokens
+                    if (seg.whole) {
+                        const float inv = sum == 0.f ? 0.f : 1.f / sum;      // (a row without keys is zero; NaN stays NaN)
+                        uint2 o = make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
+                        if (sum == 0.f) o = make_uint2(0, 0);
+                        *reinterpret_cast<uint2*>(p.out + (((long long)seg.b * p.Hq + h) * p.N + i) * D + part * EXC + col) = o;
+                    } else {
+                        const long long at = (2LL * blockIdx.x + (seg.begins ? 1 : 0)) * ROWS + mt * 16 + r;
+                        *reinterpret_cast<float4*>(p.part_acc + at * D + part * EXC + col) = v;
+                        if (part == 0 && col == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(ref, sum);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Adds the parts of the items that paged_kernel divided, and writes the zeros of those without keys.  One warp per query row.
+template <int D, int MT, bool BF16, int BITS>
+__global__ void __launch_bounds__(kPagedThreads) combine_kernel(const __grid_constant__ PagedParams p) {
+    using CFG = PagedConfig<D, MT, BITS>;
+    constexpr int KB = CFG::KB, ROWS = CFG::ROWS, LPR = D / 4, PER = 32 / LPR;   // lanes of a row; parts taken at a time
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int per = p.Hkv * p.groups, b = blockIdx.x / per, item = blockIdx.x % per;
+    const int r = blockIdx.y * kPagedWarps + warp, row = (item % p.groups) * ROWS + r;
+    const bool row_ok = row < p.N * p.G;
+    // (lengths are inputs: they were there before paged_kernel started)
+    long long before = 0, total = 0;
+    for (int i = lane; i < p.seq.B; i += 32) {
+        const int n = blocks_of<KB>(p, i).n;
+        total += n;
+        if (i < b) before += n;
+    }
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    total *= per;
+    const int n = blocks_of<KB>(p, b).n, parts = line_parts(p, total);
+    const long long first = before * per + (long long)item * n;
+    const int col = (lane % LPR) * 4;
+    uint16_t* out = p.out + (((long long)b * p.Hq + (item / p.groups) * p.G + row % p.G) * p.N + row / p.G) * D + col;
+    int c0 = 0, c1 = 0;                                  // the CTAs that have its blocks
+    if (n > 0) {
+        auto holder = [&](long long at) {
+            int c = static_cast<int>(min((long long)parts - 1, at * parts / total));
+            while (cut(total, parts, c) > at) --c;
+            while (cut(total, parts, c + 1) <= at) ++c;
+            return c;
+        };
+        c0 = holder(first);
+        c1 = holder(first + n - 1);
+    }
+    // (every CTA waits: this grid must not end, and let the stream go on, before paged_kernel has)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!row_ok || (n > 0 && c0 == c1)) return;          // no row, or finished in paged_kernel
+    if (n == 0) {
+        if (lane < LPR) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
+        return;
+    }
+    // slot 1 of the CTA where the item begins, slot 0 of those where it goes on
+    auto slot = [&](int c) { return (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r; };
+    float ref = -1e30f, sum = 0.f;
+    for (int c = c0 + lane; c <= c1; c += 32) ref = fmaxf(ref, __ldcg(p.part_ml + 2 * slot(c)));
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    #pragma unroll 8
+    for (int c = c0 + lane / LPR; c <= c1; c += PER) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot(c)));
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_acc + slot(c) * D + col));
+        const float f = exp2_ftz(ml.x - ref);
+        sum = fmaf(f, ml.y, sum);
+        v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
+    }
+    #pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        v.z += __shfl_xor_sync(0xffffffffu, v.z, o); v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
+    }
+    if (lane < LPR) {
+        const float inv = 1.f / sum;
+        uint2 o = make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
+        if (sum == 0.f) o = make_uint2(0, 0);
+        *reinterpret_cast<uint2*>(out) = o;
+    }
+}
+
+}  // namespace bob

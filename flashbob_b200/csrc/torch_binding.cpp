@@ -21,7 +21,9 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <array>
 #include <cmath>
+#include <cstring>
 #include <optional>
 
 namespace {
@@ -40,6 +42,11 @@ struct Library {
     decltype(&bob_sm100_read_status) read_status = nullptr;
     decltype(&bob_sm100_last_status) last_status = nullptr;
     decltype(&bob_sm100_error_string) error_string = nullptr;
+    decltype(&bob_sm100_rotate) rotate = nullptr;
+    decltype(&bob_sm100_cache_append) cache_append = nullptr;
+    decltype(&bob_sm100_cache_read) cache_read = nullptr;
+    decltype(&bob_sm100_paged_workspace_bytes) paged_workspace_bytes = nullptr;
+    decltype(&bob_sm100_paged_fwd) paged_fwd = nullptr;
 };
 Library lib;
 PyObject* error_class = nullptr;           // BobSm100Error
@@ -253,6 +260,163 @@ Tensor sdpa(const Tensor& q, const Tensor& k, const Tensor& v, const Mask& m) {
     return r.out;
 }
 
+// ---- rotary positions -------------------------------------------------------------------------------
+// The kernels for positions and the paged cache read any layout with unit stride along the head dim, strides that are
+// multiples of 8 elements (zero for an expanded tensor) and a 16-byte aligned base.
+Tensor tokens_ready(const Tensor& t) {
+    bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0 && t.stride(i) >= 0;
+    return ok ? t : t.contiguous();
+}
+
+int32_t dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? BOB_SM100_BF16 : BOB_SM100_FP16; }
+
+// As finish(), for calls whose kernels report to the device's word only.
+void finish_reported(int rc, const char* what, int device, bool check_status) {
+    if (rc) fail(what, rc);
+    if (check_status) c10::cuda::getCurrentCUDAStream(device).synchronize();
+    if ((rc = lib.last_status(device)))
+        fail((check_status ? std::string(what) + " (device status)" : "an earlier libbob_sm100 kernel on cuda:" + std::to_string(device) +
+              " (seen after " + what + "; its results are undefined)"), rc);
+}
+
+struct Rotation {
+    bob_sm100_rotary rotary = {};
+    int64_t first = 0;
+    bool inverse = false, check_status = false;
+};
+
+// x[0] and x[1] [B, H, N, D], of which one may be undefined, turned to their positions (undefined: first + row).
+std::array<Tensor, 2> run_rotate(const std::array<Tensor, 2>& x, const Tensor& positions, const Rotation& r) {
+    bob_sm100_rotate_args a = {};
+    std::array<Tensor, 2> in, out;
+    int n = 0, device = 0;
+    for (int i = 0; i < 2; ++i) {
+        if (!x[i].defined()) continue;
+        in[i] = tokens_ready(x[i]);
+        out[i] = empty(in[i].sizes(), in[i].scalar_type(), in[i]);
+        a.B = static_cast<int32_t>(in[i].size(0)); a.N = static_cast<int32_t>(in[i].size(2)); a.D = static_cast<int32_t>(in[i].size(3));
+        a.dtype = dtype_of(in[i]);
+        a.device = device = in[i].device().index();
+        a.heads[n] = static_cast<int32_t>(in[i].size(1));
+        a.in[n] = ptr(in[i]);
+        a.out[n] = ptr(out[i]);
+        set_strides(a.in_strides[n++], in[i]);
+    }
+    if (positions.defined()) {                   // [N] or [B, N]
+        a.positions = ptr(positions);
+        a.position_bits = positions.scalar_type() == at::kLong ? 64 : 32;
+        a.position_strides[0] = positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
+        a.position_strides[1] = positions.stride(-1);
+    }
+    a.first = r.first;
+    a.inverse = r.inverse;
+    a.rotary = r.rotary;
+    const int rc = lib.rotate(&a, c10::cuda::getCurrentCUDAStream(device).stream());
+    finish_reported(rc, "bob_sm100_rotate", device, r.check_status);
+    return out;
+}
+
+std::array<Tensor, 2> rotate(const std::array<Tensor, 2>& x, const Tensor& positions, const Rotation& r);
+
+// The gradient of a rotation is the rotation back, recorded like any other: differentiable any number of times.
+struct RotateNode : Node {
+    Rotation rotation;
+    SavedVariable positions;
+    bool has[2] = {false, false};
+    std::string name() const override { return "RotaryBackward"; }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        std::array<Tensor, 2> u;
+        for (int i = 0, n = 0; i < 2; ++i)
+            if (has[i]) u[i] = grads[n++];
+        if (!u[0].defined() && !u[1].defined()) return variable_list(2);
+        for (const Tensor& t : u)
+            TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "forward-mode AD is unsupported; differentiate with "
+                                        "reverse mode (torch.autograd.grad twice) instead");
+        Rotation back = rotation;
+        back.inverse = !back.inverse;
+        std::array<Tensor, 2> g = rotate(u, positions.unpack(), back);
+        return {g[0], g[1]};
+    }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        positions.reset_data();
+    }
+};
+
+std::array<Tensor, 2> rotate(const std::array<Tensor, 2>& x, const Tensor& positions, const Rotation& r) {
+    std::array<Tensor, 2> y;
+    {
+        Untracked untracked;
+        const c10::cuda::CUDAGuard device((x[0].defined() ? x[0] : x[1]).device());
+        y = run_rotate(x, positions, r);
+    }
+    if (torch::autograd::compute_requires_grad(x[0], x[1])) {
+        auto node = make_node<RotateNode>();
+        node->set_next_edges(torch::autograd::collect_next_edges(x[0], x[1]));
+        node->rotation = r;
+        node->positions = SavedVariable(positions, false);
+        for (int i = 0; i < 2; ++i) {
+            node->has[i] = y[i].defined();
+            if (y[i].defined()) torch::autograd::set_history(y[i], node);
+        }
+    }
+    return y;
+}
+
+// ---- paged cache ------------------------------------------------------------------------------------
+struct Cache {
+    Tensor data[2], scales[2];
+    bob_sm100_cache c = {};
+};
+struct Sequences {
+    Tensor table, lengths, counts;
+    bob_sm100_sequences s = {};
+};
+
+void run_append(const Tensor& k_, const Tensor& v_, Cache& cache, const Sequences& seq, const bob_sm100_rotary& rotary, bool check_status) {
+    const Tensor k = tokens_ready(k_), v = tokens_ready(v_);
+    int64_t ks[3], vs[3];
+    set_strides(ks, k);
+    set_strides(vs, v);
+    const int rc = lib.cache_append(&cache.c, &seq.s, &rotary, static_cast<int>(k.size(2)), ptr(k), ks, ptr(v), vs, stream_of(k));
+    for (int i = 0; i < 2; ++i) {                // (written to: what autograd has saved of them is stale)
+        cache.data[i].unsafeGetTensorImpl()->bump_version();
+        if (cache.scales[i].defined()) cache.scales[i].unsafeGetTensorImpl()->bump_version();
+    }
+    finish_reported(rc, "bob_sm100_cache_append", cache.c.device, check_status);
+}
+
+std::array<Tensor, 2> run_read(const Cache& cache, const Sequences& seq, int64_t n, at::ScalarType type, bool check_status) {
+    const std::array<int64_t, 4> size{seq.s.B, cache.c.heads, n, cache.c.D};
+    std::array<Tensor, 2> out{empty(size, type, cache.data[0]), empty(size, type, cache.data[0])};
+    const int rc = lib.cache_read(&cache.c, &seq.s, static_cast<int>(n), ptr(out[0]), ptr(out[1]), stream_of(out[0]));
+    finish_reported(rc, "bob_sm100_cache_read", cache.c.device, check_status);
+    return out;
+}
+
+Tensor run_paged(const Tensor& q_, const Cache& cache, const Sequences& seq, const bob_sm100_rotary& rotary, bool causal, int64_t window,
+                 std::optional<double> scale, bool check_status) {
+    const Tensor q = tokens_ready(q_);
+    const Tensor out = empty(q.sizes(), q.scalar_type(), q);
+    bob_sm100_paged_args a = {};
+    a.cache = cache.c;
+    a.seq = seq.s;
+    a.rotary = rotary;
+    a.Hq = static_cast<int32_t>(q.size(1)); a.N = static_cast<int32_t>(q.size(2));
+    a.is_causal = causal;
+    a.window = static_cast<int32_t>(window);
+    a.q = ptr(q);
+    set_strides(a.q_strides, q);
+    a.out = ptr(out);
+    a.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(q.size(3))));
+    const Tensor ws = empty({static_cast<int64_t>(lib.paged_workspace_bytes(&a))}, at::kByte, q);
+    const int rc = lib.paged_fwd(&a, ptr(ws), stream_of(q));
+    finish_reported(rc, "bob_sm100_paged_fwd", cache.c.device, check_status);
+    return out;
+}
+
 // ---- Python entry points ----------------------------------------------------------------------------
 bool is_int(PyObject* o) { return PyLong_CheckExact(o); }       // a bool is a subclass: not exact
 
@@ -411,10 +575,130 @@ PyObject* py_second(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(error class, addresses of fwd, bwd1, bwd2, workspace_bytes, read_status, last_status, error_string)
+// The bytes of a bob_sm100_rotary; None: no rotation.
+bob_sm100_rotary rotary_arg(PyObject* o) {
+    bob_sm100_rotary r = {};
+    if (o == Py_None) return r;
+    char* data = nullptr;
+    Py_ssize_t size = 0;
+    if (PyBytes_AsStringAndSize(o, &data, &size)) throw python_error();
+    if (size != static_cast<Py_ssize_t>(sizeof(r))) throw torch::TypeError("a rotation is " + std::to_string(sizeof(r)) + " bytes");
+    std::memcpy(&r, data, sizeof(r));
+    return r;
+}
+
+// (keys, values, key scales or None, value scales or None, 16-bit type of the rows), checked by the caller
+Cache cache_args(PyObject* const* a) {
+    Cache r;
+    bob_sm100_cache& c = r.c;
+    for (int i = 0; i < 2; ++i) {
+        const Tensor& t = r.data[i] = tensor_arg(a[i]);
+        const int64_t size = t.element_size();
+        c.data[i] = ptr(t);
+        for (int k = 0; k < 3; ++k) c.strides[i][k] = t.stride(k) * size;
+        r.scales[i] = optional_tensor_arg(a[2 + i]);
+        c.scales[i] = ptr(r.scales[i]);
+        if (r.scales[i].defined())
+            for (int k = 0; k < 3; ++k) c.scale_strides[i][k] = r.scales[i].stride(k) * 4;
+    }
+    const Tensor& k = r.data[0];
+    c.bits = r.scales[0].defined() ? 4 : 16;
+    c.pages = static_cast<int32_t>(k.size(0)); c.heads = static_cast<int32_t>(k.size(1)); c.page_size = static_cast<int32_t>(k.size(2));
+    c.D = static_cast<int32_t>(k.size(3)) * (c.bits == 4 ? 2 : 1);
+    c.dtype = PyObject_IsTrue(a[4]) ? BOB_SM100_BF16 : BOB_SM100_FP16;
+    c.device = k.device().index();
+    return r;
+}
+
+// (page table, lengths, counts or None), checked by the caller
+Sequences sequence_args(PyObject* const* a) {
+    Sequences r;
+    r.table = tensor_arg(a[0]);
+    if (r.table.stride(1) != 1) r.table = r.table.contiguous();
+    r.lengths = tensor_arg(a[1]).contiguous();
+    r.counts = optional_tensor_arg(a[2]);
+    if (r.counts.defined()) r.counts = r.counts.contiguous();
+    r.s.B = static_cast<int32_t>(r.table.size(0)); r.s.max_pages = static_cast<int32_t>(r.table.size(1));
+    r.s.table = static_cast<const int32_t*>(ptr(r.table));
+    r.s.table_stride = r.table.stride(0);
+    r.s.lengths = static_cast<const int32_t*>(ptr(r.lengths));
+    r.s.counts = static_cast<const int32_t*>(ptr(r.counts));
+    return r;
+}
+
+// rotate(q, k or None, rotary, positions or None, first, check_status) -> (q, k)
+PyObject* py_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    want(n, 6);
+    const std::array<Tensor, 2> x{tensor_arg(a[0]), optional_tensor_arg(a[1])};
+    Rotation r;
+    r.rotary = rotary_arg(a[2]);
+    const Tensor positions = optional_tensor_arg(a[3]);
+    r.first = int_arg(a[4]);
+    r.check_status = PyObject_IsTrue(a[5]);
+    const std::array<Tensor, 2> y = without_gil([&] { return rotate(x, positions, r); });
+    return tuple_of({y[0], y[1]});
+    END_HANDLE_TH_ERRORS
+}
+
+// cache_append(k, v, <cache>, <sequences>, rotary or None, check_status)
+PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    want(n, 12);
+    Untracked untracked;
+    const Tensor &k = tensor_arg(a[0]), &v = tensor_arg(a[1]);
+    const c10::cuda::CUDAGuard device(k.device());
+    Cache cache = cache_args(a + 2);
+    const Sequences seq = sequence_args(a + 7);
+    const bob_sm100_rotary rotary = rotary_arg(a[10]);
+    const bool check = PyObject_IsTrue(a[11]);
+    without_gil([&] { run_append(k, v, cache, seq, rotary, check); return 0; });
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// cache_read(<cache>, <sequences>, n, check_status) -> (k, v)
+PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    want(n, 10);
+    Untracked untracked;
+    const c10::cuda::CUDAGuard device(tensor_arg(a[0]).device());
+    const Cache cache = cache_args(a);
+    const Sequences seq = sequence_args(a + 5);
+    const int64_t rows = int_arg(a[8]);
+    const bool check = PyObject_IsTrue(a[9]);
+    const std::array<Tensor, 2> r =
+        without_gil([&] { return run_read(cache, seq, rows, cache.c.dtype == BOB_SM100_BF16 ? at::kBFloat16 : at::kHalf, check); });
+    return tuple_of({r[0], r[1]});
+    END_HANDLE_TH_ERRORS
+}
+
+// paged(q, <cache>, <sequences>, rotary or None, is_causal, window_size, scale or None, check_status) -> out
+PyObject* py_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    want(n, 14);
+    Untracked untracked;
+    const Tensor& q = tensor_arg(a[0]);
+    const c10::cuda::CUDAGuard device(q.device());
+    const Cache cache = cache_args(a + 1);
+    const Sequences seq = sequence_args(a + 6);
+    const bob_sm100_rotary rotary = rotary_arg(a[9]);
+    const bool causal = PyObject_IsTrue(a[10]), check = PyObject_IsTrue(a[13]);
+    const int64_t window = int_arg(a[11]);
+    std::optional<double> scale;
+    if (a[12] != Py_None) {
+        scale = PyFloat_AsDouble(a[12]);
+        if (PyErr_Occurred()) throw python_error();
+    }
+    return THPVariable_Wrap(without_gil([&] { return run_paged(q, cache, seq, rotary, causal, window, scale, check); }));
+    END_HANDLE_TH_ERRORS
+}
+
+// bind(error class, addresses of fwd, bwd1, bwd2, workspace_bytes, read_status, last_status, error_string, rotate,
+// cache_append, cache_read, paged_workspace_bytes, paged_fwd)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    want(n, 8);
+    want(n, 13);
     auto address = [&](int i) { return reinterpret_cast<void*>(int_arg(a[i])); };
     Py_INCREF(a[0]);
     error_class = a[0];
@@ -425,6 +709,11 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     lib.read_status = reinterpret_cast<decltype(lib.read_status)>(address(5));
     lib.last_status = reinterpret_cast<decltype(lib.last_status)>(address(6));
     lib.error_string = reinterpret_cast<decltype(lib.error_string)>(address(7));
+    lib.rotate = reinterpret_cast<decltype(lib.rotate)>(address(8));
+    lib.cache_append = reinterpret_cast<decltype(lib.cache_append)>(address(9));
+    lib.cache_read = reinterpret_cast<decltype(lib.cache_read)>(address(10));
+    lib.paged_workspace_bytes = reinterpret_cast<decltype(lib.paged_workspace_bytes)>(address(11));
+    lib.paged_fwd = reinterpret_cast<decltype(lib.paged_fwd)>(address(12));
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -433,6 +722,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     BOB_METHOD("try_sdpa", py_try_sdpa), BOB_METHOD("sdpa", py_sdpa), BOB_METHOD("forward", py_forward),
     BOB_METHOD("first_backward", py_first), BOB_METHOD("second_backward", py_second), BOB_METHOD("bind", py_bind),
+    BOB_METHOD("rotate", py_rotate), BOB_METHOD("cache_append", py_append), BOB_METHOD("cache_read", py_read), BOB_METHOD("paged", py_paged),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "bob_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

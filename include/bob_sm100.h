@@ -155,6 +155,89 @@ int bob_sm100_bwd2_noalloc(const bob_sm100_geom* geom, const void* q, const void
  * bob_sm100_read_status, hence this reader.  Allocates nothing. */
 int bob_sm100_noalloc_read_status(int device, void* stream);
 
+/* ---- positions, a paged cache and attention over it (no counterpart in the reference) ------------------------
+ *
+ * Tensors of tokens are [B, H, N, D] as above (element strides of batch, head and row; unit stride along D; multiples of
+ * 8; 16-byte aligned), with D = 32, 64 or 128.  These entry points allocate nothing, wait for nothing and can be
+ * captured.  What only the GPU knows (page table, lengths, counts) is checked there: an entry outside the cache or a
+ * length or count out of range sets the device's status word (bob_sm100_last_status), and the rows that it
+ * concerns are neither read nor written. */
+
+/* Rotary positions: pair i turns elements (i, i + pairs), interleaved (2 i, 2 i + 1), by position * turns[i] / 2^64
+ * turns, and is multiplied by factor; elements from 2 * pairs on are left alone.  pairs = 0: no rotation. */
+typedef struct bob_sm100_rotary {
+    int32_t pairs;        /* at most D / 2 */
+    int32_t interleaved;
+    double factor;
+    uint64_t turns[64];
+} bob_sm100_rotary;
+
+/* One or two tensors (heads[1] = 0: one) turned to their positions.  inverse: the angles negated, which is the gradient.
+ * Row n of batch b sits at positions[b * position_strides[0] + n * position_strides[1]] (position_bits 32 or 64), or
+ * at first + n where positions is NULL.  Results are contiguous. */
+typedef struct bob_sm100_rotate_args {
+    int32_t B, N, D, dtype, device;
+    int32_t heads[2];
+    int32_t inverse;
+    const void* in[2];
+    int64_t in_strides[2][3];
+    void* out[2];
+    const void* positions;
+    int64_t position_strides[2];
+    int64_t first;
+    int32_t position_bits;
+    int32_t reserved;
+    bob_sm100_rotary rotary;
+} bob_sm100_rotate_args;
+
+/* A cache of pages: [pages, heads, page_size, D] keys and values.  bits 16: dtype elements.  bits 4: bytes of two codes
+ * (element 2 j in the low half of byte j) and fp32 (scale, zero) per row, value = code * scale + zero.  Byte strides of
+ * page, head and row: multiples of 16, for scales of 8; rows have unit stride, and addresses are 16-byte
+ * aligned (scales 8).  page_size is a power of two from 16 to 4096. */
+typedef struct bob_sm100_cache {
+    int32_t pages, heads, page_size, D, dtype, bits, device;
+    int32_t reserved;
+    void* data[2];        /* keys, values */
+    int64_t strides[2][3];
+    void* scales[2];
+    int64_t scale_strides[2][3];
+} bob_sm100_cache;
+
+/* B sequences: position t of sequence b is row t % page_size of page table[b * table_stride + t / page_size];
+ * lengths[b] positions are there with the new ones, the last counts[b] (NULL: all N rows of the call) are new. */
+typedef struct bob_sm100_sequences {
+    int32_t B, max_pages;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    const int32_t* counts;
+} bob_sm100_sequences;
+
+/* Attention over a cache: query i of sequence b sits at lengths[b] - counts[b] + i and is turned to that position first.
+ * out is contiguous [B, Hq, N, D]; rows from counts[b] on, and rows without keys, are zero.  workspace_bytes is known
+ * from these arguments alone (not from lengths). */
+typedef struct bob_sm100_paged_args {
+    bob_sm100_cache cache;
+    bob_sm100_sequences seq;
+    bob_sm100_rotary rotary;
+    int32_t Hq, N;
+    int32_t is_causal, window;
+    const void* q;
+    int64_t q_strides[3];
+    void* out;
+    float scale;
+    int32_t reserved;
+} bob_sm100_paged_args;
+
+int bob_sm100_rotate(const bob_sm100_rotate_args* args, void* stream);
+/* Rows 0 ... counts[b] - 1 of k and v (heads of the cache, N rows) into the pages; k is turned to its positions. */
+int bob_sm100_cache_append(const bob_sm100_cache* cache, const bob_sm100_sequences* seq, const bob_sm100_rotary* rotary, int N,
+                           const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, void* stream);
+/* Positions 0 ... n - 1 of every sequence into contiguous [B, heads, n, D] k and v; rows from lengths[b] on are zero. */
+int bob_sm100_cache_read(const bob_sm100_cache* cache, const bob_sm100_sequences* seq, int n, void* k, void* v, void* stream);
+size_t bob_sm100_paged_workspace_bytes(const bob_sm100_paged_args* args);
+int bob_sm100_paged_fwd(const bob_sm100_paged_args* args, void* workspace, void* stream);
+
 /* Known-answer check of the tensor-core plumbing: a [128,64] x b [64,64] (same 16-bit format).
  * out is fp32 [8,128,64]: out[0] = a b^T; out[1] = a b; out[2] = a b^T with a staged through
  * thread-written swizzled shared memory; out[3], out[4] = the two halves of one 128-wide product
