@@ -19,7 +19,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libbob_sm100.so"
 TORCH_MODULE = PKG / "bob_torch.so"
 SOURCES = ("api.cu", "selftest.cu", "noalloc.cu", "paged.cu")
-HEADERS = ("ptx.cuh", "sweep.cuh", "decode.cuh", "tmap.h", "internal.h", "rotary.cuh", "cache.cuh", "paged.cuh")
+HEADERS = ("ptx.cuh", "sequence.cuh", "sweep.cuh", "decode.cuh", "tmap.h", "internal.h", "rotary.cuh", "cache.cuh", "paged.cuh")
 
 
 def _nvcc() -> str:

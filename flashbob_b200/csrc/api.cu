@@ -116,6 +116,8 @@ static int launch_sweep(const bob_sm100_geom* g, SweepParams& prm, const TensorA
         if (!a.ptr) return 0;
         int rc = check_strides(a.strides, a.ptr);
         if (rc) return rc;
+        if (MODE == kFwdPaged && !a.q_side)      // [pages, Hkv, page_size, D]
+            return make_tile_map(&prm.map[t], a.ptr, kType, g->D, 1 << prm.seq.page_shift, g->Hkv, prm.seq.pages, a.strides[2], a.strides[1], a.strides[0], prm.box_rows);
         return make_tile_map(&prm.map[t], a.ptr, kType, g->D, a.q_side ? g->Nq : g->Nk,
                              a.q_side ? g->Hq : g->Hkv, g->B, a.strides[2], a.strides[1],
                              a.strides[0], box_rows);
@@ -176,11 +178,11 @@ static int dispatch(const bob_sm100_geom* g, SweepParams& prm, const TensorArg* 
     constexpr bool kSecond = (MODE == kBwd2Row || MODE == kBwd2Col);
     if (g->D <= 64) {
         if constexpr (kSecond)           return launch_sweep<MODE, 64, 64, BF16, 1, 32, false>(g, prm, tensors, stream, counter_slot);
-        else if constexpr (MODE == kFwd) return launch_sweep<MODE, 64, 128, BF16, 2, 128, false>(g, prm, tensors, stream, counter_slot);
+        else if constexpr (is_forward(MODE)) return launch_sweep<MODE, 64, 128, BF16, 2, 128, false>(g, prm, tensors, stream, counter_slot);
         else                             return launch_sweep<MODE, 64, 64, BF16, 2, 32, false>(g, prm, tensors, stream, counter_slot);
     }
     if constexpr (kSecond)           return launch_sweep<MODE, 128, 32, BF16, 1, 16, false>(g, prm, tensors, stream, counter_slot);
-    else if constexpr (MODE == kFwd) return launch_sweep<MODE, 128, 128, BF16, 2, 128, true>(g, prm, tensors, stream, counter_slot);
+    else if constexpr (is_forward(MODE)) return launch_sweep<MODE, 128, 128, BF16, 2, 128, true>(g, prm, tensors, stream, counter_slot);
     else                             return launch_sweep<MODE, 128, 64, BF16, 2, 32, true>(g, prm, tensors, stream, counter_slot);
 }
 
@@ -455,6 +457,34 @@ extern "C" int bob_sm100_fwd(const bob_sm100_geom* g, const void* q, const void*
     t[kTK] = {k, g->k_strides, false};
     t[kTV] = {v, g->v_strides, false};
     return dispatch_dtype<kFwd>(g, p, t, s, 0);
+}
+
+// Forward over a paged cache for many query rows; `q` and its strides may be those of turned queries in the workspace.
+int bob::sweep_paged(const bob_sm100_paged_args* a, const SequenceParams& seq, const void* q, const int64_t* q_strides, void* workspace, cudaStream_t s) {
+    int rc = begin_call(workspace, s);
+    if (rc) return rc;
+    const bob_sm100_cache& c = a->cache;
+    bob_sm100_geom g = {};
+    g.B = seq.B; g.Hq = a->Hq; g.Hkv = c.heads; g.Nq = a->N; g.Nk = 1; g.D = c.D;       // (every sequence has its own length)
+    g.dtype = c.dtype;
+    g.is_causal = a->is_causal;
+    g.device = c.device;
+    g.scale = a->scale;
+    SweepParams p;
+    fill_common(&g, p, workspace);
+    p.window = std::min(a->window, 1 << 28);
+    p.sticky = seq.sticky;
+    p.seq = seq;
+    p.box_rows = std::min(c.page_size, 128);
+    p.res0 = a->out;
+    int64_t strides[2][3];
+    for (int w = 0; w < 2; ++w)
+        for (int i = 0; i < 3; ++i) strides[w][i] = c.strides[w][i] / 2;
+    TensorArg t[kNumTensors] = {};
+    t[kTQ] = {q, q_strides, true};
+    t[kTK] = {c.data[0], strides[0], false};
+    t[kTV] = {c.data[1], strides[1], false};
+    return dispatch_dtype<kFwdPaged>(&g, p, t, s, 0);
 }
 
 extern "C" int bob_sm100_bwd1(const bob_sm100_geom* g, const void* q, const void* k, const void* v,

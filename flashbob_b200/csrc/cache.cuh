@@ -13,41 +13,9 @@
 #pragma once
 
 #include "rotary.cuh"
+#include "sequence.cuh"
 
 namespace bob {
-
-enum : int { kStatusBadPage = 21, kStatusBadLength = 22 };
-
-struct SequenceParams {
-    const int* table; long long table_stride;
-    const int* lengths;
-    const int* counts;            // null: every row of the call
-    int B, max_pages, pages, page_shift;
-    int* sticky;                  // host-visible status word (may be null)
-};
-
-__device__ __forceinline__ void report(int* sticky, int code) {
-    if (sticky) { *reinterpret_cast<volatile int*>(sticky) = code; __threadfence_system(); }
-}
-
-struct Sequence { int length, count, start; bool ok; };          // start: position of row 0, negative only if not ok
-
-__device__ __forceinline__ Sequence sequence_of(const SequenceParams& p, int b, int N) {
-    Sequence s;
-    const int length = __ldg(p.lengths + b), count = p.counts ? __ldg(p.counts + b) : N;
-    const long long room = (long long)p.max_pages << p.page_shift;
-    s.length = static_cast<int>(min(max((long long)length, 0LL), room));
-    s.count = min(max(count, 0), N);
-    s.start = s.length - s.count;
-    s.ok = length == s.length && count == s.count && s.start >= 0;
-    return s;
-}
-
-// The page of a position below its sequence's length; -1 if the table's entry is no page.
-__device__ __forceinline__ int page_of(const SequenceParams& p, int b, int position) {
-    const int page = __ldg(p.table + b * p.table_stride + (position >> p.page_shift));
-    return static_cast<unsigned>(page) < static_cast<unsigned>(p.pages) ? page : -1;
-}
 
 struct CacheTensor {
     uint8_t* data; long long sp, sh, sr;                         // byte strides: page, head, row

@@ -2,6 +2,9 @@
 #pragma once
 
 #include "../../include/bob_sm100.h"
+#include "sequence.cuh"
+
+#include <cuda_runtime.h>
 
 namespace bob {
 
@@ -14,6 +17,10 @@ int bwd2_impl(const bob_sm100_geom* g, const void* q, const void* k, const void*
               const float* lse, const float* delta, const float* pk, const void* dO, const void* dQ,
               const void* uQ, const void* uK, const void* uV, void* Qbar, void* Kbar, void* Vbar,
               void* dObar, void* workspace, void* stream, int* sticky, int part);
+
+// Forward over a 16-bit paged cache through the kernel for many rows (arguments checked, the device is current): clears the
+// workspace's status block, which is all of the workspace that it uses.
+int sweep_paged(const bob_sm100_paged_args* a, const SequenceParams& seq, const void* q, const int64_t* q_strides, void* workspace, cudaStream_t stream);
 
 // The per-device host-visible status word: its device address (create = true: page-locks it on first
 // use; null if that failed) or its host address (create = false; null before first use).

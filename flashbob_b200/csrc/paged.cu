@@ -100,8 +100,9 @@ template <class F> static void with_type(int dtype, F f) {
 // shares its sines and cosines between them.
 constexpr int64_t kManyThreads = (int64_t)kPagedSms * 2048;
 
-static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream) {
+static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream, const int* lengths = nullptr, const int* counts = nullptr) {
     RotateParams p = {};
+    p.lengths = lengths; p.counts = counts;
     p.rotary = a->rotary;
     if (a->inverse)
         for (uint64_t& x : p.rotary.turns) x = 0 - x;
@@ -189,13 +190,28 @@ static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int 
 // ---- attention --------------------------------------------------------------------------------------------------
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-struct PagedPlan { int mt, groups, ctas; size_t acc_offset, bytes; };
+// sweep: through the kernel for many rows, after a kernel that turns the queries into the workspace.
+struct PagedPlan { bool sweep; int mt, groups, ctas; size_t q_offset, acc_offset, bytes; };
+
+constexpr int kPagedRows = 32;         // most rows of a KV head's queries that a 16-bit cache's paged_kernel takes
 
 static int block_keys(int D, int bits) { return bits == 16 ? 2048 / D : (D == 128 ? 32 : 64); }
+
+// The kernel for many rows takes its queries as tiles: those to be turned, and expanded ones, are written out first.
+static bool copies_queries(const bob_sm100_paged_args* a) {
+    const int64_t* s = a->q_strides;
+    return a->rotary.pairs || (s[0] == 0 && a->seq.B > 1) || (s[1] == 0 && a->Hq > 1) || (s[2] == 0 && a->N > 1);
+}
 
 static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
     PagedPlan d = {};
     const int64_t R = (int64_t)a->N * (a->Hq / a->cache.heads);
+    d.sweep = a->cache.bits == 16 && R > kPagedRows;
+    if (d.sweep) {
+        d.q_offset = 256;
+        d.bytes = d.q_offset + (copies_queries(a) ? (size_t)a->seq.B * a->Hq * a->N * a->cache.D * 2 : 0);
+        return d;
+    }
     d.mt = R <= 16 ? 1 : 2;
     d.groups = (int)((R + 16 * d.mt - 1) / (16 * d.mt));
     // no more CTAs than the longest possible sequences have work for
@@ -252,6 +268,24 @@ static int launch_paged(PagedParams& p, int device, cudaStream_t stream) {
 
 static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_t stream) {
     const PagedPlan d = paged_plan(a);
+    if (d.sweep) {
+        const SequenceParams seq = sequences(&a->cache, &a->seq);
+        const void* q = a->q;
+        int64_t strides[3] = {a->q_strides[0], a->q_strides[1], a->q_strides[2]};
+        if (copies_queries(a)) {
+            bob_sm100_rotate_args r = {};
+            r.B = a->seq.B; r.N = a->N; r.D = a->cache.D; r.dtype = a->cache.dtype; r.device = a->cache.device;
+            r.heads[0] = a->Hq;
+            r.in[0] = q;
+            for (int i = 0; i < 3; ++i) r.in_strides[0][i] = strides[i];
+            r.out[0] = static_cast<char*>(workspace) + d.q_offset;
+            r.rotary = a->rotary;
+            if (int rc = run_rotate(&r, stream, a->seq.lengths, a->seq.counts)) return rc;
+            q = r.out[0];
+            strides[2] = a->cache.D; strides[1] = strides[2] * a->N; strides[0] = strides[1] * a->Hq;
+        }
+        return sweep_paged(a, seq, q, strides, workspace, stream);
+    }
     PagedParams p = {};
     p.rotary = a->rotary;
     p.seq = sequences(&a->cache, &a->seq);

@@ -180,6 +180,7 @@ struct RotateParams {
     int B, N, D;
     const void* positions; int wide; long long pos_sb, pos_sn;   // int64 or int32; null: first + row
     int64_t first;
+    const int *lengths, *counts;  // not null: the positions of a paged call's rows (counts null: all N), not the above
 };
 
 constexpr int kRotateThreads = 256;
@@ -205,7 +206,9 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
         if (th < t.H) x[k] = place.load(t.in + b * t.in_sb + th * t.in_sh + n * t.in_sn);
     }
     int64_t position = p.first + n;
-    if (p.positions) {
+    if (p.lengths) {
+        position = __ldg(p.lengths + b) - (p.counts ? __ldg(p.counts + b) : p.N) + n;
+    } else if (p.positions) {
         const long long at = b * p.pos_sb + n * p.pos_sn;
         position = p.wide ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
     }

@@ -27,6 +27,7 @@
 #pragma once
 
 #include "ptx.cuh"
+#include "sequence.cuh"
 
 namespace bob {
 
@@ -43,7 +44,10 @@ namespace bob {
 #define BOB_TR_FLUSH
 #endif
 
-enum Mode : int { kFwd = 0, kBwd1Row = 1, kBwd1Col = 2, kBwd2Row = 3, kBwd2Col = 4 };
+enum Mode : int { kFwd = 0, kBwd1Row = 1, kBwd1Col = 2, kBwd2Row = 3, kBwd2Col = 4, kFwdPaged = 5 };
+// kFwdPaged: the forward over a paged cache.  Queries are [B, Hq, N, D] as ever; keys and values come from the pages of
+// SweepParams::seq, every sequence has a length and a number of queries of its own, and there is no lse.
+__host__ __device__ constexpr bool is_forward(int mode) { return mode == kFwd || mode == kFwdPaged; }
 enum TensorId : int { kTQ = 0, kTK, kTV, kTDO, kTUQ, kTUK, kTUV, kTOUT, kNumTensors };
 
 // Status codes written to the status word by a CTA that gave up on a wait.
@@ -76,10 +80,13 @@ struct SweepParams {
     int* sticky;                  // optional second word that a CTA giving up also writes (host-visible memory)
     int* work_counter;            // persistent launches: next work item (zeroed by the host); null: one item per CTA
     long long* trace;             // development builds with BOB_TRACE
+    SequenceParams seq;           // kFwdPaged: map[kTK] and map[kTV] are of pages [pages, Hkv, page_size, D]
+    int box_rows;                 // ... rows of a page that one copy takes: a page, or a tile of it
 };
 
 template <int MODE> struct ModeTraits;
 template <> struct ModeTraits<kFwd>     { static constexpr int NOWN = 1, NOTH = 2, NSC = 1, NOUT = 1, NOPER = 1; static constexpr bool COL = false; };
+template <> struct ModeTraits<kFwdPaged> : ModeTraits<kFwd> {};
 template <> struct ModeTraits<kBwd1Row> { static constexpr int NOWN = 2, NOTH = 2, NSC = 2, NOUT = 2, NOPER = 2; static constexpr bool COL = false; };
 template <> struct ModeTraits<kBwd1Col> { static constexpr int NOWN = 2, NOTH = 2, NSC = 2, NOUT = 2, NOPER = 2; static constexpr bool COL = true; };
 template <> struct ModeTraits<kBwd2Row> { static constexpr int NOWN = 3, NOTH = 4, NSC = 4, NOUT = 2, NOPER = 4; static constexpr bool COL = false; };
@@ -87,14 +94,14 @@ template <> struct ModeTraits<kBwd2Col> { static constexpr int NOWN = 4, NOTH = 
 
 // Which global tensor fills own slot / other slot `i` of a mode.
 template <int MODE> __host__ __device__ constexpr int own_tensor(int i) {
-    if (MODE == kFwd) return kTQ;
+    if (is_forward(MODE)) return kTQ;
     if (MODE == kBwd1Row) return i == 0 ? kTQ : kTDO;
     if (MODE == kBwd1Col) return i == 0 ? kTK : kTV;
     if (MODE == kBwd2Row) return i == 0 ? kTQ : (i == 1 ? kTDO : kTUQ);
     return i == 0 ? kTK : (i == 1 ? kTV : (i == 2 ? kTUK : kTUV));
 }
 template <int MODE> __host__ __device__ constexpr int other_tensor(int i) {
-    if (MODE == kFwd || MODE == kBwd1Row) return i == 0 ? kTK : kTV;
+    if (is_forward(MODE) || MODE == kBwd1Row) return i == 0 ? kTK : kTV;
     if (MODE == kBwd1Col) return i == 0 ? kTQ : kTDO;
     if (MODE == kBwd2Row) return i == 0 ? kTK : (i == 1 ? kTUK : (i == 2 ? kTV : kTUV));   // K, uK adjacent; V, uV adjacent
     return i == 0 ? kTQ : (i == 1 ? kTUQ : kTDO);                                          // Q, uQ adjacent
@@ -117,7 +124,7 @@ struct SweepConfig {
     static constexpr int NPW = GP * NG;                    // pointwise threads
     static_assert(NPW == 256 || NPW == 512, "two or four pointwise warpgroups");
     static_assert(NG == 1 || NG == 2, "one or two pointwise groups");
-    static_assert(MODE != kFwd || (NG == 2 && CW == TN), "forward: two groups, one thread per row");
+    static_assert(!is_forward(MODE) || (NG == 2 && CW == TN), "forward: two groups, one thread per row");
     // One more warpgroup holds the role warps: score products, TMA producer, output products, results.
     // Two warps issue products because the queue in front of the tensor pipe is short (a few
     // instructions): while one warp is between two bursts - barriers, commits, loop - the other's
@@ -142,7 +149,7 @@ struct SweepConfig {
     static constexpr int OWN_TILES = MT::NOWN + (OWN_OUT ? 1 : 0);
     // Swept tiles sit in a ring of slots.  A slot holds all tensors of a tile; in the forward, K and V tiles
     // take slots in turn (K is free again after the scores, V after the output product).
-    static constexpr bool SPLIT_KV = MODE == kFwd;
+    static constexpr bool SPLIT_KV = is_forward(MODE);
     static constexpr int SLOT_TENSORS = SPLIT_KV ? 1 : MT::NOTH;
     static constexpr int SLOTS_PER_TILE = SPLIT_KV ? 2 : 1;
     static constexpr int OTH_SUB_BYTES = TN * 128;         // one 64-element-wide sub-tile of a swept tensor
@@ -151,7 +158,7 @@ struct SweepConfig {
     static constexpr int SC_COLS = MT::NSC * TN;
     static constexpr int OPER_COLS_EACH = TN / 2;          // 128 x TN 16-bit values, two per 32-bit column
     static constexpr int OPER_COLS = ALIAS ? 0 : MT::NOPER * OPER_COLS_EACH;
-    static constexpr int NACC = (MODE == kFwd) ? NG : MT::NOUT;
+    static constexpr int NACC = is_forward(MODE) ? NG : MT::NOUT;
     static constexpr int OUT_COLS = NACC * DPAD;
     static constexpr int TMEM_BASE_NEED = NG * (SC_COLS + OPER_COLS) + OUT_COLS;
     // Second backward: where tensor memory has DPAD / 2 columns to spare, the first own tile (Q, or K
@@ -172,7 +179,7 @@ struct SweepConfig {
     // while the next item runs.  A thread owns one row of the result: storing it straight to global memory
     // touches 32 lines per instruction and kept the pointwise threads busy for 2000 (16-bit) to 4500 (with
     // fp32 pk) cycles per item.
-    static constexpr bool STAGED_OUT = MODE <= kBwd1Col || (MODE == kBwd2Col && DPAD == 64);
+    static constexpr bool STAGED_OUT = MODE <= kBwd1Col || MODE == kFwdPaged || (MODE == kBwd2Col && DPAD == 64);
     static constexpr bool STAGED_PK = MODE == kBwd1Row && DPAD == 64;          // (no room at head dim 128)
     static constexpr int N_STAGED = STAGED_OUT ? (MODE == kBwd1Col || MODE == kBwd2Col ? 2 : 1) : 0;
     static constexpr int IO_BYTES = STAGED_IO ? 32 * 1024 : N_STAGED * OWN_TILE_BYTES + (STAGED_PK ? DPAD * 512 : 0);
@@ -191,11 +198,11 @@ struct SweepConfig {
     static_assert(!TURN_PK || DPAD / (NSPLIT * NG) == 32, "128 bytes of an fp32 row per thread");
     // shared memory map (offsets from the 1024-byte aligned base)
     static constexpr int RED_COPIES = MODE == kBwd2Row && DPAD == 64 ? 2 : 1;
-    static constexpr int RED_FLOATS = MODE == kFwd ? 8 * 128 : (MODE == kBwd1Row ? NG * NSPLIT * 128 : (MODE == kBwd2Row ? RED_COPIES * 2 * NG * NSPLIT * 128 : 0));
+    static constexpr int RED_FLOATS = is_forward(MODE) ? 8 * 128 : (MODE == kBwd1Row ? NG * NSPLIT * 128 : (MODE == kBwd2Row ? RED_COPIES * 2 * NG * NSPLIT * 128 : 0));
     static constexpr int NSTAT = MT::COL ? (BWD2 ? 4 : 2) : 0;                  // per-query statistics of a swept tile
     static constexpr int RING = 4;                                              // work items announced ahead
     static constexpr int MAX_SLOTS = 8;
-    static constexpr int NBARS = 3 * MAX_SLOTS + 9 + 4 * NG + 2 * RING + (MODE == kFwd ? 8 : 0);
+    static constexpr int NBARS = 3 * MAX_SLOTS + 9 + 4 * NG + 2 * RING + (is_forward(MODE) ? 8 : 0);
     static constexpr int MISC_BYTES = NBARS * 8 + 16 + 8 * RING;
     static constexpr int SMEM_LIMIT = 232448;
     static constexpr int SLOT_ROOM = (SMEM_LIMIT - OWN_TILES * OWN_TILE_BYTES - IO_BYTES - RED_FLOATS * 4 - MISC_BYTES) / (SLOT_BYTES + NSTAT * TN * 4);
@@ -262,7 +269,7 @@ __global__ void __launch_bounds__(SweepConfig<MODE, DPAD, TN, NG, CW, ALIAS>::NT
 sweep_kernel(const __grid_constant__ SweepParams p) {
     static_assert(!ALLT || MODE == kBwd2Row || MODE == kBwd2Col, "only the second backward has tangents");
     using CFG = SweepConfig<MODE, DPAD, TN, NG, CW, ALIAS>;
-    static_assert(CW == 16 || CW == 32 || CW == 48 || ((CW == 64 || CW == 128) && MODE == kFwd), "score columns per pointwise thread");
+    static_assert(CW == 16 || CW == 32 || CW == 48 || ((CW == 64 || CW == 128) && is_forward(MODE)), "score columns per pointwise thread");
     using MT = ModeTraits<MODE>;
     constexpr int NSPLIT = CFG::NSPLIT, NPW = CFG::NPW, GP = CFG::GP, NSLOT = CFG::NSLOT, KSUB = CFG::KSUB;
     constexpr int SPT = CFG::SLOTS_PER_TILE;
@@ -318,7 +325,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
     const int per_rank = grid_heads * p.B;
     const int n_items = n_own_tiles * per_rank;
     const int n_outer = COL ? p.G : 1;
-    const int doff = p.delta_off;                // q_offset - k_offset, within +-2^29 (see the host's fill_mask)
+    const int doff_all = p.delta_off;            // q_offset - k_offset, within +-2^29 (see the host's fill_mask)
     // kernel parameters that the per-tile code needs, read once
     const bool causal = p.is_causal != 0;
     const int window = p.window;
@@ -326,7 +333,9 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
     // compile-time constants, so the loads and arithmetic of F and C are unconditional instead of
     // predicated on values only known at run time.
     const bool has_uq = ALLT || p.has_uq != 0, has_uk = ALLT || p.has_uk != 0, has_uv = ALLT || p.has_uv != 0;
-    struct Item { int own0, head, batch, kv_head, t_lo, t_hi, T, total; };
+    // lo, hi: other-side positions that can be unmasked; n_own, n_oth, doff: the sequence's own (kFwdPaged only)
+    struct Item { int own0, head, batch, kv_head, t_lo, t_hi, T, total, lo, hi, n_own, n_oth, doff; };
+    constexpr bool PAGED = MODE == kFwdPaged;
     auto decode = [&](int item) {
         Item w;
         const int tile_rank = item / per_rank;
@@ -337,18 +346,26 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         const int own_tile = (!COL && causal) ? (n_own_tiles - 1 - tile_rank) : tile_rank;
         w.own0 = own_tile * 128;
         w.kv_head = COL ? w.head : w.head / p.G;
-        int lo = 0, hi = n_oth;                  // other-side positions [lo, hi) that can be unmasked
-        const int own_last = min(w.own0 + 127, n_own - 1);
+        w.n_own = n_own; w.n_oth = n_oth; w.doff = doff_all;
+        if constexpr (PAGED) {
+            const Sequence q = sequence_of(p.seq, w.batch, p.Nq);
+            w.n_own = q.count; w.n_oth = q.length; w.doff = q.start;
+        }
+        const int doff = w.doff;
+        int lo = 0, hi = w.n_oth;                // other-side positions [lo, hi) that can be unmasked
+        const int own_last = min(w.own0 + 127, w.n_own - 1);
         // (lengths are at most 2^28, |doff| 2^29 and the window 2^30: 32-bit sums cannot overflow)
         if (causal) {
             if (!COL) {
-                hi = min(n_oth, own_last + doff + 1);
+                hi = min(w.n_oth, own_last + doff + 1);
                 if (window > 0) lo = max(0, w.own0 + doff - window + 1);
             } else {
                 lo = max(0, w.own0 - doff);
                 if (window > 0) hi = min(n_oth, own_last - doff + window);
             }
         }
+        if (PAGED && w.own0 >= w.n_own) hi = 0;  // rows behind the sequence's queries
+        w.lo = lo; w.hi = hi;
         w.t_lo = (hi > lo) ? lo / TN : 0;
         w.t_hi = (hi > lo) ? (hi + TN - 1) / TN : 0;
         w.T = w.t_hi - w.t_lo;
@@ -360,6 +377,8 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
 #define BOB_ITEM_LOCALS(w)                                                                         \
     const int own0 = (w).own0, head = (w).head, batch = (w).batch, kv_head = (w).kv_head;         \
     const int t_lo = (w).t_lo, t_hi = (w).t_hi, total = (w).total;                                 \
+    const int doff = PAGED ? (w).doff : doff_all, item_own = PAGED ? (w).n_own : n_own, item_oth = PAGED ? (w).n_oth : n_oth; \
+    (void)doff; (void)item_own; (void)item_oth;                                                    \
     (void)own0; (void)head; (void)batch; (void)kv_head; (void)t_lo; (void)t_hi; (void)total;
 
     auto give_up = [&](int code) {
@@ -400,7 +419,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         mbar_init(bar_io_full, 1);
         mbar_init(bar_io_ready, NPW / 32);
         mbar_init(bar_io_free, 1);
-        if constexpr (MODE == kFwd) { for (int i = 0; i < 8; ++i) mbar_init(bar_ring0 + 8u * (2 * RING + i), 1); }
+        if constexpr (is_forward(MODE)) { for (int i = 0; i < 8; ++i) mbar_init(bar_ring0 + 8u * (2 * RING + i), 1); }
         mbar_fence_init();
     }
     if (warp == NPW / 32) {
@@ -492,6 +511,12 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                 }
             }
         };
+        if constexpr (PAGED) {
+            if (blockIdx.x == 0) {
+                for (int b = lane; b < p.B; b += 32)
+                    if (!sequence_of(p.seq, b, p.Nq).ok) give_up(kStatusBadLength);
+            }
+        }
         for (int k_item = 0; alive; ++k_item) {
             const int slot = k_item % RING;
             if (!__all_sync(0xffffffffu, mbar_wait(bar_item_empty(slot), ((k_item / RING) & 1) ^ 1))) {
@@ -509,7 +534,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
             if (item < 0) break;
             const Item w = decode(item);
             BOB_ITEM_LOCALS(w)
-            if constexpr (!COL && MODE != kFwd) {
+            if constexpr (!COL && !is_forward(MODE)) {
                 // The pointwise threads start the item by reading their rows' statistics with plain loads:
                 // ask for those lines now, a few tiles before they get there.
                 const long long rs0 = ((long long)batch * p.Hq + head) * p.Nq + own0;
@@ -541,6 +566,17 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
             }
             ++n_live;
             int tile = t_lo, outer = 0;          // swept tile, and its head in the group
+            // kFwdPaged: lane j has the tile's j-th box of rows; its page, -1 where none of the rows is in reach.  Read one
+            // tile ahead.
+            auto find_page = [&](int next) -> int {
+                const int key = next * TN + lane * p.box_rows;
+                if (lane * p.box_rows >= TN || key >= w.hi || key + p.box_rows <= w.lo) return -1;
+                const int page = page_of(p.seq, batch, key);
+                if (page < 0) give_up(kStatusBadPage);
+                return page;
+            };
+            int page = -1;
+            if constexpr (PAGED) page = find_page(tile);
             for (int it = 0; alive && it < total; ++it) {
                 const int oth_head = COL ? (head * p.G + outer) : kv_head;
                 #pragma unroll
@@ -550,7 +586,18 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                         alive = false;
                         continue;
                     }
-                    if (lane == 0) {
+                    if constexpr (PAGED) {
+                        const uint32_t copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                        if (lane == 0) mbar_arrive_expect_tx(bar_full(s), copies * KSUB * p.box_rows * 128);
+                        __syncwarp();
+                        if (page >= 0) {
+                            const int row = (tile * TN + lane * p.box_rows) & ((1 << p.seq.page_shift) - 1);
+                            #pragma unroll
+                            for (int ks = 0; ks < KSUB; ++ks)
+                                tma_load_4d(oth_addr(s, ks, 0) + lane * p.box_rows * 128, &p.map[part == 0 ? kTK : kTV], bar_full(s), ks * 64, row, kv_head, page);
+                        }
+                        __syncwarp();
+                    } else if (lane == 0) {
                         uint32_t bytes = 0;
                         #pragma unroll
                         for (int i = 0; i < CFG::SLOT_TENSORS; ++i)
@@ -581,6 +628,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                     if (++s == NSLOT) { s = 0; ++round; }
                 }
                 if (++tile == t_hi) { tile = t_lo; ++outer; }
+                if constexpr (PAGED) { if (it + 1 < total) page = find_page(tile); }
                 if constexpr (COL) { if (it + 1 < total) load_stats(tile, head * p.G + outer, batch); }
             }
         }
@@ -745,7 +793,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                     }
                     BOB_TR(2)
                     tc_fence_after_sync();
-                    if constexpr (MODE == kFwd) {
+                    if constexpr (is_forward(MODE)) {
                         score_mma(NS1{}, sc, 0, 0, 0, st16, false);
                     } else if constexpr (MODE == kBwd1Row || MODE == kBwd1Col) {
                         score_mma(NS1{}, sc, 0, 0, 0, st16, false);     // S  = Q K^T      | S^T  = K Q^T
@@ -822,7 +870,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                     BOB_TR(1)
                     tc_fence_after_sync();
                     const bool acc = it > 0;
-                    if constexpr (MODE == kFwd) {
+                    if constexpr (is_forward(MODE)) {
                         out_mma(g, g, 0, 0, st16, it >= NG);                 // O_g += P V (group g's own accumulator)
                     } else if constexpr (MODE == kBwd1Row) {
                         out_mma(g, 0, 0, 0, st16, acc);                      // dQ += dS K
@@ -901,7 +949,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         const Item w = decode(item);
         BOB_ITEM_LOCALS(w)
         const int own_idx = own0 + row;
-        const bool own_ok = own_idx < n_own;
+        const bool own_ok = own_idx < item_own;
         const long long row_stat = ((long long)batch * p.Hq + head) * p.Nq + own_idx;   // row-owned only
 
         // per-row state (row-owned modes): -lse*log2e and -delta of my row
@@ -1011,7 +1059,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
             // 0 <= dist (< window)
             uint32_t vmask[(CW + 31) / 32];          // bit c % 32 of word c / 32: column c of mine is unmasked
             if (!full) {
-                int mlo = 0, mhi = min(CW - 1, n_oth - (oth0 + col0) - 1);
+                int mlo = 0, mhi = min(CW - 1, item_oth - (oth0 + col0) - 1);
                 if (causal) {
                     if constexpr (!COL) {
                         const int d0 = own_idx + doff - (oth0 + col0);       // dist falls with the column
@@ -1041,7 +1089,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                 if constexpr (!ALIAS) { if (last_s >= 0) wait(bar_empty(last_s), last_par, kStatusTimeoutPw); }
             };
 
-            if constexpr (MODE == kFwd) {
+            if constexpr (is_forward(MODE)) {
                 // One thread owns a whole row of the tile.
                 float s_[CW];
                 #pragma unroll
@@ -1114,6 +1162,23 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                 const float2 t = __fadd2_rn(__fadd2_rn(sum4[0], sum4[1]), __fadd2_rn(sum4[2], sum4[3]));
                 l_run += t.x + t.y;
                 first_tile = false;
+                if constexpr (PAGED) {
+                    // Value rows that no row of the item attends to: probability zero, but what lies there (the rest of a
+                    // page, or of an earlier tile) may be NaN.  They become zero before the product.
+                    if (oth0 < w.lo || oth0 + TN > w.hi) {
+                        int vs = s + 1, vp = par;
+                        if (vs == NSLOT) { vs = 0; vp ^= 1; }
+                        wait(bar_full(vs), vp, kStatusTimeoutPw);
+                        if (oth0 + row < w.lo || oth0 + row >= w.hi) {
+                            #pragma unroll
+                            for (int ks = 0; ks < KSUB; ++ks) {
+                                #pragma unroll
+                                for (int i = 0; i < 8; ++i) st_shared_v4(oth_addr(vs, ks, 0) + row * 128 + 16 * i, 0, 0, 0, 0);
+                            }
+                        }
+                        fence_proxy_async_smem();
+                    }
+                }
             } else {
                 // accumulator order: S, dP (first backward) or S, F, dP, C (second backward).
                 // My CW columns are taken in rounds of 16.  Without ALIAS every round's loads are issued at once
@@ -1262,8 +1327,8 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         {
             // swept tiles [full_lo, full_hi) pair with my own tile entirely unmasked and in range
             int full_lo = 0, full_hi = 0;
-            if (own0 + 127 < n_own) {
-                int lo = 0, hi = n_oth / TN;                        // tiles that lie inside the tensor
+            if (own0 + 127 < item_own) {
+                int lo = 0, hi = item_oth / TN;                        // tiles that lie inside the tensor
                 if (causal) {
                     // oldest and newest own position of the tile pair against the swept tile's extremes
                     if constexpr (!COL) {
@@ -1307,7 +1372,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         BOB_TR(5)
         exp_base += grp == 0 ? total / 2 : (total + 1) / 2;
         float fwd_k0 = 0.f, fwd_k1 = 0.f;            // forward: weights of the two groups' accumulators
-        if constexpr (MODE == kFwd) {
+        if constexpr (is_forward(MODE)) {
             // both groups' (reference, sum) of my row -> the row's normaliser and lse.  The
             // exchange buffer alternates between items: a thread may start the next item while
             // another still reads this one's values.
@@ -1323,7 +1388,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
             // a group that took no tile of this item has never written its accumulator
             fwd_k0 = (total >= 1) ? a0 * inv : 0.f;
             fwd_k1 = (total >= 2) ? a1 * inv : 0.f;
-            if (grp == 0 && own_ok) p.lse[row_stat] = (l > 0.f) ? (m + log2f(l)) * kLn2 : -INFINITY;
+            if (MODE == kFwd && grp == 0 && own_ok) p.lse[row_stat] = (l > 0.f) ? (m + log2f(l)) * kLn2 : -INFINITY;
         }
         // my row's pk columns, on their way while the row sums are combined and the last products finish
         constexpr int PKN = CFG::STAGED_IO ? DPAD / (NSPLIT * NG) : 1;
@@ -1459,7 +1524,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                 float* a0 = EARLY ? acc0[EARLY ? c / 16 : 0] : late0;
                 float* a1 = EARLY ? acc1[EARLY ? c / 16 : 0] : late1;
                 if (col >= p.D) continue;
-                if constexpr (MODE == kFwd) {
+                if constexpr (is_forward(MODE)) {
                     // weighted sum of the two groups' accumulators (weight 0: never written, not read)
                     #pragma unroll
                     for (int i = 0; i < 16; ++i)

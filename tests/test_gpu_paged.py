@@ -82,6 +82,15 @@ def test_several_new_tokens(bits, N, counts, kw, D, dtype):
     _check(lengths, [min(n, c) for n, c in zip(lengths, counts)], N, 8, 2, D, dtype, bits, 32, rotary=rotary, **kw)
 
 
+@pytest.mark.parametrize("page", [16, 64, 128, 1024])
+@pytest.mark.parametrize("kw", [dict(), dict(window_size=100), dict(is_causal=False)])
+@pytest.mark.parametrize("D,dtype", [(32, torch.bfloat16), (64, torch.float16), (128, torch.bfloat16)])
+def test_chunks_over_pages_of_every_size(page, kw, D, dtype):
+    """More rows than fit a tile, sequences that end inside, at and behind one, more items than SMs."""
+    lengths, counts = [1300, 128, 129, 700, 0, 257, 640], [300, 128, 1, 129, 0, 256, 0]
+    _check(lengths, counts, 300, 8, 4, D, dtype, 16, page, **kw)
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("D", [32, 128])
 def test_whole_prompts(bits, D):
@@ -249,6 +258,17 @@ def test_other_layouts_of_cache_and_rows(bits):
     odd = torch.zeros(2, 6, 4, D + 4, dtype=dtype, device="cuda")[..., :D]       # rows that start at no multiple of 16 bytes
     odd.copy_(q)
     assert torch.equal(sdpa_paged(odd, plain, seqs.table, seqs.lengths, rotary=Rotary(D)), a)
+
+
+@pytest.mark.parametrize("rotary", [None, Rotary(64)])
+def test_many_expanded_queries(rotary):
+    seqs = R.Sequences([300, 200], 16)
+    cache = _cache(seqs, 2, 64, torch.bfloat16, 16)
+    q = _heads((2, 1, 90, 64), torch.bfloat16, 6, "bhnd").expand(2, 4, 90, 64)
+    a = sdpa_paged(q, cache, seqs.table, seqs.lengths, rotary=rotary)
+    assert torch.equal(a, sdpa_paged(q.contiguous(), cache, seqs.table, seqs.lengths, rotary=rotary))
+    want, bound = R.attention(q, cache, seqs, rotary=rotary)
+    R.close(a, want, bound, 0)
 
 
 def test_pages_shared_between_sequences():
