@@ -191,7 +191,7 @@ static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int 
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // sweep: through the kernel for many rows, after a kernel that turns the queries into the workspace.
-struct PagedPlan { bool sweep; int mt, groups, ctas; size_t q_offset, acc_offset, bytes; };
+struct PagedPlan { bool sweep; int rows, groups, ctas; size_t q_offset, acc_offset, bytes; };
 
 constexpr int kPagedRows = 32;         // most rows of a KV head's queries that a 16-bit cache's paged_kernel takes
 
@@ -212,13 +212,13 @@ static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
         d.bytes = d.q_offset + (copies_queries(a) ? (size_t)a->seq.B * a->Hq * a->N * a->cache.D * 2 : 0);
         return d;
     }
-    d.mt = R <= 16 ? 1 : 2;
-    d.groups = (int)((R + 16 * d.mt - 1) / (16 * d.mt));
+    d.rows = R <= 8 ? 8 : (R <= 16 ? 16 : 32);
+    d.groups = (int)((R + d.rows - 1) / d.rows);
     // no more CTAs than the longest possible sequences have work for
     const int64_t kb = block_keys(a->cache.D, a->cache.bits), most = ((int64_t)a->seq.max_pages * a->cache.page_size + kb - 1) / kb;
     const int64_t line = most * a->seq.B * a->cache.heads * d.groups;
-    d.ctas = (int)std::min<int64_t>(2 * kPagedSms, std::max<int64_t>(1, line / kPagedMinBlocks));
-    const size_t rows = (size_t)d.ctas * 2 * 16 * d.mt;
+    d.ctas = (int)std::min<int64_t>((d.rows == 8 ? 3 : 2) * kPagedSms, std::max<int64_t>(1, line / kPagedMinBlocks));
+    const size_t rows = (size_t)d.ctas * 2 * d.rows;
     d.acc_offset = up256(rows * 2 * sizeof(float));
     d.bytes = d.acc_offset + rows * a->cache.D * sizeof(float);
     return d;
@@ -241,29 +241,29 @@ static int check_paged(const bob_sm100_paged_args* a) {
     return reinterpret_cast<uintptr_t>(a->out) % 16 ? kBadAlign : 0;
 }
 
-template <int D, int MT, bool BF16, int BITS>
+template <int D, int ROWS, bool BF16, int BITS>
 static int launch_paged(PagedParams& p, int device, cudaStream_t stream) {
-    using CFG = PagedConfig<D, MT, BITS>;
+    using CFG = PagedConfig<D, ROWS, BITS>;
     static std::atomic<uint64_t> done{0};
     const uint64_t bit = 1ull << device;
     if (!(done.load(std::memory_order_acquire) & bit)) {
-        if (cudaFuncSetAttribute(paged_kernel<D, MT, BF16, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, CFG::SMEM) != cudaSuccess) return kBadAttr;
+        if (cudaFuncSetAttribute(paged_kernel<D, ROWS, BF16, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, CFG::SMEM) != cudaSuccess) return kBadAttr;
         done.fetch_or(bit, std::memory_order_release);
     }
-    paged_kernel<D, MT, BF16, BITS><<<p.ctas, kPagedThreads, CFG::SMEM, stream>>>(p);
+    paged_kernel<D, ROWS, BF16, BITS><<<p.ctas, kPagedThreads, CFG::SMEM, stream>>>(p);
     if (int rc = launched()) return rc;
     // started while paged_kernel runs, and waits for it
     cudaLaunchAttribute early = {};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    const int rows = std::min(CFG::ROWS, p.N * p.G);
+    const int rows = std::min(ROWS, p.N * p.G);
     cfg.gridDim = dim3((unsigned)(p.seq.B * p.Hkv * p.groups), (unsigned)((rows + kPagedWarps - 1) / kPagedWarps));
     cfg.blockDim = dim3(kPagedThreads);
     cfg.stream = stream;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, combine_kernel<D, MT, BF16, BITS>, p) == cudaSuccess ? 0 : kBadLaunch;
+    return cudaLaunchKernelEx(&cfg, combine_kernel<D, ROWS, BF16, BITS>, p) == cudaSuccess ? 0 : kBadLaunch;
 }
 
 static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_t stream) {
@@ -304,14 +304,18 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
     int rc = 0;
     with_type(a->cache.dtype, [&](auto bf16) {
         constexpr bool BF = decltype(bf16)::value;
-        auto dim = [&](auto mt, auto bits) {
-            constexpr int MT = decltype(mt)::value, BITS = decltype(bits)::value;
-            if (a->cache.D == 32) rc = launch_paged<32, MT, BF, BITS>(p, a->cache.device, stream);
-            else if (a->cache.D == 64) rc = launch_paged<64, MT, BF, BITS>(p, a->cache.device, stream);
-            else rc = launch_paged<128, MT, BF, BITS>(p, a->cache.device, stream);
+        auto dim = [&](auto rows, auto bits) {
+            constexpr int ROWS = decltype(rows)::value, BITS = decltype(bits)::value;
+            if (a->cache.D == 32) rc = launch_paged<32, ROWS, BF, BITS>(p, a->cache.device, stream);
+            else if (a->cache.D == 64) rc = launch_paged<64, ROWS, BF, BITS>(p, a->cache.device, stream);
+            else rc = launch_paged<128, ROWS, BF, BITS>(p, a->cache.device, stream);
         };
-        if (a->cache.bits == 16) { if (d.mt == 1) dim(Int<1>{}, Int<16>{}); else dim(Int<2>{}, Int<16>{}); }
-        else { if (d.mt == 1) dim(Int<1>{}, Int<4>{}); else dim(Int<2>{}, Int<4>{}); }
+        auto width = [&](auto bits) {
+            if (d.rows == 8) dim(Int<8>{}, bits);
+            else if (d.rows == 16) dim(Int<16>{}, bits);
+            else dim(Int<32>{}, bits);
+        };
+        if (a->cache.bits == 16) width(Int<16>{}); else width(Int<4>{});
     });
     return rc;
 }

@@ -1,8 +1,12 @@
 // Attention of new tokens' queries over a paged cache, 16-bit or 4-bit: out = softmax(scale q k^T + mask) v.
 //
-// What bounds it: reading the cached rows once.  A KV head's queries (count tokens x G heads, 16 or 32 rows at a time)
-// share every row that is read, and the products run on mma.sync (m16n8k16): a step of generation needs at most 16 rows of
+// What bounds it: reading the cached rows once.  A KV head's queries (count tokens x G heads, 8, 16 or 32 rows at a time)
+// share every row that is read, and the products run on mma.sync (m16n8k16): a step of generation needs a few rows of
 // a product, where tcgen05's 128 would be padding, and its operands come straight from the registers that decode 4 bits.
+//
+// Up to 16 rows, queries and probabilities go through the products in two 16-bit parts each (the value rounded, and what
+// the rounding left), so that only the result is rounded to 16 bits.  With up to 8 rows the second parts are rows 8 ... 15 of
+// the same product, which would be padding, and cost nothing; with up to 16 they are a second product.
 //
 // Every warp is a stream of its own: it copies blocks of KB keys into its ring in shared memory (cp.async, NST - 1 blocks
 // ahead, also across the ends of its work), waits for its own copies only, and keeps its own running maximum, sum and
@@ -37,9 +41,12 @@ struct PagedParams {
 constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedMinBlocks = 4;          // blocks that are worth a CTA of their own
 
-template <int D_, int MT_, int BITS_>
+template <int D_, int ROWS_, int BITS_>
 struct PagedConfig {
-    static constexpr int D = D_, MT = MT_, BITS = BITS_, ROWS = 16 * MT;
+    static constexpr int D = D_, ROWS = ROWS_, BITS = BITS_;
+    static constexpr bool PARTS = ROWS <= 16;                    // two parts of queries and probabilities
+    static constexpr int MT = ROWS == 8 ? 1 : 2;                 // products of 16 rows
+    static constexpr int LR = ROWS / 8;                          // rows of a thread
     // 16 bits: 4 KB of keys and 4 KB of values per block.  4 bits: 2 to 2.5 KB each, where the work per block counts.
     static constexpr int KB = BITS == 16 ? 2048 / D : (D == 128 ? 32 : 64);
     static constexpr int ROW_BYTES = D * BITS / 8, CHUNKS = ROW_BYTES / 16;
@@ -47,16 +54,24 @@ struct PagedConfig {
     static constexpr int V_STRIDE = BITS == 16 ? ROW_BYTES : (D == 128 ? 80 : (D == 64 ? 48 : 16));
     static constexpr int OFF_V = KB * ROW_BYTES, OFF_SK = OFF_V + KB * V_STRIDE, OFF_SV = OFF_SK + (BITS == 4 ? KB * 8 : 0);
     static constexpr int STAGE = OFF_SV + (BITS == 4 ? KB * 8 : 0);
-    static constexpr int NST = BITS == 16 ? 3 : 4;
-    // columns that 16 rows of an accumulator bring into a ring slot at a time
-    static constexpr int EX_COLS = 64 * D <= STAGE ? D : D / 2;
-    static_assert(64 * EX_COLS <= STAGE && STAGE % 16 == 0, "an accumulator passes through a slot");
+    static constexpr int CTAS = ROWS == 8 ? 3 : 2;              // per SM
+    static constexpr int NST = BITS == 16 ? (CTAS == 2 ? 3 : 2) : (CTAS == 2 ? 4 : 3);
+    // columns that EX_ROWS rows of an accumulator bring into a ring slot at a time
+    static constexpr int EX_ROWS = ROWS == 8 ? 8 : 16;
+    static constexpr int EX_COLS = 4 * EX_ROWS * D <= STAGE ? D : D / 2;
+    static_assert(4 * EX_ROWS * EX_COLS <= STAGE && STAGE % 16 == 0, "an accumulator passes through a slot");
     static constexpr int Q_STRIDE = 2 * D + 16;                  // bytes of a query row; the 16 spread rows over the banks
-    static constexpr int OFF_Q = kPagedWarps * NST * STAGE, OFF_ML = OFF_Q + ROWS * Q_STRIDE;
-    static constexpr int OFF_SLOT = OFF_ML + 2 * kPagedWarps * 16 * 4;
+    static constexpr int OFF_Q = kPagedWarps * NST * STAGE, OFF_ML = OFF_Q + 16 * MT * Q_STRIDE;
+    static constexpr int OFF_SLOT = OFF_ML + 2 * kPagedWarps * EX_ROWS * 4;
     static constexpr int SMEM = OFF_SLOT + 16;
 };
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -89,6 +104,18 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// A product with a value's first part, and with the rest of it.  An infinite element makes the second one infinite of
+// either sign or NaN, and decides the first alone.
+__device__ __forceinline__ float whole(float first, float rest) { return fabsf(rest) < INFINITY ? first + rest : first; }
+
+// Nibbles i and i + 4 of a word as a pair of 16-bit numbers 1 + c / 16.
+template <bool BF16>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
+    constexpr int AT = BF16 ? 3 : 6;                     // where the code goes: the mantissa's upper four bits
+    const int by = 4 * i - AT;
+    return ((by < 0 ? w << -by : w >> by) & (0x000f000fu << AT)) | (BF16 ? 0x3f803f80u : 0x3c003c00u);
 }
 
 // Blocks [first, first + n) of KB keys that the queries of sequence b attend to, of every KV head and row group.
@@ -180,26 +207,37 @@ struct Cursor {
     }
 };
 
-// Row `r` of a KV head's queries (token r / G, head r % G), turned to its position, into shared memory.
+// 16 elements of a query row, turned to its position, into shared memory; the second parts go to `rest` (if there).
 template <int D, bool BF16, int FORM>
-__device__ __forceinline__ void bring_query(const PagedParams& p, uint16_t* dst, const uint16_t* src, int c, int position) {
+__device__ __forceinline__ void bring_query(const PagedParams& p, uint16_t* dst, uint16_t* rest, const uint16_t* src, int c, int position) {
     const RowPlace<FORM> place(c, p.rotary.pairs);
     Turner<FORM, BF16, float> turn;
     const Chunks x = place.load(src);
     turn.set(p.rotary, c, position);
-    place.store(dst, turn(x));
+    float v[16], r[16];
+    turn.values(x, v);
+    const Chunks y{narrow8<BF16>(v), narrow8<BF16>(v + 8)};
+    place.store(dst, y);
+    if (!rest) return;
+    widen8<BF16>(y.a, r);
+    widen8<BF16>(y.b, r + 8);
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = v[i] - r[i];
+    place.store(rest, Chunks{narrow8<BF16>(r), narrow8<BF16>(r + 8)});
 }
 
-template <int D, int MT, bool BF16, int BITS>
-__global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_constant__ PagedParams p) {
-    using CFG = PagedConfig<D, MT, BITS>;
-    constexpr int KB = CFG::KB, NT = KB / 8, KS = D / 16, ROWS = CFG::ROWS, NST = CFG::NST, STAGE = CFG::STAGE;
+template <int D, int ROWS, bool BF16, int BITS>
+__global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CTAS)) paged_kernel(const __grid_constant__ PagedParams p) {
+    using CFG = PagedConfig<D, ROWS, BITS>;
+    constexpr int KB = CFG::KB, NT = KB / 8, KS = D / 16, NST = CFG::NST, STAGE = CFG::STAGE, MT = CFG::MT, LR = CFG::LR;
+    constexpr bool PARTS = CFG::PARTS;
     constexpr float kLog2e = 1.4426950408889634f, kNone = -1e30f;
     extern __shared__ __align__(128) uint8_t paged_smem[];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
     const uint32_t ring = smem_u32(paged_smem) + warp * NST * STAGE;
-    float* sm_m = reinterpret_cast<float*>(paged_smem + CFG::OFF_ML);            // [warp][16]
-    float* sm_l = sm_m + kPagedWarps * 16;
+    constexpr int EXR = CFG::EX_ROWS, EXC = CFG::EX_COLS;
+    float* sm_m = reinterpret_cast<float*>(paged_smem + CFG::OFF_ML);            // [warp][EXR]
+    float* sm_l = sm_m + kPagedWarps * EXR;
     volatile int* sm_slot = reinterpret_cast<volatile int*>(paged_smem + CFG::OFF_SLOT);
     asm volatile("griddepcontrol.launch_dependents;");
 
@@ -234,31 +272,43 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
             }
         }
     };
+    constexpr int RPC = 32 / CFG::CHUNKS;                // rows of a warp-wide copy
+    auto swizzled = [](int r, int ch) { return BITS == 4 ? ch : ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3); };
     auto copy_block = [&]() {
         if (more) {
             const uint32_t dst = ring + fill * STAGE;
             const int key0 = src.blk * KB, mask = (1 << p.seq.page_shift) - 1;
+            const bool inside = key0 >= src.lo && key0 + KB <= src.hi && !__any_sync(0xffffffffu, lane < KB / 16 && page_ids < 0);
             #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const CacheTensor& c = p.cache[w];
                 const uint8_t* head = c.data + src.kv_head * c.sh;
-                #pragma unroll
-                for (int k = 0; k < KB * CFG::CHUNKS / 32; ++k) {
-                    const int id = k * 32 + lane, r = id / CFG::CHUNKS, ch = id % CFG::CHUNKS, key = key0 + r;
-                    const int page = __shfl_sync(0xffffffffu, page_ids, r / 16);
-                    const bool there = key >= src.lo && key < src.hi && page >= 0;
-                    const uint8_t* from = there ? head + page * c.sp + (key & mask) * c.sr + 16 * ch : c.data;
-                    uint32_t to = dst + (w ? CFG::OFF_V + r * CFG::V_STRIDE : r * CFG::ROW_BYTES);
-                    if constexpr (BITS == 16) to += 16 * (ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3));
-                    else to += 16 * ch;
-                    copy16(to, from, there);
+                const int ch = lane % CFG::CHUNKS;
+                auto to = [&](int r) { return dst + (w ? CFG::OFF_V + r * CFG::V_STRIDE : r * CFG::ROW_BYTES) + 16 * swizzled(r, ch); };
+                if (inside) {
+                    // rows of 16 keys lie in one page, one after another
+                    #pragma unroll
+                    for (int sub = 0; sub < KB / 16; sub += RPC > 16 ? RPC / 16 : 1) {
+                        const int r0 = 16 * sub + lane / CFG::CHUNKS;
+                        const int page = __shfl_sync(0xffffffffu, page_ids, r0 / 16);
+                        const uint8_t* from = head + page * c.sp + ((key0 + r0) & mask) * c.sr + 16 * ch;
+                        #pragma unroll
+                        for (int k = 0; k < (RPC > 16 ? 1 : 16 / RPC); ++k) copy16(to(r0 + k * RPC), from + k * RPC * c.sr);
+                    }
+                } else {
+                    #pragma unroll 1
+                    for (int r = lane / CFG::CHUNKS; r < KB; r += RPC) {
+                        const int page = __shfl_sync(0xffffffffu, page_ids, r / 16), key = key0 + r;
+                        const bool there = key >= src.lo && key < src.hi && page >= 0;
+                        copy16(to(r), there ? head + page * c.sp + (key & mask) * c.sr + 16 * ch : c.data, there);
+                    }
                 }
                 if constexpr (BITS == 4) {
                     #pragma unroll
                     for (int k = 0; k < KB / 32; ++k) {
                         const int r = k * 32 + lane, key = key0 + r;
                         const int page = __shfl_sync(0xffffffffu, page_ids, r / 16);
-                        const bool there = key >= src.lo && key < src.hi && page >= 0;
+                        const bool there = inside || (key >= src.lo && key < src.hi && page >= 0);
                         const float* from = there ? c.scales + page * c.ssp + src.kv_head * c.ssh + (key & mask) * c.ssr : c.scales;
                         copy8(dst + (w ? CFG::OFF_SV : CFG::OFF_SK) + 8 * r, from, there);
                     }
@@ -287,19 +337,27 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
         for (int id = tid; id < ROWS * (D / 16); id += kPagedThreads) {
             const int r = row0 + id / (D / 16), c = id % (D / 16), i = r / p.G, h = seg.kv_head * p.G + r % p.G;
             uint16_t* dst = reinterpret_cast<uint16_t*>(paged_smem + CFG::OFF_Q + (id / (D / 16)) * CFG::Q_STRIDE);
+            uint16_t* rest = PARTS ? dst + ROWS * CFG::Q_STRIDE / 2 : nullptr;
             if (r < R && i < s.count) {
                 const uint16_t* from = p.q + seg.b * p.q_sb + h * p.q_sh + i * p.q_sn;
-                if (p.form == kHalf) bring_query<D, BF16, kHalf>(p, dst, from, c, s.start + i);
-                else if (p.form == kInterleaved) bring_query<D, BF16, kInterleaved>(p, dst, from, c, s.start + i);
-                else bring_query<D, BF16, kScattered>(p, dst, from, c, s.start + i);
+                if (p.form == kHalf) bring_query<D, BF16, kHalf>(p, dst, rest, from, c, s.start + i);
+                else if (p.form == kInterleaved) bring_query<D, BF16, kInterleaved>(p, dst, rest, from, c, s.start + i);
+                else bring_query<D, BF16, kScattered>(p, dst, rest, from, c, s.start + i);
             } else {
                 RowPlace<kInterleaved>(c, 0).store(dst, Chunks{});
+                if (PARTS) RowPlace<kInterleaved>(c, 0).store(rest, Chunks{});
             }
         }
         __syncthreads();
         uint32_t qa[MT][KS][4];
-        float q_sum[MT][2];                              // 4 bits: sum of a row's elements
+        float q_sum[LR];                                 // 4 bits: sum of a row's elements
         (void)q_sum;
+        // row of mine (LR of them) that half hr of product mt has, or a part of
+        auto my_row = [](int mt, int hr) { return ROWS == 8 ? 0 : ROWS == 16 ? hr : 2 * mt + hr; };
+        if constexpr (BITS == 4) {
+            #pragma unroll
+            for (int k = 0; k < LR; ++k) q_sum[k] = 0.f;
+        }
         #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const uint32_t base = smem_u32(paged_smem) + CFG::OFF_Q + mt * 16 * CFG::Q_STRIDE;
@@ -328,34 +386,28 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                         }
                     }
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    q_sum[mt][hr] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+                    q_sum[my_row(mt, hr)] += sum + __shfl_xor_sync(0xffffffffu, sum, 2);
                 }
             }
         }
-        int lo[MT][2], hi[MT][2];                        // keys that my rows attend to
-        int all_lo = 0, all_hi = 0x7fffffff;             // ... that every row of the item does
+        int lo[LR], hi[LR];                              // keys that my rows attend to
         #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            #pragma unroll
-            for (int hr = 0; hr < 2; ++hr) {
-                const int i = (row0 + mt * 16 + hr * 8 + g) / p.G;
-                hi[mt][hr] = p.causal ? min(s.length, s.start + i + 1) : s.length;
-                lo[mt][hr] = p.window > 0 ? s.start + i - p.window + 1 : 0;
-            }
+        for (int k = 0; k < LR; ++k) {
+            const int i = (row0 + 8 * k + g) / p.G;
+            hi[k] = p.causal ? min(s.length, s.start + i + 1) : s.length;
+            lo[k] = p.window > 0 ? s.start + i - p.window + 1 : 0;
         }
-        {
-            const int i0 = row0 / p.G, i1 = (row0 + ROWS - 1) / p.G;
-            all_hi = p.causal ? min(s.length, s.start + i0 + 1) : s.length;
-            all_lo = p.window > 0 ? s.start + i1 - p.window + 1 : 0;
-        }
-        float acc[MT][D / 8][4], m[MT][2], l[MT][2], z[MT][2];       // z: 4 bits, what every column gains
+        // ... that every row of the item does
+        const int all_hi = p.causal ? min(s.length, s.start + row0 / p.G + 1) : s.length;
+        const int all_lo = p.window > 0 ? s.start + (row0 + ROWS - 1) / p.G - p.window + 1 : 0;
+        float acc[MT][D / 8][4], m[LR], l[LR], z[LR];    // z: 4 bits, what every column gains
         #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             #pragma unroll
             for (int i = 0; i < D / 8; ++i) acc[mt][i][0] = acc[mt][i][1] = acc[mt][i][2] = acc[mt][i][3] = 0.f;
-            m[mt][0] = m[mt][1] = kNone;
-            l[mt][0] = l[mt][1] = z[mt][0] = z[mt][1] = 0.f;
         }
+        #pragma unroll
+        for (int k = 0; k < LR; ++k) { m[k] = kNone; l[k] = z[k] = 0.f; }
 
         #pragma unroll 1
         for (int blk = seg.blk + warp; blk < seg.last; blk += kPagedWarps) {
@@ -366,7 +418,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
             copy_block();
 
             // ---- scores -----------------------------------------------------------------------------------
-            float sc[MT][NT][4];
+            float sc[MT][NT][4], x[LR][NT][2];           // products; scores of my rows
             #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 #pragma unroll
@@ -379,7 +431,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                     for (int pr = 0; pr < NT / 2; ++pr) {
                         const int r = pr * 16 + (lane / 16) * 8 + lane % 8, ch = 2 * ks + (lane / 8) % 2;
                         uint32_t kf[4];
-                        ldsm4(base + r * CFG::ROW_BYTES + 16 * (ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3)), kf);
+                        ldsm4(base + r * CFG::ROW_BYTES + 16 * swizzled(r, ch), kf);
                         #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             mma16816<BF16>(sc[mt][2 * pr], qa[mt][ks], kf[0], kf[1]);
@@ -388,11 +440,8 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                     }
                 }
             } else {
-                // codes as 16-bit numbers 128 + c (bf16) or 1024 + c (fp16): one operation on a pair.  What the offset
-                // adds to a score, offset * q_sum, goes with the row's zero; in fp32 it costs 2^-24 * 1024 |q_sum| <
-                // 1e-3 of a step of the codes.
-                constexpr uint32_t kOffset = BF16 ? 0x43004300u : 0x64006400u;
-                constexpr float kOff = BF16 ? 128.f : 1024.f;
+                // codes as 16-bit numbers b = 1 + c / 16, exactly: a shift and one operation on a pair.  A score is
+                // scale q . c + zero sum q = 16 scale q . b + (zero - 16 scale) sum q.
                 constexpr int NWD = D / 32;
                 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -402,22 +451,29 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                     for (int j = 0; j < NWD; ++j) {
                         #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            const uint32_t b0 = ((w[j] >> (8 * half)) & 0x000f000fu) | kOffset;
-                            const uint32_t b1 = ((w[j] >> (8 * half + 4)) & 0x000f000fu) | kOffset;
+                            const uint32_t b0 = code_pair<BF16>(w[j], 2 * half), b1 = code_pair<BF16>(w[j], 2 * half + 1);
                             #pragma unroll
                             for (int mt = 0; mt < MT; ++mt) mma16816<BF16>(sc[mt][nt], qa[mt][2 * j + half], b0, b1);
                         }
                     }
-                    uint32_t raw[4];                     // (scale, zero) of keys 2 t and 2 t + 1
-                    lds_words<4>(base + CFG::OFF_SK + 8 * (8 * nt + 2 * t), raw);
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                uint32_t raw[4];                         // 4 bits: (scale, zero) of keys 2 t and 2 t + 1
+                if constexpr (BITS == 4) lds_words<4>(base + CFG::OFF_SK + 8 * (8 * i + 2 * t), raw);
+                #pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if constexpr (ROWS == 8) x[0][i][e] = whole(sc[0][i][e], sc[0][i][2 + e]);
                     #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float scale = __uint_as_float(raw[2 * k]), add = fmaf(-kOff, scale, __uint_as_float(raw[2 * k + 1]));
+                    for (int hr = 0; hr < 2; ++hr) {
+                        if constexpr (ROWS == 16) x[hr][i][e] = whole(sc[0][i][2 * hr + e], sc[MT - 1][i][2 * hr + e]);
+                        if constexpr (ROWS == 32) { x[hr][i][e] = sc[0][i][2 * hr + e]; x[2 + hr][i][e] = sc[MT - 1][i][2 * hr + e]; }
+                    }
+                    if constexpr (BITS == 4) {
+                        const float scale = 16.f * __uint_as_float(raw[2 * e]), add = __uint_as_float(raw[2 * e + 1]) - scale;
                         #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            #pragma unroll
-                            for (int hr = 0; hr < 2; ++hr) sc[mt][nt][2 * hr + k] = fmaf(sc[mt][nt][2 * hr + k], scale, add * q_sum[mt][hr]);
-                        }
+                        for (int k = 0; k < LR; ++k) x[k][i][e] = fmaf(x[k][i][e], scale, add * q_sum[k]);
                     }
                 }
             }
@@ -427,45 +483,47 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
             const bool masked = key0 < all_lo || key0 + KB > all_hi;
             if (masked) {
                 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
+                for (int k = 0; k < LR; ++k) {
                     #pragma unroll
                     for (int i = 0; i < NT; ++i) {
                         #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int key = key0 + 8 * i + 2 * t + (e & 1);
-                            if (key < lo[mt][e >> 1] || key >= hi[mt][e >> 1]) sc[mt][i][e] = -INFINITY;
+                        for (int e = 0; e < 2; ++e) {
+                            const int key = key0 + 8 * i + 2 * t + e;
+                            if (key < lo[k] || key >= hi[k]) x[k][i][e] = -INFINITY;
                         }
                     }
                 }
             }
             uint32_t pa[MT][NT / 2][4];                  // probabilities as the second product's operand
             bool grow = false;
-            float mt_[MT][2];
+            float top[LR];
             #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int k = 0; k < LR; ++k) {
+                float v = fmaxf(x[k][0][0], x[k][0][1]);
                 #pragma unroll
-                for (int hr = 0; hr < 2; ++hr) {
-                    float v = fmaxf(sc[mt][0][2 * hr], sc[mt][0][2 * hr + 1]);
-                    #pragma unroll
-                    for (int i = 1; i < NT; ++i) v = fmaxf(v, fmaxf(sc[mt][i][2 * hr], sc[mt][i][2 * hr + 1]));
-                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-                    mt_[mt][hr] = fmaxf(v * c_exp, kNone);           // (the scale is positive)
-                    grow = grow || mt_[mt][hr] > m[mt][hr] + 8.f;
-                }
+                for (int i = 1; i < NT; ++i) v = fmaxf(v, fmaxf(x[k][i][0], x[k][i][1]));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+                top[k] = fmaxf(v * c_exp, kNone);        // (the scale is positive)
+                grow = grow || top[k] > m[k] + 8.f;
             }
             // the reference moves only when the maximum has outgrown it by 2^8
             if (__any_sync(0xffffffffu, grow)) {
+                float f[LR];
+                #pragma unroll
+                for (int k = 0; k < LR; ++k) {
+                    const float ref = fmaxf(m[k], top[k]);
+                    f[k] = exp2_ftz(m[k] - ref);
+                    m[k] = ref;
+                    l[k] *= f[k];
+                    if constexpr (BITS == 4) z[k] *= f[k];
+                }
                 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     #pragma unroll
-                    for (int hr = 0; hr < 2; ++hr) {
-                        const float ref = fmaxf(m[mt][hr], mt_[mt][hr]), f = exp2_ftz(m[mt][hr] - ref);
-                        m[mt][hr] = ref;
-                        l[mt][hr] *= f;
-                        if constexpr (BITS == 4) z[mt][hr] *= f;
+                    for (int i = 0; i < D / 8; ++i) {
                         #pragma unroll
-                        for (int i = 0; i < D / 8; ++i) { acc[mt][i][2 * hr] *= f; acc[mt][i][2 * hr + 1] *= f; }
+                        for (int e = 0; e < 4; ++e) acc[mt][i][e] *= f[my_row(mt, e >> 1)];
                     }
                 }
             }
@@ -474,25 +532,36 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                 uint32_t raw[4];                         // 4 bits: (scale, zero) of the values of keys 2 t, 2 t + 1
                 if constexpr (BITS == 4) lds_words<4>(base + CFG::OFF_SV + 8 * (8 * i + 2 * t), raw);
                 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
+                for (int k = 0; k < LR; ++k) {
+                    float pr[2];
+                    constexpr bool PB = BITS == 4 || BF16;
                     #pragma unroll
-                    for (int hr = 0; hr < 2; ++hr) {
-                        float pr[2];
-                        #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            pr[k] = exp2_ftz(fmaf(sc[mt][i][2 * hr + k], c_exp, -m[mt][hr]));
-                            l[mt][hr] += pr[k];
-                            if constexpr (BITS == 4) {
-                                // value = scale (code - 8) + (zero + 8 scale): the first part goes through the product, with
-                                // the scale in the probability, the second is the same for every column.  Rounded to
-                                // bf16 in both types (2^-9, a sixtieth of what half a step of the codes is): a scale
-                                // may lie outside fp16.
-                                const float scale = __uint_as_float(raw[2 * k]), mid = fmaf(8.f, scale, __uint_as_float(raw[2 * k + 1]));
-                                if (!masked || pr[k] != 0.f) z[mt][hr] = fmaf(pr[k], mid, z[mt][hr]);
-                                pr[k] = !masked || pr[k] != 0.f ? pr[k] * scale : 0.f;
-                            }
+                    for (int e = 0; e < 2; ++e) {
+                        pr[e] = exp2_ftz(fmaf(x[k][i][e], c_exp, -m[k]));
+                        l[k] += pr[e];
+                        if constexpr (BITS == 4) {
+                            // value = 16 scale b + (zero - 16 scale): the first part goes through the product, with 16 scale
+                            // in the probability, the second is the same for every column.  In bf16 for both
+                            // types: a scale may lie outside fp16.  A masked key's scale may be NaN.
+                            const float scale = 16.f * __uint_as_float(raw[2 * e]), add = __uint_as_float(raw[2 * e + 1]) - scale;
+                            const float was = pr[e];
+                            const bool use = !masked || pr[e] != 0.f;
+                            pr[e] = use ? pr[e] * scale : 0.f;
+                            // (one part: about the middle, so that its rounding, 2^-9, meets b - 3/2 and not b)
+                            if (use) z[k] = fmaf(was, PARTS ? add : fmaf(1.5f, scale, add), z[k]);
                         }
-                        pa[mt][i / 2][2 * (i % 2) + hr] = pack2<BITS == 4 ? true : BF16>(pr[0], pr[1]);
+                    }
+                    const uint32_t first = pack2<PB>(pr[0], pr[1]);
+                    float back[2];
+                    if constexpr (PB) { back[0] = __uint_as_float(first << 16); back[1] = __uint_as_float(first & 0xffff0000u); }
+                    else { const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&first)); back[0] = f2.x; back[1] = f2.y; }
+                    if constexpr (BITS == 4 && !PARTS) z[k] = fmaf(-1.5f, back[0] + back[1], z[k]);
+                    if constexpr (PARTS) {
+                        const uint32_t rest = pack2<PB>(pr[0] - back[0], pr[1] - back[1]);
+                        if constexpr (ROWS == 8) { pa[0][i / 2][2 * (i % 2)] = first; pa[0][i / 2][2 * (i % 2) + 1] = rest; }
+                        else { pa[0][i / 2][2 * (i % 2) + k] = first; pa[MT - 1][i / 2][2 * (i % 2) + k] = rest; }
+                    } else {
+                        pa[k / 2][i / 2][2 * (i % 2) + k % 2] = first;
                     }
                 }
             }
@@ -505,7 +574,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                     for (int dp = 0; dp < D / 16; ++dp) {
                         const int r = kk * 16 + lane % 16, ch = 2 * dp + lane / 16;
                         uint32_t vf[4];
-                        ldsm4_trans(base + CFG::OFF_V + r * CFG::ROW_BYTES + 16 * (ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3)), vf);
+                        ldsm4_trans(base + CFG::OFF_V + r * CFG::ROW_BYTES + 16 * swizzled(r, ch), vf);
                         #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             mma16816<BF16>(acc[mt][2 * dp], pa[mt][kk], vf[0], vf[1]);
@@ -517,12 +586,6 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                 // thread g holds words NWG g ... of a value row: column n of product (word, nibble) is element
                 // 8 (NWG n + word) + nibble.  (D = 32: four words, lanes 4 ... 7 take their upper nibbles.)
                 constexpr int NWG = D >= 64 ? D / 64 : 1, NIB = D >= 64 ? 8 : 4;
-                const __nv_bfloat162 k136 = __floats2bfloat162_rn(136.f, 136.f);
-                auto centred = [&](uint32_t x) {         // two codes as bf16 c - 8, exactly
-                    x = (x & 0x000f000fu) | 0x43004300u;
-                    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), k136);
-                    return *reinterpret_cast<const uint32_t*>(&y);
-                };
                 #pragma unroll
                 for (int kk = 0; kk < NT / 2; ++kk) {
                     uint32_t w[4][NWG];
@@ -533,16 +596,16 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                     }
                     #pragma unroll
                     for (int word = 0; word < NWG; ++word) {
-                        uint32_t x[2][2];                // [keys 2 t, or 2 t + 8][nibbles 0 ... 3, or 4 ... 7] of two keys
+                        uint32_t two[2][2];              // [keys 2 t, or 2 t + 8][nibbles 0 ... 3, or 4 ... 7] of two keys
                         #pragma unroll
                         for (int k = 0; k < 2; ++k) {
-                            x[k][0] = __byte_perm(w[2 * k][word], w[2 * k + 1][word], 0x5410);
-                            x[k][1] = __byte_perm(w[2 * k][word], w[2 * k + 1][word], 0x7632);
-                            if (D == 32 && g >= 4) x[k][0] = x[k][1];
+                            two[k][0] = __byte_perm(w[2 * k][word], w[2 * k + 1][word], 0x5410);
+                            two[k][1] = __byte_perm(w[2 * k][word], w[2 * k + 1][word], 0x7632);
+                            if (D == 32 && g >= 4) two[k][0] = two[k][1];
                         }
                         #pragma unroll
                         for (int i = 0; i < NIB; ++i) {
-                            const uint32_t b0 = centred(x[0][i / 4] >> (4 * (i % 4))), b1 = centred(x[1][i / 4] >> (4 * (i % 4)));
+                            const uint32_t b0 = code_pair<true>(two[0][i / 4], i % 4), b1 = code_pair<true>(two[1][i / 4], i % 4);
                             #pragma unroll
                             for (int mt = 0; mt < MT; ++mt) mma16816<true>(acc[mt][word * NIB + i], pa[mt][kk], b0, b1);
                         }
@@ -551,28 +614,28 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
             }
         }
 
-        // ---- the four warps' parts, through their free ring slots, 16 rows at a time -----------------------
+        // ---- the four warps' parts, through their free ring slots, EXR rows at a time ----------------------
         // the element that column n (0 ... 7) of accumulator tile i stands for
         auto column = [&](int i, int n) {
             if constexpr (BITS == 16) return 8 * i + n;
             else if constexpr (D >= 64) return 8 * ((D / 64) * n + i / 8) + i % 8;
             else return 8 * (n % 4) + 4 * (n / 4) + i;
         };
-        constexpr int EXC = CFG::EX_COLS;
         __syncwarp();                                    // (the slot that is free now was read last)
         #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            if (mt > 0) __syncthreads();
+        for (int pass = 0; pass < ROWS / EXR; ++pass) {
+            if (pass > 0) __syncthreads();
             #pragma unroll
-            for (int hr = 0; hr < 2; ++hr) {
-                float sum = l[mt][hr], zs = z[mt][hr];
+            for (int j = 0; j < EXR / 8; ++j) {
+                const int k = pass * (EXR / 8) + j;      // my row
+                float sum = l[k], zs = z[k];
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 if constexpr (BITS == 4) {
                     zs += __shfl_xor_sync(0xffffffffu, zs, 1);
-                    z[mt][hr] = zs + __shfl_xor_sync(0xffffffffu, zs, 2);
+                    z[k] = zs + __shfl_xor_sync(0xffffffffu, zs, 2);
                 }
-                if (t == 0) { sm_m[warp * 16 + hr * 8 + g] = m[mt][hr]; sm_l[warp * 16 + hr * 8 + g] = sum; }
+                if (t == 0) { sm_m[warp * EXR + j * 8 + g] = m[k]; sm_l[warp * EXR + j * 8 + g] = sum; }
             }
             if (lane == 0) sm_slot[warp] = (warp * NST + fill) * STAGE;
             #pragma unroll
@@ -582,27 +645,34 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
                     #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = g + 8 * (e >> 1), col = column(i, 2 * t + (e & 1)) - part * EXC;
-                        if (EXC == D || (col >= 0 && col < EXC))
-                            mine[r * EXC + (col ^ ((r & 3) << 3))] = acc[mt][i][e] + (BITS == 4 ? z[mt][e >> 1] : 0.f);
+                    for (int j = 0; j < EXR / 8; ++j) {
+                        #pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int r = g + 8 * j, col = column(i, 2 * t + e) - part * EXC;
+                            float v;
+                            if constexpr (ROWS == 8) v = whole(acc[0][i][e], acc[0][i][2 + e]);
+                            else if constexpr (ROWS == 16) v = whole(acc[0][i][2 * j + e], acc[MT - 1][i][2 * j + e]);
+                            else v = acc[pass][i][2 * j + e];
+                            if constexpr (BITS == 4) v += z[pass * (EXR / 8) + j];
+                            if (EXC == D || (col >= 0 && col < EXC)) mine[r * EXC + (col ^ ((r & 3) << 3))] = v;
+                        }
                     }
                 }
                 __syncthreads();
                 #pragma unroll 1
-                for (int id = tid; id < 16 * EXC / 4; id += kPagedThreads) {
-                    const int r = id / (EXC / 4), col = (id % (EXC / 4)) * 4, row = row0 + mt * 16 + r;
+                for (int id = tid; id < EXR * EXC / 4; id += kPagedThreads) {
+                    const int r = id / (EXC / 4), col = (id % (EXC / 4)) * 4, row = row0 + pass * EXR + r;
                     if (row >= R) continue;
                     float ref = sm_m[r];
                     #pragma unroll
-                    for (int w = 1; w < kPagedWarps; ++w) ref = fmaxf(ref, sm_m[w * 16 + r]);
+                    for (int w = 1; w < kPagedWarps; ++w) ref = fmaxf(ref, sm_m[w * EXR + r]);
                     float sum = 0.f;
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     #pragma unroll
                     for (int w = 0; w < kPagedWarps; ++w) {
-                        const float f = exp2_ftz(sm_m[w * 16 + r] - ref);
+                        const float f = exp2_ftz(sm_m[w * EXR + r] - ref);
                         const float4 x = *reinterpret_cast<const float4*>(paged_smem + sm_slot[w] + 4 * (r * EXC + (col ^ ((r & 3) << 3))));
-                        sum = fmaf(f, sm_l[w * 16 + r], sum);
+                        sum = fmaf(f, sm_l[w * EXR + r], sum);
                         v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
                     }
                     const int i = row / p.G, h = seg.kv_head * p.G + row % p.G;
@@ -613,7 +683,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
                         if (sum == 0.f) o = make_uint2(0, 0);
                         *reinterpret_cast<uint2*>(p.out + (((long long)seg.b * p.Hq + h) * p.N + i) * D + part * EXC + col) = o;
                     } else {
-                        const long long at = (2LL * blockIdx.x + (seg.begins ? 1 : 0)) * ROWS + mt * 16 + r;
+                        const long long at = (2LL * blockIdx.x + (seg.begins ? 1 : 0)) * ROWS + pass * EXR + r;
                         *reinterpret_cast<float4*>(p.part_acc + at * D + part * EXC + col) = v;
                         if (part == 0 && col == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(ref, sum);
                     }
@@ -624,10 +694,10 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_kernel(const __grid_co
 }
 
 // Adds the parts of the items that paged_kernel divided, and writes the zeros of those without keys.  One warp per query row.
-template <int D, int MT, bool BF16, int BITS>
+template <int D, int ROWS, bool BF16, int BITS>
 __global__ void __launch_bounds__(kPagedThreads) combine_kernel(const __grid_constant__ PagedParams p) {
-    using CFG = PagedConfig<D, MT, BITS>;
-    constexpr int KB = CFG::KB, ROWS = CFG::ROWS, LPR = D / 4, PER = 32 / LPR;   // lanes of a row; parts taken at a time
+    using CFG = PagedConfig<D, ROWS, BITS>;
+    constexpr int KB = CFG::KB, LPR = D / 4, PER = 32 / LPR;   // lanes of a row; parts taken at a time
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int per = p.Hkv * p.groups, b = blockIdx.x / per, item = blockIdx.x % per;
     const int r = blockIdx.y * kPagedWarps + warp, row = (item % p.groups) * ROWS + r;

@@ -136,23 +136,29 @@ struct Turner {
             if (j < active) turn_factors(position, r.turns[8 * place + j], static_cast<T>(r.factor), s[j], c[j]);
         }
     }
+    static constexpr int STEP = FORM == kInterleaved ? 2 : 1, PARTNER = FORM == kInterleaved ? 1 : 8;
+    // The 16 elements in fp32, turned.
+    __device__ __forceinline__ void values(const Chunks& x, float (&v)[16]) const {
+        widen8<BF16>(x.a, v);
+        widen8<BF16>(x.b, v + 8);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float a = v[STEP * j], b = v[STEP * j + PARTNER];
+            if (j < active) {                                // (elements that do not turn keep their bits)
+                v[STEP * j] = a * c[j] - b * s[j];
+                v[STEP * j + PARTNER] = b * c[j] + a * s[j];
+            }
+        }
+    }
     __device__ __forceinline__ Chunks operator()(const Chunks& x) const {
         if (active == 0) return x;
         float v[16];
-        widen8<BF16>(x.a, v);
-        widen8<BF16>(x.b, v + 8);
-        constexpr int STEP = FORM == kInterleaved ? 2 : 1, PARTNER = FORM == kInterleaved ? 1 : 8;
         if constexpr (sizeof(T) == 4) {
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float a = v[STEP * j], b = v[STEP * j + PARTNER];
-                if (j < active) {                            // (elements that do not turn keep their bits)
-                    v[STEP * j] = a * c[j] - b * s[j];
-                    v[STEP * j + PARTNER] = b * c[j] + a * s[j];
-                }
-            }
+            values(x, v);
             return Chunks{narrow8<BF16>(v), narrow8<BF16>(v + 8)};
         } else {
+            widen8<BF16>(x.a, v);
+            widen8<BF16>(x.b, v + 8);
             uint32_t w[16];
             #pragma unroll
             for (int j = 0; j < 8; ++j) {

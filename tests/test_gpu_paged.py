@@ -327,6 +327,19 @@ def test_an_infinite_score_makes_its_row_nan_and_no_other():
     assert out[0, 0::2].isnan().all() and out[0, 1::2].isfinite().all() and out[1].isfinite().all()
 
 
+@pytest.mark.parametrize("N", [1, 4, 40])
+def test_an_infinite_value_reaches_its_column_and_no_other(N):
+    seqs = R.Sequences([300, 300], 16)
+    cache = _cache(seqs, 1, 64, torch.bfloat16, 16)
+    page, row = seqs.table[0, 33 // 16].long(), 33 % 16
+    cache.v[page, 0, row, 5] = -math.inf
+    q = _heads((2, 4, N, 64), torch.bfloat16, 2)
+    out = sdpa_paged(q, cache, seqs.table, seqs.lengths)
+    assert (out[0, ..., 5] == -math.inf).all()
+    out[0, ..., 5] = 0
+    assert out.isfinite().all()
+
+
 def test_generation_step_by_step_equals_one_attention_over_the_whole():
     """Prompts, then tokens one at a time, against the operator for contiguous tensors on the whole sequences."""
     B, Hq, Hkv, D, dtype = 3, 8, 2, 64, torch.bfloat16
