@@ -49,6 +49,8 @@ struct PagedConfig {
     static constexpr int LR = ROWS / 8;                          // rows of a thread
     // 16 bits: 4 KB of keys and 4 KB of values per block.  4 bits: 2 to 2.5 KB each, where the work per block counts.
     static constexpr int KB = BITS == 16 ? 2048 / D : (D == 128 ? 32 : 64);
+    static constexpr int SUB = 2048 / D;                         // keys of a block that are computed at a time
+    static_assert(KB % SUB == 0 && SUB % 16 == 0, "whole products");
     static constexpr int ROW_BYTES = D * BITS / 8, CHUNKS = ROW_BYTES / 16;
     // 4 bits: a thread reads a word of four rows two apart; these strides put the rows into different banks
     static constexpr int V_STRIDE = BITS == 16 ? ROW_BYTES : (D == 128 ? 80 : (D == 64 ? 48 : 16));
@@ -108,15 +110,29 @@ __device__ __forceinline__ float exp2_ftz(float x) {
 
 // A product with a value's first part, and with the rest of it.  An infinite element makes the second one infinite of
 // either sign or NaN, and decides the first alone.
-__device__ __forceinline__ float whole(float first, float rest) { return fabsf(rest) < INFINITY ? first + rest : first; }
+// (Codes are finite.)
+template <int BITS>
+__device__ __forceinline__ float whole(float first, float rest) { return BITS == 4 || fabsf(rest) < INFINITY ? first + rest : first; }
 
-// Nibbles i and i + 4 of a word as a pair of 16-bit numbers 1 + c / 16.
+// Pairs of codes as pairs of 16-bit numbers 1 + c / 16: a shift and one logic operation, if mask and exponent come from
+// registers (with both as constants the compiler takes two operations).
 template <bool BF16>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
-    constexpr int AT = BF16 ? 3 : 6;                     // where the code goes: the mantissa's upper four bits
-    const int by = 4 * i - AT;
-    return ((by < 0 ? w << -by : w >> by) & (0x000f000fu << AT)) | (BF16 ? 0x3f803f80u : 0x3c003c00u);
-}
+struct CodePairs {
+    static constexpr int AT = BF16 ? 3 : 6;              // where the code goes: the mantissa's upper four bits
+    uint32_t mask, one;
+    __device__ __forceinline__ CodePairs() {
+        asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(0x000f000fu << AT));
+        asm volatile("mov.b32 %0, %1;" : "=r"(one) : "n"(BF16 ? 0x3f803f80u : 0x3c003c00u));
+    }
+    // nibbles i and i + 4 of a word
+    __device__ __forceinline__ uint32_t operator()(uint32_t w, int i) const {
+        const int by = 4 * i - AT;
+        const uint32_t x = by < 0 ? w << -by : w >> by;
+        uint32_t r;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(one));       // (x & mask) | one
+        return r;
+    }
+};
 
 // Blocks [first, first + n) of KB keys that the queries of sequence b attend to, of every KV head and row group.
 struct BlockRange { int first, n; };
@@ -229,7 +245,7 @@ __device__ __forceinline__ void bring_query(const PagedParams& p, uint16_t* dst,
 template <int D, int ROWS, bool BF16, int BITS>
 __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CTAS)) paged_kernel(const __grid_constant__ PagedParams p) {
     using CFG = PagedConfig<D, ROWS, BITS>;
-    constexpr int KB = CFG::KB, NT = KB / 8, KS = D / 16, NST = CFG::NST, STAGE = CFG::STAGE, MT = CFG::MT, LR = CFG::LR;
+    constexpr int KB = CFG::KB, SUB = CFG::SUB, NT = SUB / 8, KS = D / 16, NST = CFG::NST, STAGE = CFG::STAGE, MT = CFG::MT, LR = CFG::LR;
     constexpr bool PARTS = CFG::PARTS;
     constexpr float kLog2e = 1.4426950408889634f, kNone = -1e30f;
     extern __shared__ __align__(128) uint8_t paged_smem[];
@@ -327,6 +343,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
 
     const float c_exp = p.scale * kLog2e;
     const int R = p.N * p.G;
+    const CodePairs<BF16> key_codes;
+    const CodePairs<true> value_codes;
     #pragma unroll 1
     while (seg.template next<ROWS>(p)) {
         const Sequence s = sequence_of(p.seq, seg.b, p.N);
@@ -413,10 +431,16 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
         for (int blk = seg.blk + warp; blk < seg.last; blk += kPagedWarps) {
             copies_wait<NST - 2>();
             __syncwarp();                                // every lane's copies are there, and the free slot is read
-            const uint32_t base = ring + slot * STAGE;
+            const uint32_t stage = ring + slot * STAGE;
             slot = slot + 1 == NST ? 0 : slot + 1;
             copy_block();
 
+            #pragma unroll 1
+            for (int sub = 0; sub < KB / SUB; ++sub) {
+            const uint32_t base = stage + sub * SUB * CFG::ROW_BYTES;            // key rows; values, scales:
+            const uint32_t base_v = stage + CFG::OFF_V + sub * SUB * CFG::V_STRIDE;
+            const uint32_t base_sk = stage + CFG::OFF_SK + sub * SUB * 8, base_sv = stage + CFG::OFF_SV + sub * SUB * 8;
+            (void)base_sk; (void)base_sv;
             // ---- scores -----------------------------------------------------------------------------------
             float sc[MT][NT][4], x[LR][NT][2];           // products; scores of my rows
             #pragma unroll
@@ -451,7 +475,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     for (int j = 0; j < NWD; ++j) {
                         #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            const uint32_t b0 = code_pair<BF16>(w[j], 2 * half), b1 = code_pair<BF16>(w[j], 2 * half + 1);
+                            const uint32_t b0 = key_codes(w[j], 2 * half), b1 = key_codes(w[j], 2 * half + 1);
                             #pragma unroll
                             for (int mt = 0; mt < MT; ++mt) mma16816<BF16>(sc[mt][nt], qa[mt][2 * j + half], b0, b1);
                         }
@@ -461,13 +485,13 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 uint32_t raw[4];                         // 4 bits: (scale, zero) of keys 2 t and 2 t + 1
-                if constexpr (BITS == 4) lds_words<4>(base + CFG::OFF_SK + 8 * (8 * i + 2 * t), raw);
+                if constexpr (BITS == 4) lds_words<4>(base_sk + 8 * (8 * i + 2 * t), raw);
                 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    if constexpr (ROWS == 8) x[0][i][e] = whole(sc[0][i][e], sc[0][i][2 + e]);
+                    if constexpr (ROWS == 8) x[0][i][e] = whole<BITS>(sc[0][i][e], sc[0][i][2 + e]);
                     #pragma unroll
                     for (int hr = 0; hr < 2; ++hr) {
-                        if constexpr (ROWS == 16) x[hr][i][e] = whole(sc[0][i][2 * hr + e], sc[MT - 1][i][2 * hr + e]);
+                        if constexpr (ROWS == 16) x[hr][i][e] = whole<BITS>(sc[0][i][2 * hr + e], sc[MT - 1][i][2 * hr + e]);
                         if constexpr (ROWS == 32) { x[hr][i][e] = sc[0][i][2 * hr + e]; x[2 + hr][i][e] = sc[MT - 1][i][2 * hr + e]; }
                     }
                     if constexpr (BITS == 4) {
@@ -479,8 +503,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             }
 
             // ---- softmax ----------------------------------------------------------------------------------
-            const int key0 = blk * KB;
-            const bool masked = key0 < all_lo || key0 + KB > all_hi;
+            const int key0 = blk * KB + sub * SUB;
+            const bool masked = key0 < all_lo || key0 + SUB > all_hi;
             if (masked) {
                 #pragma unroll
                 for (int k = 0; k < LR; ++k) {
@@ -530,7 +554,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             #pragma unroll
             for (int i = 0; i < NT; ++i) {
                 uint32_t raw[4];                         // 4 bits: (scale, zero) of the values of keys 2 t, 2 t + 1
-                if constexpr (BITS == 4) lds_words<4>(base + CFG::OFF_SV + 8 * (8 * i + 2 * t), raw);
+                if constexpr (BITS == 4) lds_words<4>(base_sv + 8 * (8 * i + 2 * t), raw);
                 #pragma unroll
                 for (int k = 0; k < LR; ++k) {
                     float pr[2];
@@ -542,13 +566,11 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         if constexpr (BITS == 4) {
                             // value = 16 scale b + (zero - 16 scale): the first part goes through the product, with 16 scale
                             // in the probability, the second is the same for every column.  In bf16 for both
-                            // types: a scale may lie outside fp16.  A masked key's scale may be NaN.
+                            // types: a scale may lie outside fp16.
                             const float scale = 16.f * __uint_as_float(raw[2 * e]), add = __uint_as_float(raw[2 * e + 1]) - scale;
-                            const float was = pr[e];
-                            const bool use = !masked || pr[e] != 0.f;
-                            pr[e] = use ? pr[e] * scale : 0.f;
                             // (one part: about the middle, so that its rounding, 2^-9, meets b - 3/2 and not b)
-                            if (use) z[k] = fmaf(was, PARTS ? add : fmaf(1.5f, scale, add), z[k]);
+                            z[k] = fmaf(pr[e], PARTS ? add : fmaf(1.5f, scale, add), z[k]);
+                            pr[e] *= scale;
                         }
                     }
                     const uint32_t first = pack2<PB>(pr[0], pr[1]);
@@ -574,7 +596,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     for (int dp = 0; dp < D / 16; ++dp) {
                         const int r = kk * 16 + lane % 16, ch = 2 * dp + lane / 16;
                         uint32_t vf[4];
-                        ldsm4_trans(base + CFG::OFF_V + r * CFG::ROW_BYTES + 16 * swizzled(r, ch), vf);
+                        ldsm4_trans(base_v + r * CFG::ROW_BYTES + 16 * swizzled(r, ch), vf);
                         #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             mma16816<BF16>(acc[mt][2 * dp], pa[mt][kk], vf[0], vf[1]);
@@ -592,7 +614,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int r = kk * 16 + 2 * t + (k & 1) + 8 * (k >> 1);
-                        lds_words<NWG>(base + CFG::OFF_V + r * CFG::V_STRIDE + 4 * (D >= 64 ? NWG * g : g % 4), w[k]);
+                        lds_words<NWG>(base_v + r * CFG::V_STRIDE + 4 * (D >= 64 ? NWG * g : g % 4), w[k]);
                     }
                     #pragma unroll
                     for (int word = 0; word < NWG; ++word) {
@@ -605,13 +627,14 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         }
                         #pragma unroll
                         for (int i = 0; i < NIB; ++i) {
-                            const uint32_t b0 = code_pair<true>(two[0][i / 4], i % 4), b1 = code_pair<true>(two[1][i / 4], i % 4);
+                            const uint32_t b0 = value_codes(two[0][i / 4], i % 4), b1 = value_codes(two[1][i / 4], i % 4);
                             #pragma unroll
                             for (int mt = 0; mt < MT; ++mt) mma16816<true>(acc[mt][word * NIB + i], pa[mt][kk], b0, b1);
                         }
                     }
                 }
             }
+            }   // sub
         }
 
         // ---- the four warps' parts, through their free ring slots, EXR rows at a time ----------------------
@@ -650,8 +673,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         for (int e = 0; e < 2; ++e) {
                             const int r = g + 8 * j, col = column(i, 2 * t + e) - part * EXC;
                             float v;
-                            if constexpr (ROWS == 8) v = whole(acc[0][i][e], acc[0][i][2 + e]);
-                            else if constexpr (ROWS == 16) v = whole(acc[0][i][2 * j + e], acc[MT - 1][i][2 * j + e]);
+                            if constexpr (ROWS == 8) v = whole<BITS>(acc[0][i][e], acc[0][i][2 + e]);
+                            else if constexpr (ROWS == 16) v = whole<BITS>(acc[0][i][2 * j + e], acc[MT - 1][i][2 * j + e]);
                             else v = acc[pass][i][2 * j + e];
                             if constexpr (BITS == 4) v += z[pass * (EXR / 8) + j];
                             if (EXC == D || (col >= 0 && col < EXC)) mine[r * EXC + (col ^ ((r & 3) << 3))] = v;
