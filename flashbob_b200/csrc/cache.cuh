@@ -22,7 +22,7 @@ struct CacheTensor {
     float* scales; long long ssp, ssh, ssr;                      // 4 bits: (scale, zero) of a row; strides in floats
 };
 
-struct AppendParams {
+struct alignas(16) AppendParams {
     bob_sm100_rotary rotary;
     SequenceParams seq;
     CacheTensor cache[2];                                        // keys, values
@@ -58,24 +58,41 @@ __device__ __forceinline__ uint2 quantise16(const Chunks& x, int per_row, float&
     zero = lo;
     scale = hi > lo ? __fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f) : 1.f;
     const float inv = __frcp_rn(scale);
-    uint32_t code[2] = {0, 0};
+    // q + 1.5 * 2^23 rounds q to a whole number, halves to even, in the last bits: its bits are kWhole + code, and eight of
+    // them, each 16 times the one before, add up to the word of codes and a constant
+    constexpr float kShift = 12582912.f;
+    constexpr uint32_t kWhole = 0x4b400000u, kExtra = kWhole * 0x11111111u;
+    uint32_t word[2] = {0, 0};
+    float border = 0.f;                                          // how far a quotient is from its code: near a border, 1/2
     #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float d = __fsub_rn(v[i], lo), q = d * inv;        // off by 3 * 2^-24 of at most 15
-        float r = rintf(q);
-        if (!(fabsf(fabsf(q - r) - 0.5f) > 1e-5f)) r = rintf(__fdiv_rn(d, scale));     // near a border, or no number
-        code[i >> 3] |= static_cast<uint32_t>(min(max(__float2int_rn(r), 0), 15)) << (4 * (i & 7));
+    for (int i = 15; i >= 0; --i) {
+        const float q = __fmul_rn(__fsub_rn(v[i], lo), inv);     // off by 3 * 2^-24 of at most 15
+        const float r = __fadd_rn(q, kShift);
+        border = max_nan(border, fabsf(__fsub_rn(q, __fsub_rn(r, kShift))));
+        word[i >> 3] = word[i >> 3] * 16 + __float_as_uint(r);
     }
-    return make_uint2(code[0], code[1]);
+    if (!(border < 0.49999f)) {                                  // (or no number)
+        word[0] = word[1] = 0;
+        #pragma unroll 1
+        for (int i = 15; i >= 0; --i) {
+            const uint32_t w = (i < 8 ? (&x.a.x) : (&x.b.x))[(i % 8) / 2];
+            const uint16_t bits = static_cast<uint16_t>(i % 2 ? w >> 16 : w);
+            const float e = BF16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
+            const uint32_t r = __float_as_uint(__fadd_rn(__fdiv_rn(__fsub_rn(e, lo), scale), kShift));
+            if (i < 8) word[0] = word[0] * 16 + r; else word[1] = word[1] * 16 + r;
+        }
+    }
+    return make_uint2(word[0] - kExtra, word[1] - kExtra);
 }
 
 constexpr int kCacheThreads = 256;
 
-// One thread: 16 elements of a new row, of HPT heads (blockIdx.y), of keys and values.  BITS 4 turns the keys in 64 bits: a
+// One thread: 16 elements of a new row of a head (blockIdx.y), of keys and values.  BITS 4 turns the keys in 64 bits: a
 // rounding that falls the other way can move an element by a whole step of the 4-bit row, 1/15 of its range.
-template <int FORM, bool BF16, int BITS, int HPT>
+template <int FORM, bool BF16, int BITS>
 __global__ void __launch_bounds__(kCacheThreads) append_kernel(const __grid_constant__ AppendParams p) {
-    const int per_row = p.D / 16;
+    __shared__ __align__(16) uint16_t stage[FORM == kScattered ? kCacheThreads * 16 : 8];
+    const int per_row = p.D / 16, h = blockIdx.y;
     const long long id = (long long)blockIdx.x * kCacheThreads + threadIdx.x, token = id / per_row;
     const int c = static_cast<int>(id % per_row);
     const int b = token < (long long)p.seq.B * p.N ? static_cast<int>(token / p.N) : -1, n = static_cast<int>(token % p.N);
@@ -84,7 +101,7 @@ __global__ void __launch_bounds__(kCacheThreads) append_kernel(const __grid_cons
     int page = 0, position = 0;
     if (there) {
         const Sequence s = sequence_of(p.seq, b, p.N);
-        if (n == 0 && c == 0 && blockIdx.y == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
+        if (n == 0 && c == 0 && h == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
         position = s.start + n;
         there = n < s.count && position >= 0;
         if (there) {
@@ -93,113 +110,89 @@ __global__ void __launch_bounds__(kCacheThreads) append_kernel(const __grid_cons
         }
     }
     if (__ballot_sync(0xffffffffu, there) == 0) return;
-    const int row = position & ((1 << p.seq.page_shift) - 1), h0 = blockIdx.y * HPT;
+    const int row = position & ((1 << p.seq.page_shift) - 1);
     const RowPlace<FORM> place(c, p.rotary.pairs);
     const RowPlace<kInterleaved> plain(c, 0);                    // 16 elements in a row
-    Chunks k[HPT], v[HPT];
-    #pragma unroll
-    for (int i = 0; i < HPT; ++i) {
-        k[i] = v[i] = Chunks{};
-        if (there && h0 + i < p.H) {
-            k[i] = place.load(p.in[0] + b * p.in_sb[0] + (h0 + i) * p.in_sh[0] + n * p.in_sn[0]);
-            v[i] = plain.load(p.in[1] + b * p.in_sb[1] + (h0 + i) * p.in_sh[1] + n * p.in_sn[1]);
-        }
+    const auto outer = outer_place(place, plain);
+    Chunks k = {}, v = {};
+    if (there) {
+        k = outer.load(p.in[0] + b * p.in_sb[0] + h * p.in_sh[0] + n * p.in_sn[0]);
+        v = plain.load(p.in[1] + b * p.in_sb[1] + h * p.in_sh[1] + n * p.in_sn[1]);
     }
-    using T = std::conditional_t<BITS == 4, double, float>;
-    Turner<FORM, BF16, T> turn;
+    Turner<FORM, BF16, std::conditional_t<BITS == 4, double, float>> turn;
     turn.set(p.rotary, c, position);
+    k = turned<FORM>(turn, place, plain, k, stage + threadIdx.x / per_row * p.D);
+    uint8_t* const dst_k = p.cache[0].data + page * p.cache[0].sp + h * p.cache[0].sh + row * p.cache[0].sr;
+    uint8_t* const dst_v = p.cache[1].data + page * p.cache[1].sp + h * p.cache[1].sh + row * p.cache[1].sr;
     if constexpr (BITS == 16) {
-        #pragma unroll
-        for (int i = 0; i < HPT; ++i) {
-            if (!there || h0 + i >= p.H) continue;
-            auto at = [&](const CacheTensor& t) { return reinterpret_cast<uint16_t*>(t.data + page * t.sp + (h0 + i) * t.sh + row * t.sr); };
-            place.store(at(p.cache[0]), turn(k[i]));
-            plain.store(at(p.cache[1]), v[i]);
-        }
+        if (!there) return;
+        outer.store(reinterpret_cast<uint16_t*>(dst_k), k);
+        plain.store(reinterpret_cast<uint16_t*>(dst_v), v);
     } else {
-        __shared__ __align__(16) uint16_t stage[FORM == kScattered ? kCacheThreads * 16 : 8];
-        #pragma unroll 1
-        for (int i = 0; i < HPT; ++i) {
-            Chunks x = turn(k[i]);
-            int first = place.first, second = place.second;
-            if constexpr (FORM == kScattered) {                  // the row's lanes bring its elements in order
-                uint16_t* mine = stage + (threadIdx.x / per_row) * p.D;
-                place.store(mine, x);
-                __syncwarp();
-                x.a = *reinterpret_cast<const uint4*>(mine + plain.first);
-                x.b = *reinterpret_cast<const uint4*>(mine + plain.second);
-                __syncwarp();
-                first = plain.first;
-                second = plain.second;
-            }
-            #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                float scale, zero;
-                const uint2 code = quantise16<BF16>(w ? v[i] : x, per_row, scale, zero);
-                if (!there || h0 + i >= p.H) continue;
-                const CacheTensor& t = p.cache[w];
-                uint8_t* dst = t.data + page * t.sp + (h0 + i) * t.sh + row * t.sr;
-                *reinterpret_cast<uint32_t*>(dst + (w ? plain.first : first) / 2) = code.x;
-                *reinterpret_cast<uint32_t*>(dst + (w ? plain.second : second) / 2) = code.y;
-                if (c == 0) *reinterpret_cast<float2*>(t.scales + page * t.ssp + (h0 + i) * t.ssh + row * t.ssr) = make_float2(scale, zero);
-            }
+        float2 sk, sv;
+        const uint2 ck = quantise16<BF16>(k, per_row, sk.x, sk.y), cv = quantise16<BF16>(v, per_row, sv.x, sv.y);
+        if (!there) return;
+        if constexpr (FORM == kQuarter) {
+            *reinterpret_cast<uint16_t*>(dst_k + place.element(0, false) / 2) = static_cast<uint16_t>(ck.x);
+            *reinterpret_cast<uint16_t*>(dst_k + place.element(4, false) / 2) = static_cast<uint16_t>(ck.x >> 16);
+            *reinterpret_cast<uint16_t*>(dst_k + place.element(0, true) / 2) = static_cast<uint16_t>(ck.y);
+            *reinterpret_cast<uint16_t*>(dst_k + place.element(4, true) / 2) = static_cast<uint16_t>(ck.y >> 16);
+        } else {
+            *reinterpret_cast<uint32_t*>(dst_k + outer.first / 2) = ck.x;
+            *reinterpret_cast<uint32_t*>(dst_k + outer.second / 2) = ck.y;
+        }
+        *reinterpret_cast<uint2*>(dst_v + 8 * c) = cv;
+        if (c == 0) {
+            *reinterpret_cast<float2*>(p.cache[0].scales + page * p.cache[0].ssp + h * p.cache[0].ssh + row * p.cache[0].ssr) = sk;
+            *reinterpret_cast<float2*>(p.cache[1].scales + page * p.cache[1].ssp + h * p.cache[1].ssh + row * p.cache[1].ssr) = sv;
         }
     }
 }
 
-// One thread: 16 elements of a cached row, of HPT heads, of keys and values.  Rows behind a sequence become zero.
-template <bool BF16, int BITS, int HPT>
+// One thread: 16 elements of a cached row of a head (blockIdx.y), of keys and values.  Rows behind a sequence become zero.
+template <bool BF16, int BITS>
 __global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_constant__ ReadParams p) {
-    const int per_row = p.D / 16;
+    const int per_row = p.D / 16, h = blockIdx.y;
     const long long id = (long long)blockIdx.x * kCacheThreads + threadIdx.x, token = id / per_row;
     if (token >= (long long)p.seq.B * p.N) return;
     const int c = static_cast<int>(id % per_row), b = static_cast<int>(token / p.N), n = static_cast<int>(token % p.N);
     const Sequence s = sequence_of(p.seq, b, 0);
-    if (n == 0 && c == 0 && blockIdx.y == 0 && __ldg(p.seq.lengths + b) != s.length) report(p.seq.sticky, kStatusBadLength);
+    if (n == 0 && c == 0 && h == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
     int page = -1;
     if (n < s.length) {
         page = page_of(p.seq, b, n);
         if (page < 0) report(p.seq.sticky, kStatusBadPage);
     }
-    const int row = n & ((1 << p.seq.page_shift) - 1), h0 = blockIdx.y * HPT;
-    Chunks x[HPT][2];
+    const int row = n & ((1 << p.seq.page_shift) - 1);
+    Chunks x[2];
+    uint2 code[2] = {};
+    float2 sc[2] = {};
     #pragma unroll
-    for (int i = 0; i < HPT; ++i) {
-        #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            x[i][w] = Chunks{};
-            if (page < 0 || h0 + i >= p.H) continue;
-            const CacheTensor& t = p.cache[w];
-            const uint8_t* src = t.data + page * t.sp + (h0 + i) * t.sh + row * t.sr;
-            if constexpr (BITS == 16) {
-                x[i][w].a = __ldg(reinterpret_cast<const uint4*>(src) + 2 * c);
-                x[i][w].b = __ldg(reinterpret_cast<const uint4*>(src) + 2 * c + 1);
-            } else {
-                const uint2 code = __ldg(reinterpret_cast<const uint2*>(src) + c);
-                const float2 sc = __ldg(reinterpret_cast<const float2*>(t.scales + page * t.ssp + (h0 + i) * t.ssh + row * t.ssr));
-                x[i][w].a = make_uint4(code.x, code.y, __float_as_uint(sc.x), __float_as_uint(sc.y));
-            }
+    for (int w = 0; w < 2; ++w) {
+        x[w] = Chunks{};
+        if (page < 0) continue;
+        const CacheTensor& t = p.cache[w];
+        const uint8_t* src = t.data + page * t.sp + h * t.sh + row * t.sr;
+        if constexpr (BITS == 16) {
+            x[w].a = __ldg(reinterpret_cast<const uint4*>(src) + 2 * c);
+            x[w].b = __ldg(reinterpret_cast<const uint4*>(src) + 2 * c + 1);
+        } else {
+            code[w] = __ldg(reinterpret_cast<const uint2*>(src) + c);
+            sc[w] = __ldg(reinterpret_cast<const float2*>(t.scales + page * t.ssp + h * t.ssh + row * t.ssr));
         }
     }
     #pragma unroll
-    for (int i = 0; i < HPT; ++i) {
-        if (h0 + i >= p.H) continue;
-        #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            Chunks y = x[i][w];
-            if constexpr (BITS == 4) {
-                const uint32_t code[2] = {y.a.x, y.a.y};
-                const float scale = __uint_as_float(y.a.z), zero = __uint_as_float(y.a.w);
-                float v[16];
-                #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = fmaf(static_cast<float>((code[j >> 3] >> (4 * (j & 7))) & 15u), scale, zero);
-                y.a = narrow8<BF16>(v);
-                y.b = narrow8<BF16>(v + 8);
-            }
-            uint4* dst = reinterpret_cast<uint4*>(p.out[w] + (((long long)b * p.H + h0 + i) * p.N + n) * p.D) + 2 * c;
-            dst[0] = y.a;
-            dst[1] = y.b;
+    for (int w = 0; w < 2; ++w) {
+        if constexpr (BITS == 4) {
+            float v[16];
+            #pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = fmaf(static_cast<float>(((j < 8 ? code[w].x : code[w].y) >> (4 * (j & 7))) & 15u), sc[w].x, sc[w].y);
+            x[w].a = narrow8<BF16>(v);
+            x[w].b = narrow8<BF16>(v + 8);
         }
+        uint4* dst = reinterpret_cast<uint4*>(p.out[w] + (((long long)b * p.H + h) * p.N + n) * p.D) + 2 * c;
+        dst[0] = x[w].a;
+        dst[1] = x[w].b;
     }
 }
 

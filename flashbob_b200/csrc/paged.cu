@@ -89,6 +89,7 @@ template <int V> struct Int { static constexpr int value = V; };
 template <class F> static void with_form(int form, F f) {
     if (form == kHalf) f(Int<kHalf>{});
     else if (form == kInterleaved) f(Int<kInterleaved>{});
+    else if (form == kQuarter) f(Int<kQuarter>{});
     else f(Int<kScattered>{});
 }
 template <class F> static void with_type(int dtype, F f) {
@@ -96,9 +97,11 @@ template <class F> static void with_type(int dtype, F f) {
     else f(std::false_type{});
 }
 
-// Threads of a grid that has enough of them to hide the memory's latency; with more, a thread takes several heads and
-// shares its sines and cosines between them.
-constexpr int64_t kManyThreads = (int64_t)kPagedSms * 2048;
+// Rows x 16 elements from which on a thread turns four heads and shares its sines between them: with fewer, one each is as
+// fast or faster (measured, one head / four, us: 40 rows 2.2 / 2.7, 2,560 rows 2.5 / 3.3, 10,240 rows 3.4 / 3.4, 98,304 rows of 64
+// elements 7.1 / 5.4, 163,840 rows 21.1 / 15.4; eight 18.4).  The cache's kernels do no better with more heads than one (98 MB:
+// 19.6, 19.1 with two, 20.5 with four).
+constexpr int64_t kSharedTurns = (int64_t)kPagedSms * 512;
 
 static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream, const int* lengths = nullptr, const int* counts = nullptr) {
     RotateParams p = {};
@@ -128,7 +131,7 @@ static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream, const
                 const dim3 grid((unsigned)blocks, (heads + HPT - 1) / HPT);
                 rotate_kernel<F, BF, HPT><<<grid, kRotateThreads, 0, stream>>>(p);
             };
-            if (threads * heads >= 4 * kManyThreads) go(Int<4>{});
+            if (threads * heads >= kSharedTurns) go(Int<4>{});
             else go(Int<1>{});
         });
     });
@@ -152,14 +155,9 @@ static int run_append(const bob_sm100_cache* c, const bob_sm100_sequences* s, co
         with_type(c->dtype, [&](auto bf16) {
             constexpr int F = decltype(form)::value;
             constexpr bool BF = decltype(bf16)::value;
-            auto go = [&](auto bits, auto hpt) {
-                constexpr int HPT = decltype(hpt)::value;
-                const dim3 grid((unsigned)blocks, (c->heads + HPT - 1) / HPT);
-                append_kernel<F, BF, decltype(bits)::value, HPT><<<grid, kCacheThreads, 0, stream>>>(p);
-            };
-            const bool many = threads * c->heads >= 4 * kManyThreads;
-            if (c->bits == 16) { if (many) go(Int<16>{}, Int<4>{}); else go(Int<16>{}, Int<1>{}); }
-            else { if (many) go(Int<4>{}, Int<4>{}); else go(Int<4>{}, Int<1>{}); }
+            const dim3 grid((unsigned)blocks, c->heads);
+            if (c->bits == 16) append_kernel<F, BF, 16><<<grid, kCacheThreads, 0, stream>>>(p);
+            else append_kernel<F, BF, 4><<<grid, kCacheThreads, 0, stream>>>(p);
         });
     });
     return launched();
@@ -175,14 +173,9 @@ static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int 
     if (blocks > 0x7fffffffLL) return kBadGeom;
     with_type(c->dtype, [&](auto bf16) {
         constexpr bool BF = decltype(bf16)::value;
-        auto go = [&](auto bits, auto hpt) {
-            constexpr int HPT = decltype(hpt)::value;
-            const dim3 grid((unsigned)blocks, (c->heads + HPT - 1) / HPT);
-            read_kernel<BF, decltype(bits)::value, HPT><<<grid, kCacheThreads, 0, stream>>>(p);
-        };
-        const bool many = threads * c->heads >= 4 * kManyThreads;
-        if (c->bits == 16) { if (many) go(Int<16>{}, Int<2>{}); else go(Int<16>{}, Int<1>{}); }
-        else { if (many) go(Int<4>{}, Int<2>{}); else go(Int<4>{}, Int<1>{}); }
+        const dim3 grid((unsigned)blocks, c->heads);
+        if (c->bits == 16) read_kernel<BF, 16><<<grid, kCacheThreads, 0, stream>>>(p);
+        else read_kernel<BF, 4><<<grid, kCacheThreads, 0, stream>>>(p);
     });
     return launched();
 }

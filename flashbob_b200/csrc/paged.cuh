@@ -23,7 +23,7 @@
 
 namespace bob {
 
-struct PagedParams {
+struct alignas(16) PagedParams {
     bob_sm100_rotary rotary;      // pairs 0: queries are taken as they are
     SequenceParams seq;
     CacheTensor cache[2];
@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                 const uint16_t* from = p.q + seg.b * p.q_sb + h * p.q_sh + i * p.q_sn;
                 if (p.form == kHalf) bring_query<D, BF16, kHalf>(p, dst, rest, from, c, s.start + i);
                 else if (p.form == kInterleaved) bring_query<D, BF16, kInterleaved>(p, dst, rest, from, c, s.start + i);
+                else if (p.form == kQuarter) bring_query<D, BF16, kQuarter>(p, dst, rest, from, c, s.start + i);
                 else bring_query<D, BF16, kScattered>(p, dst, rest, from, c, s.start + i);
             } else {
                 RowPlace<kInterleaved>(c, 0).store(dst, Chunks{});

@@ -4,11 +4,13 @@
 // same map with the angles negated, so one kernel serves forward and every order of backward.
 //
 // Angles: a frequency is kept as the 64-bit fraction of a turn per position.  position * fraction modulo 2^64 is then
-// the exact angle modulo a turn, for any position, in one integer product, and sincospi needs no range reduction;
+// the exact angle modulo a turn, for any position, in one integer product, and a sine needs no range reduction;
 // position * frequency in fp32 is off by 0.004 radians at position 100,000.
 //
 // What bounds it: one read and one write of every element.  A thread turns the same 16 elements (8 pairs) of HPT heads of
-// a token, so its 8 sines and cosines (about 300 instructions) are shared by them and their loads are in flight together.
+// a token, so its 8 sines and cosines are shared by them and their loads are in flight together.  They are the special-
+// function unit's: off by 2^-20.9 at most, a thousandth of the result's rounding in fp16 (with sincospif, four times the
+// instructions, the kernel spent 31 us on 84 MB with one head a thread, 18 with four).
 #pragma once
 
 #include "ptx.cuh"
@@ -17,26 +19,69 @@
 namespace bob {
 
 // How a thread's 16 elements lie in a row.  kHalf: two 16-byte chunks, partners `pairs` elements apart (pairs a multiple of
-// 8); kInterleaved: 16 elements in a row; kScattered: as kHalf for any number of pairs, element by element.
-enum RotaryForm : int { kHalf = 0, kInterleaved = 1, kScattered = 2 };
+// 8); kInterleaved: 16 elements in a row; kQuarter: as kHalf in four 8-byte pieces (pairs a multiple of 4); kScattered: the
+// same for any number of pairs, element by element in shared memory (4 times as slow as the others: 103 us on 168 MB).
+enum RotaryForm : int { kHalf = 0, kInterleaved = 1, kScattered = 2, kQuarter = 3 };
 
 inline int rotary_form(const bob_sm100_rotary* r) {
-    return r->interleaved ? kInterleaved : (r->pairs % 8 ? kScattered : kHalf);
+    return r->interleaved ? kInterleaved : (r->pairs % 8 == 0 ? kHalf : (r->pairs % 4 == 0 ? kQuarter : kScattered));
 }
 
 __device__ __forceinline__ int64_t angle_of(int64_t position, uint64_t turn) {      // 2^-64 turns, in [-1/2, 1/2) turns
     return static_cast<int64_t>(static_cast<uint64_t>(position) * turn);
 }
 __device__ __forceinline__ void turn_factors(int64_t position, uint64_t turn, float factor, float& s, float& c) {
-    // the upper 32 bits: 2^-33 of a turn, 7e-10 radians, far below the rounding of a sine in fp32
-    sincospif(static_cast<float>(static_cast<int32_t>(angle_of(position, turn) >> 32)) * 0x1p-31f, &s, &c);
-    s *= factor;
-    c *= factor;
+    // the upper 32 bits: 2^-33 of a turn, 7e-10 radians
+    const float x = static_cast<float>(static_cast<int32_t>(angle_of(position, turn) >> 32)) * 1.4629180792671596e-9f;      // 2 pi / 2^32
+    s = __sinf(x) * factor;
+    c = __cosf(x) * factor;
 }
+
+// Sine and cosine of a whole turn's 256 parts.
+struct TurnTable { double2 at[256]; };
+constexpr double sine_series(double x) {
+    double term = x, sum = x;
+    for (int k = 1; k < 14; ++k) { term *= -x * x / ((2 * k) * (2 * k + 1)); sum += term; }
+    return sum;
+}
+constexpr double cosine_series(double x) {
+    double term = 1, sum = 1;
+    for (int k = 1; k < 14; ++k) { term *= -x * x / ((2 * k - 1) * (2 * k)); sum += term; }
+    return sum;
+}
+constexpr TurnTable make_turn_table() {
+    TurnTable t = {};
+    for (int i = 0; i < 256; ++i) {
+        const int octant = i / 32, j = i % 32;           // 45 degrees each: series of at most pi / 4
+        const double x = 0.024543692606170259675489401 * (octant % 2 ? 32 - j : j);        // 2 pi / 256
+        const double s = sine_series(x), c = cosine_series(x);
+        const double ss[8] = {s, c, c, s, -s, -c, -c, -s}, cc[8] = {c, s, -s, -c, -c, -s, s, c};
+        t.at[i].x = ss[octant];
+        t.at[i].y = cc[octant];
+    }
+    return t;
+}
+__device__ const TurnTable kTurnTable = make_turn_table();
+
+// In 64 bits: the part of a turn from the table, the rest (at most 2^-9 of a turn, x = 0.0123) by the series
+// x - x^3/6 + x^5/120 and 1 - x^2/2 + x^4/24 - x^6/720, which end below 1e-17.
 __device__ __forceinline__ void turn_factors(int64_t position, uint64_t turn, double factor, double& s, double& c) {
-    sincospi(static_cast<double>(angle_of(position, turn)) * 0x1p-63, &s, &c);
-    s *= factor;
-    c *= factor;
+    const uint64_t a = static_cast<uint64_t>(angle_of(position, turn)) + (1ull << 55);      // to the nearest of 256
+    const double2 t = kTurnTable.at[a >> 56];
+    const double x = static_cast<double>(static_cast<int64_t>(a & ((1ull << 56) - 1)) - (1ll << 55)) * 3.4061215800210806e-19;     // 2 pi / 2^64
+    const double x2 = x * x;
+    const double sx = fma(x * x2, fma(x2, 1.0 / 120, -1.0 / 6), x), cx = fma(x2, fma(x2, fma(x2, -1.0 / 720, 1.0 / 24), -0.5), 1.0);
+    s = factor * fma(t.x, cx, t.y * sx);
+    c = factor * fma(t.y, cx, -(t.x * sx));
+}
+
+// Frequencies 2 i and 2 i + 1 of a rotation that is a kernel parameter, by its address: read as constants, which a warp takes
+// one address at a time, the eight frequencies of every thread took most of the kernel's time (29 us, with them as ordinary
+// loads 15, on 84 MB with one head a thread).
+__device__ __forceinline__ ulonglong2 turn_pair(const bob_sm100_rotary& r, int i) {
+    ulonglong2 x;
+    asm("ld.v2.u64 {%0, %1}, [%2];" : "=l"(x.x), "=l"(x.y) : "l"(r.turns + 2 * i));
+    return x;
 }
 
 // Two 16-byte chunks of a row, as they are loaded.
@@ -57,9 +102,10 @@ struct RowPlace {
             second = first + 8;
         }
     }
-    // kScattered: the elements of pair 8 c + j
+    // kScattered, kQuarter: the elements of pair 8 c + j
     __device__ __forceinline__ int element(int j, bool partner) const {
         const int i = 8 * c + j;
+        if (FORM == kQuarter) return i < pairs ? i + (partner ? pairs : 0) : 2 * i + (partner ? 4 : 0);     // (j = 0 or 4)
         return i < pairs ? i + (partner ? pairs : 0) : 2 * i + (partner ? 1 : 0);
     }
     __device__ __forceinline__ Chunks load(const uint16_t* row) const {
@@ -73,9 +119,14 @@ struct RowPlace {
             }
             x.a = make_uint4(w[0], w[1], w[2], w[3]);
             x.b = make_uint4(w[4], w[5], w[6], w[7]);
+        } else if constexpr (FORM == kQuarter) {
+            const uint2 a0 = *reinterpret_cast<const uint2*>(row + element(0, false)), a1 = *reinterpret_cast<const uint2*>(row + element(4, false));
+            const uint2 b0 = *reinterpret_cast<const uint2*>(row + element(0, true)), b1 = *reinterpret_cast<const uint2*>(row + element(4, true));
+            x.a = make_uint4(a0.x, a0.y, a1.x, a1.y);
+            x.b = make_uint4(b0.x, b0.y, b1.x, b1.y);
         } else {
-            x.a = __ldg(reinterpret_cast<const uint4*>(row + first));
-            x.b = __ldg(reinterpret_cast<const uint4*>(row + second));
+            x.a = *reinterpret_cast<const uint4*>(row + first);
+            x.b = *reinterpret_cast<const uint4*>(row + second);
         }
         return x;
     }
@@ -89,6 +140,11 @@ struct RowPlace {
                 row[element(2 * j, true)] = static_cast<uint16_t>(w[4 + j]);
                 row[element(2 * j + 1, true)] = static_cast<uint16_t>(w[4 + j] >> 16);
             }
+        } else if constexpr (FORM == kQuarter) {
+            *reinterpret_cast<uint2*>(row + element(0, false)) = make_uint2(x.a.x, x.a.y);
+            *reinterpret_cast<uint2*>(row + element(4, false)) = make_uint2(x.a.z, x.a.w);
+            *reinterpret_cast<uint2*>(row + element(0, true)) = make_uint2(x.b.x, x.b.y);
+            *reinterpret_cast<uint2*>(row + element(4, true)) = make_uint2(x.b.z, x.b.w);
         } else {
             *reinterpret_cast<uint4*>(row + first) = x.a;
             *reinterpret_cast<uint4*>(row + second) = x.b;
@@ -131,9 +187,11 @@ struct Turner {
     __device__ __forceinline__ void set(const bob_sm100_rotary& r, int place, int64_t position) {
         active = min(8, max(0, r.pairs - 8 * place));
         #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            s[j] = 0; c[j] = 1;
-            if (j < active) turn_factors(position, r.turns[8 * place + j], static_cast<T>(r.factor), s[j], c[j]);
+        for (int j = 0; j < 8; j += 2) {
+            const ulonglong2 turn = turn_pair(r, 4 * place + j / 2);         // (64 of them are there)
+            s[j] = s[j + 1] = 0; c[j] = c[j + 1] = 1;
+            if (j < active) turn_factors(position, turn.x, static_cast<T>(r.factor), s[j], c[j]);
+            if (j + 1 < active) turn_factors(position, turn.y, static_cast<T>(r.factor), s[j + 1], c[j + 1]);
         }
     }
     static constexpr int STEP = FORM == kInterleaved ? 2 : 1, PARTNER = FORM == kInterleaved ? 1 : 8;
@@ -174,14 +232,38 @@ struct Turner {
     }
 };
 
+// Turns a row's 16 elements that were loaded in order (kScattered: through `stage`, the row's place in shared memory; the
+// lanes of a row are in one warp, and all lanes call this) or as `place` loads them.
+template <int FORM, class TURN>
+__device__ __forceinline__ Chunks turned(const TURN& turn, const RowPlace<FORM>& place, const RowPlace<kInterleaved>& plain, Chunks x, uint16_t* stage) {
+    if constexpr (FORM == kScattered) {
+        plain.store(stage, x);
+        __syncwarp();
+        const Chunks y = turn(place.load(stage));
+        __syncwarp();
+        place.store(stage, y);
+        __syncwarp();
+        x = plain.load(stage);
+        __syncwarp();
+        return x;
+    } else {
+        return turn(x);
+    }
+}
+// The place of the 16 elements that a thread loads from, and stores to, global memory.
+template <int FORM>
+__device__ __forceinline__ auto outer_place(const RowPlace<FORM>& place, const RowPlace<kInterleaved>& plain) {
+    if constexpr (FORM == kScattered) return plain; else return place;
+}
+
 struct RotateTensor {
     const uint16_t* in; long long in_sb, in_sh, in_sn;      // element strides: batch, head, row
     uint16_t* out;                                          // contiguous [B, H, N, D]
     int H;
 };
 
-struct RotateParams {
-    bob_sm100_rotary rotary;
+struct alignas(16) RotateParams {
+    bob_sm100_rotary rotary;      // (first: its frequencies are 16-byte aligned)
     RotateTensor t[2];
     int B, N, D;
     const void* positions; int wide; long long pos_sb, pos_sn;   // int64 or int32; null: first + row
@@ -197,9 +279,12 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
     const int per_row = p.D / 16;
     const long long id = (long long)blockIdx.x * kRotateThreads + threadIdx.x;
     const long long token = id / per_row;
-    if (token >= (long long)p.B * p.N) return;
-    const int c = static_cast<int>(id % per_row), b = static_cast<int>(token / p.N), n = static_cast<int>(token % p.N);
+    const bool there = token < (long long)p.B * p.N;             // (the others stay for their warp)
+    const int c = static_cast<int>(id % per_row), b = there ? static_cast<int>(token / p.N) : 0, n = there ? static_cast<int>(token % p.N) : 0;
+    __shared__ __align__(16) uint16_t stage[FORM == kScattered ? kRotateThreads * 16 : 8];
     const RowPlace<FORM> place(c, p.rotary.pairs);
+    const RowPlace<kInterleaved> plain(c, 0);                    // 16 elements in a row
+    const auto outer = outer_place(place, plain);
     const int h0 = blockIdx.y * HPT;
     Chunks x[HPT];
     #pragma unroll
@@ -209,7 +294,7 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
         const RotateTensor& t = p.t[second];
         const int th = second ? h - p.t[0].H : h;
         x[k] = Chunks{};
-        if (th < t.H) x[k] = place.load(t.in + b * t.in_sb + th * t.in_sh + n * t.in_sn);
+        if (there && th < t.H) x[k] = outer.load(t.in + b * t.in_sb + th * t.in_sh + n * t.in_sn);
     }
     int64_t position = p.first + n;
     if (p.lengths) {
@@ -226,7 +311,8 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
         const bool second = h >= p.t[0].H;
         const RotateTensor& t = p.t[second];
         const int th = second ? h - p.t[0].H : h;
-        if (th < t.H) place.store(t.out + (((long long)b * t.H + th) * p.N + n) * p.D, turn(x[k]));
+        const Chunks y = turned<FORM>(turn, place, plain, x[k], stage + threadIdx.x / per_row * p.D);
+        if (there && th < t.H) outer.store(t.out + (((long long)b * t.H + th) * p.N + n) * p.D, y);
     }
 }
 

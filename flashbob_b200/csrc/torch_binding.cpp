@@ -626,6 +626,118 @@ Sequences sequence_args(PyObject* const* a) {
     return r;
 }
 
+// The argument checks of the operations on positions and the paged cache in their common, valid form, as common_call has
+// them for the operator: what is not plainly valid is left to the Python side, whose checks say what is allowed.
+bool common_heads(const Tensor& t) {
+    const auto type = t.scalar_type();
+    if (!t.is_cuda() || t.dim() != 4 || (type != at::kHalf && type != at::kBFloat16) || t.numel() <= 0 || t._fw_grad(0).defined()) return false;
+    const int64_t D = t.size(3);
+    return (D == 32 || D == 64 || D == 128) && t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX && t.size(2) <= (1 << 28);
+}
+bool common_rotary(PyObject* packed, PyObject* head_dim, int64_t D) {
+    return packed == Py_None || (PyBytes_CheckExact(packed) && is_int(head_dim) && PyLong_AsLongLong(head_dim) == D);
+}
+bool common_rows(const Tensor& t, const Tensor& cache_k, PyObject* scales, PyObject* bf16) {
+    return common_heads(t) && t.device() == cache_k.device() && t.scalar_type() == (bf16 == Py_True ? at::kBFloat16 : at::kHalf) &&
+           t.size(3) == cache_k.size(3) * (scales == Py_None ? 1 : 2) && !(t.requires_grad() && at::GradMode::is_enabled());
+}
+bool common_sequences(PyObject* const* a, const Tensor& cache_k, int64_t B) {
+    for (int i = 0; i < 3; ++i) {
+        if (i == 2 && a[i] == Py_None) continue;
+        if (!THPVariable_Check(a[i])) return false;
+        const Tensor& t = THPVariable_Unpack(a[i]);
+        if (t.scalar_type() != at::kInt || t.dim() != (i ? 1 : 2) || t.numel() <= 0 || t.device() != cache_k.device() || t.size(0) != B) return false;
+    }
+    return THPVariable_Unpack(a[0]).size(1) * cache_k.size(2) <= (1 << 28);
+}
+
+// try_rotate(q, k or None, rotary, its head_dim, positions or None, offset, check_status) -> (q, k), or None
+PyObject* py_try_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    want(n, 7);
+    if (torch::jit::tracer::isTracing()) Py_RETURN_NONE;
+    std::array<Tensor, 2> x;
+    for (int i = 0; i < 2; ++i) {
+        if (i == 1 && a[i] == Py_None) continue;
+        if (!THPVariable_Check(a[i])) Py_RETURN_NONE;
+        x[i] = THPVariable_Unpack(a[i]);
+        if (!common_heads(x[i])) Py_RETURN_NONE;
+    }
+    const Tensor& q = x[0];
+    if (x[1].defined() && (x[1].device() != q.device() || x[1].scalar_type() != q.scalar_type() || x[1].size(0) != q.size(0) ||
+                           x[1].size(2) != q.size(2) || x[1].size(3) != q.size(3))) Py_RETURN_NONE;
+    if (a[2] == Py_None || !common_rotary(a[2], a[3], q.size(3)) || !is_int(a[5])) Py_RETURN_NONE;
+    Rotation r;
+    int overflow = 0;
+    r.first = PyLong_AsLongLongAndOverflow(a[5], &overflow);
+    if (overflow || r.first < 0 || r.first >= (int64_t(1) << 62)) Py_RETURN_NONE;
+    Tensor positions;
+    if (a[4] != Py_None) {
+        if (!THPVariable_Check(a[4]) || r.first) Py_RETURN_NONE;
+        positions = THPVariable_Unpack(a[4]);
+        const auto type = positions.scalar_type();
+        const int64_t dim = positions.dim();
+        if ((type != at::kLong && type != at::kInt) || positions.device() != q.device() || dim < 1 || dim > 2 || positions.size(-1) != q.size(2) ||
+            (dim == 2 && positions.size(0) != q.size(0))) Py_RETURN_NONE;
+    }
+    r.rotary = rotary_arg(a[2]);
+    r.check_status = a[6] == Py_True;
+    const std::array<Tensor, 2> y = without_gil([&] { return rotate(x, positions, r); });
+    return tuple_of({y[0], y[1]});
+    END_HANDLE_TH_ERRORS
+}
+
+// try_append(k, v, <cache>, <sequences>, rotary or None, its head_dim, check_status) -> whether it was done
+PyObject* py_try_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    want(n, 13);
+    if (torch::jit::tracer::isTracing() || !THPVariable_Check(a[0]) || !THPVariable_Check(a[1])) Py_RETURN_FALSE;
+    const Tensor &k = THPVariable_Unpack(a[0]), &v = THPVariable_Unpack(a[1]), &ck = THPVariable_Unpack(a[2]);
+    if (!common_rows(k, ck, a[4], a[6]) || !common_rows(v, ck, a[4], a[6]) || k.sizes() != v.sizes() || k.size(1) != ck.size(1) ||
+        !common_sequences(a + 7, ck, k.size(0)) || !common_rotary(a[10], a[11], k.size(3))) Py_RETURN_FALSE;
+    Untracked untracked;
+    const c10::cuda::CUDAGuard device(k.device());
+    Cache cache = cache_args(a + 2);
+    const Sequences seq = sequence_args(a + 7);
+    const bob_sm100_rotary rotary = rotary_arg(a[10]);
+    const bool check = a[12] == Py_True;
+    without_gil([&] { run_append(k, v, cache, seq, rotary, check); return 0; });
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// try_paged(q, <cache>, <sequences>, rotary or None, its head_dim, is_causal, scale, window_size, check_status) -> out, or None
+PyObject* py_try_paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    want(n, 15);
+    if (torch::jit::tracer::isTracing() || !THPVariable_Check(a[0])) Py_RETURN_NONE;
+    const Tensor &q = THPVariable_Unpack(a[0]), &ck = THPVariable_Unpack(a[1]);
+    if (!common_rows(q, ck, a[3], a[5])) Py_RETURN_NONE;
+    const int64_t group = q.size(1) / ck.size(1);
+    if (group * ck.size(1) != q.size(1) || group < 1 || group > 32 || !common_sequences(a + 6, ck, q.size(0)) || !common_rotary(a[9], a[10], q.size(3)))
+        Py_RETURN_NONE;
+    if (!PyBool_Check(a[11]) || !is_int(a[13])) Py_RETURN_NONE;
+    const bool causal = a[11] == Py_True;
+    int overflow = 0;
+    const int64_t window = PyLong_AsLongLongAndOverflow(a[13], &overflow);
+    if (overflow || window < 0 || window > (1 << 28) || (!causal && (window > 0 || a[9] != Py_None))) Py_RETURN_NONE;
+    std::optional<double> scale;
+    if (a[12] != Py_None) {
+        if (!PyFloat_CheckExact(a[12])) Py_RETURN_NONE;
+        const float s = static_cast<float>(PyFloat_AS_DOUBLE(a[12]));
+        if (!(s > 0) || !std::isfinite(s)) Py_RETURN_NONE;
+        scale = PyFloat_AS_DOUBLE(a[12]);
+    }
+    Untracked untracked;
+    const c10::cuda::CUDAGuard device(q.device());
+    const Cache cache = cache_args(a + 1);
+    const Sequences seq = sequence_args(a + 6);
+    const bob_sm100_rotary rotary = rotary_arg(a[9]);
+    const bool check = a[14] == Py_True;
+    return THPVariable_Wrap(without_gil([&] { return run_paged(q, cache, seq, rotary, causal, window, scale, check); }));
+    END_HANDLE_TH_ERRORS
+}
+
 // rotate(q, k or None, rotary, positions or None, first, check_status) -> (q, k)
 PyObject* py_rotate(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -723,6 +835,7 @@ PyMethodDef methods[] = {
     BOB_METHOD("try_sdpa", py_try_sdpa), BOB_METHOD("sdpa", py_sdpa), BOB_METHOD("forward", py_forward),
     BOB_METHOD("first_backward", py_first), BOB_METHOD("second_backward", py_second), BOB_METHOD("bind", py_bind),
     BOB_METHOD("rotate", py_rotate), BOB_METHOD("cache_append", py_append), BOB_METHOD("cache_read", py_read), BOB_METHOD("paged", py_paged),
+    BOB_METHOD("try_rotate", py_try_rotate), BOB_METHOD("try_append", py_try_append), BOB_METHOD("try_paged", py_try_paged),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "bob_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -48,7 +48,7 @@ class PagedCache:
     dimension, rows that start at multiples of 16 bytes (scales: 8) and no two rows in one place.
     """
 
-    __slots__ = ("k", "v", "k_scales", "v_scales", "dtype", "bits", "_args")
+    __slots__ = ("k", "v", "k_scales", "v_scales", "dtype", "bits", "_args", "_on_gpu")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, *, k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None,
                  dtype: torch.dtype | None = None):
@@ -96,6 +96,7 @@ class PagedCache:
                 reach = s * (n - 1) + reach
         self.k, self.v, self.k_scales, self.v_scales, self.dtype = k, v, k_scales, v_scales, dtype
         self._args = (k, v, k_scales, v_scales, dtype == torch.bfloat16)
+        self._on_gpu = k.is_cuda
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, page_size: int, head_dim: int, *, dtype: torch.dtype = torch.bfloat16, bits: int = 16,
@@ -134,6 +135,17 @@ class PagedCache:
 # --------------------------------------------------------------------------------------
 # argument checks
 # --------------------------------------------------------------------------------------
+def _plain_rotary(rotary):
+    """The native calls' form of `rotary`; None if it is none of the kind."""
+    if rotary is None:
+        return None, None
+    return (rotary._packed, rotary.head_dim) if isinstance(rotary, Rotary) else None
+
+
+def _native_call(cache, turn_args) -> bool:
+    return turn_args is not None and isinstance(cache, PagedCache) and cache._on_gpu and not torch._C._are_functorch_transforms_active()
+
+
 def _check_cache(cache) -> None:
     if not isinstance(cache, PagedCache):
         raise TypeError(f"cache must be a PagedCache, got {type(cache).__name__}")
@@ -220,6 +232,10 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, page_table: t
     looked at, and no other row of the cache changes.  Pages may be shared between sequences as long as nothing is
     written to them: two new rows for one place leave either there.
     """
+    # The usual valid CUDA call is recognised natively; everything else takes the checks below.
+    turn_args = _plain_rotary(rotary)
+    if _native_call(cache, turn_args) and _native.load().try_append(k, v, *cache._args, page_table, lengths, counts, *turn_args, ops._CHECK_STATUS):
+        return
     check_plain_call()
     _check_cache(cache)
     _check_rows("k", k, cache)
@@ -283,6 +299,11 @@ def sdpa_paged(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, len
     Key and value rows that no query of its sequence attends to have no part in the result, whatever they hold.  H_Q is a multiple of
     H_KV, up to 32 times.
     """
+    turn_args = _plain_rotary(rotary)
+    if _native_call(cache, turn_args):
+        out = _native.load().try_paged(q, *cache._args, page_table, lengths, counts, *turn_args, is_causal, scale, window_size, ops._CHECK_STATUS)
+        if out is not None:
+            return out
     check_plain_call()
     _check_cache(cache)
     _check_rows("q", q, cache)

@@ -179,6 +179,11 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, rotary: Rotary, *, pos
     Row n sits at position offset + n, or at positions[n] or positions[b, n] (int32 or int64, any values).  Differentiable
     any number of times with respect to q and k.  CUDA tensors must be fp16 or bf16 with D in {32, 64, 128}.
     """
+    # The usual valid CUDA call is recognised natively; everything else takes the checks below.
+    if isinstance(rotary, Rotary) and isinstance(q, torch.Tensor) and q.is_cuda and not torch._C._are_functorch_transforms_active():
+        out = _native.load().try_rotate(q, k, rotary._packed, rotary.head_dim, positions, offset, ops._CHECK_STATUS)
+        if out is not None:
+            return out
     check_plain_call()
     check_heads("q", q)
     packed = check_rotary(rotary, q.shape[3])

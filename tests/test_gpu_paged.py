@@ -113,7 +113,7 @@ def test_one_long_sequence_in_many_parts(bits):
 
 
 @pytest.mark.parametrize("rotary", [dict(rotary_dim=2), dict(rotary_dim=6), dict(rotary_dim=12, interleaved=True), dict(rotary_dim=16), dict(rotary_dim=64),
-                                    dict(rotary_dim=50), dict(scaling="linear", factor=2.0), dict(scaling="ntk", factor=4.0, interleaved=True)])
+                                    dict(rotary_dim=50), dict(rotary_dim=24), dict(scaling="linear", factor=2.0), dict(scaling="ntk", factor=4.0, interleaved=True)])
 @pytest.mark.parametrize("bits", [16, 4])
 def test_forms_of_rotation_in_append_and_attention(rotary, bits):
     D, dtype = 64, torch.float16

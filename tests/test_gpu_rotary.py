@@ -10,7 +10,7 @@ from flashbob_b200.rotary import Rotary, apply_rotary
 
 pytestmark = pytest.mark.gpu
 
-FORMS = [dict(), dict(interleaved=True), dict(rotary_dim=16), dict(rotary_dim=2), dict(rotary_dim=10), dict(rotary_dim=18, interleaved=True), dict(rotary_dim=28),
+FORMS = [dict(), dict(interleaved=True), dict(rotary_dim=16), dict(rotary_dim=2), dict(rotary_dim=10), dict(rotary_dim=18, interleaved=True), dict(rotary_dim=28), dict(rotary_dim=8),
          dict(scaling="yarn", factor=4.0, original_length=512), dict(scaling="ntk", factor=2.0), dict(scaling="linear", factor=8.0, theta=500.0)]
 TINY = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -25}
 
