@@ -27,7 +27,7 @@ struct alignas(16) AppendParams {
     SequenceParams seq;
     CacheTensor cache[2];                                        // keys, values
     const uint16_t* in[2]; long long in_sb[2], in_sh[2], in_sn[2];
-    int H, N, D;
+    int H, N, D, heads_each;
 };
 
 struct ReadParams {
@@ -41,8 +41,10 @@ __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.N
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
 // Quantises a row of D = 16 * per_row elements, 16 of them in each of per_row neighbouring lanes (all lanes of the warp
-// call this).  Every operation is rounded to nearest in fp32, so the codes are those of the formula in plain arithmetic: the
-// product with the reciprocal stands for the quotient only where both round to the same code for certain.
+// call this).  Every operation is rounded to nearest in fp32, so the codes are those of the formula in plain arithmetic.  The
+// quotient is Markstein's: with y the rounded reciprocal of b, q = a y and r = a - b q (one rounding, exact), q + r y is
+// a / b correctly rounded.  (Rows of 8-bit mantissas have quotients on the border between two codes all the time, so an
+// approximate quotient with a division for those near a border costs more: 65 us on 63 MB against 44 without.)
 template <bool BF16>
 __device__ __forceinline__ uint2 quantise16(const Chunks& x, int per_row, float& scale, float& zero) {
     float v[16];
@@ -63,20 +65,20 @@ __device__ __forceinline__ uint2 quantise16(const Chunks& x, int per_row, float&
     constexpr float kShift = 12582912.f;
     constexpr uint32_t kWhole = 0x4b400000u, kExtra = kWhole * 0x11111111u;
     uint32_t word[2] = {0, 0};
-    float border = 0.f;                                          // how far a quotient is from its code: near a border, 1/2
-    #pragma unroll
-    for (int i = 15; i >= 0; --i) {
-        const float q = __fmul_rn(__fsub_rn(v[i], lo), inv);     // off by 3 * 2^-24 of at most 15
-        const float r = __fadd_rn(q, kShift);
-        border = max_nan(border, fabsf(__fsub_rn(q, __fsub_rn(r, kShift))));
-        word[i >> 3] = word[i >> 3] * 16 + __float_as_uint(r);
-    }
-    if (!(border < 0.49999f)) {                                  // (or no number)
-        word[0] = word[1] = 0;
+    if (scale > 1e-30f && scale < 1e30f) {                       // nothing here overflows or gets too small to be exact
+        #pragma unroll
+        for (int i = 15; i >= 0; --i) {
+            const float d = __fsub_rn(v[i], lo), q = __fmul_rn(d, inv);
+            word[i >> 3] = word[i >> 3] * 16 + __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-q, scale, d), inv, q), kShift));
+        }
+    } else {
+        const uint32_t w[8] = {x.a.x, x.a.y, x.a.z, x.a.w, x.b.x, x.b.y, x.b.z, x.b.w};
         #pragma unroll 1
         for (int i = 15; i >= 0; --i) {
-            const uint32_t w = (i < 8 ? (&x.a.x) : (&x.b.x))[(i % 8) / 2];
-            const uint16_t bits = static_cast<uint16_t>(i % 2 ? w >> 16 : w);
+            uint32_t pair = w[0];
+            #pragma unroll
+            for (int j = 1; j < 8; ++j) pair = i / 2 == j ? w[j] : pair;
+            const uint16_t bits = static_cast<uint16_t>(i % 2 ? pair >> 16 : pair);
             const float e = BF16 ? __uint_as_float(static_cast<uint32_t>(bits) << 16) : __half2float(__ushort_as_half(bits));
             const uint32_t r = __float_as_uint(__fadd_rn(__fdiv_rn(__fsub_rn(e, lo), scale), kShift));
             if (i < 8) word[0] = word[0] * 16 + r; else word[1] = word[1] * 16 + r;
@@ -87,12 +89,12 @@ __device__ __forceinline__ uint2 quantise16(const Chunks& x, int per_row, float&
 
 constexpr int kCacheThreads = 256;
 
-// One thread: 16 elements of a new row of a head (blockIdx.y), of keys and values.  BITS 4 turns the keys in 64 bits: a
+// One thread: 16 elements of a new row, of one head (blockIdx.y) or, with the same sines, of several: keys and values.  BITS 4 turns the keys in 64 bits: a
 // rounding that falls the other way can move an element by a whole step of the 4-bit row, 1/15 of its range.
 template <int FORM, bool BF16, int BITS>
 __global__ void __launch_bounds__(kCacheThreads) append_kernel(const __grid_constant__ AppendParams p) {
     __shared__ __align__(16) uint16_t stage[FORM == kScattered ? kCacheThreads * 16 : 8];
-    const int per_row = p.D / 16, h = blockIdx.y;
+    const int each = BITS == 4 ? p.heads_each : 1, per_row = p.D / 16, h0 = blockIdx.y * each, h1 = min(p.H, h0 + each);
     const long long id = (long long)blockIdx.x * kCacheThreads + threadIdx.x, token = id / per_row;
     const int c = static_cast<int>(id % per_row);
     const int b = token < (long long)p.seq.B * p.N ? static_cast<int>(token / p.N) : -1, n = static_cast<int>(token % p.N);
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(kCacheThreads) append_kernel(const __grid_cons
     int page = 0, position = 0;
     if (there) {
         const Sequence s = sequence_of(p.seq, b, p.N);
-        if (n == 0 && c == 0 && h == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
+        if (n == 0 && c == 0 && h0 == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
         position = s.start + n;
         there = n < s.count && position >= 0;
         if (there) {
@@ -114,37 +116,48 @@ __global__ void __launch_bounds__(kCacheThreads) append_kernel(const __grid_cons
     const RowPlace<FORM> place(c, p.rotary.pairs);
     const RowPlace<kInterleaved> plain(c, 0);                    // 16 elements in a row
     const auto outer = outer_place(place, plain);
-    Chunks k = {}, v = {};
-    if (there) {
-        k = outer.load(p.in[0] + b * p.in_sb[0] + h * p.in_sh[0] + n * p.in_sn[0]);
-        v = plain.load(p.in[1] + b * p.in_sb[1] + h * p.in_sh[1] + n * p.in_sn[1]);
-    }
+    const uint16_t* src_k = p.in[0] + b * p.in_sb[0] + n * p.in_sn[0];
+    const uint16_t* src_v = p.in[1] + b * p.in_sb[1] + n * p.in_sn[1];
+    uint8_t* const page_k = p.cache[0].data + page * p.cache[0].sp + row * p.cache[0].sr;
+    uint8_t* const page_v = p.cache[1].data + page * p.cache[1].sp + row * p.cache[1].sr;
+    auto fetch = [&](int h, Chunks& k, Chunks& v) {
+        k = v = Chunks{};
+        if (!there) return;
+        k = outer.load(src_k + h * p.in_sh[0]);
+        v = plain.load(src_v + h * p.in_sh[1]);
+    };
+    Chunks next_k, next_v;
+    fetch(h0, next_k, next_v);
     Turner<FORM, BF16, std::conditional_t<BITS == 4, double, float>> turn;
     turn.set(p.rotary, c, position);
-    k = turned<FORM>(turn, place, plain, k, stage + threadIdx.x / per_row * p.D);
-    uint8_t* const dst_k = p.cache[0].data + page * p.cache[0].sp + h * p.cache[0].sh + row * p.cache[0].sr;
-    uint8_t* const dst_v = p.cache[1].data + page * p.cache[1].sp + h * p.cache[1].sh + row * p.cache[1].sr;
-    if constexpr (BITS == 16) {
-        if (!there) return;
-        outer.store(reinterpret_cast<uint16_t*>(dst_k), k);
-        plain.store(reinterpret_cast<uint16_t*>(dst_v), v);
-    } else {
-        float2 sk, sv;
-        const uint2 ck = quantise16<BF16>(k, per_row, sk.x, sk.y), cv = quantise16<BF16>(v, per_row, sv.x, sv.y);
-        if (!there) return;
-        if constexpr (FORM == kQuarter) {
-            *reinterpret_cast<uint16_t*>(dst_k + place.element(0, false) / 2) = static_cast<uint16_t>(ck.x);
-            *reinterpret_cast<uint16_t*>(dst_k + place.element(4, false) / 2) = static_cast<uint16_t>(ck.x >> 16);
-            *reinterpret_cast<uint16_t*>(dst_k + place.element(0, true) / 2) = static_cast<uint16_t>(ck.y);
-            *reinterpret_cast<uint16_t*>(dst_k + place.element(4, true) / 2) = static_cast<uint16_t>(ck.y >> 16);
+    #pragma unroll 1
+    for (int h = h0; h < h1; ++h) {
+        const Chunks k = turned<FORM>(turn, place, plain, next_k, stage + threadIdx.x / per_row * p.D), v = next_v;
+        if (h + 1 < h1) fetch(h + 1, next_k, next_v);
+        uint8_t* const dst_k = page_k + h * p.cache[0].sh;
+        uint8_t* const dst_v = page_v + h * p.cache[1].sh;
+        if constexpr (BITS == 16) {
+            if (!there) continue;
+            outer.store(reinterpret_cast<uint16_t*>(dst_k), k);
+            plain.store(reinterpret_cast<uint16_t*>(dst_v), v);
         } else {
-            *reinterpret_cast<uint32_t*>(dst_k + outer.first / 2) = ck.x;
-            *reinterpret_cast<uint32_t*>(dst_k + outer.second / 2) = ck.y;
-        }
-        *reinterpret_cast<uint2*>(dst_v + 8 * c) = cv;
-        if (c == 0) {
-            *reinterpret_cast<float2*>(p.cache[0].scales + page * p.cache[0].ssp + h * p.cache[0].ssh + row * p.cache[0].ssr) = sk;
-            *reinterpret_cast<float2*>(p.cache[1].scales + page * p.cache[1].ssp + h * p.cache[1].ssh + row * p.cache[1].ssr) = sv;
+            float2 sk, sv;
+            const uint2 ck = quantise16<BF16>(k, per_row, sk.x, sk.y), cv = quantise16<BF16>(v, per_row, sv.x, sv.y);
+            if (!there) continue;
+            if constexpr (FORM == kQuarter) {
+                *reinterpret_cast<uint16_t*>(dst_k + place.element(0, false) / 2) = static_cast<uint16_t>(ck.x);
+                *reinterpret_cast<uint16_t*>(dst_k + place.element(4, false) / 2) = static_cast<uint16_t>(ck.x >> 16);
+                *reinterpret_cast<uint16_t*>(dst_k + place.element(0, true) / 2) = static_cast<uint16_t>(ck.y);
+                *reinterpret_cast<uint16_t*>(dst_k + place.element(4, true) / 2) = static_cast<uint16_t>(ck.y >> 16);
+            } else {
+                *reinterpret_cast<uint32_t*>(dst_k + outer.first / 2) = ck.x;
+                *reinterpret_cast<uint32_t*>(dst_k + outer.second / 2) = ck.y;
+            }
+            *reinterpret_cast<uint2*>(dst_v + 8 * c) = cv;
+            if (c == 0) {
+                *reinterpret_cast<float2*>(p.cache[0].scales + page * p.cache[0].ssp + h * p.cache[0].ssh + row * p.cache[0].ssr) = sk;
+                *reinterpret_cast<float2*>(p.cache[1].scales + page * p.cache[1].ssp + h * p.cache[1].ssh + row * p.cache[1].ssr) = sv;
+            }
         }
     }
 }

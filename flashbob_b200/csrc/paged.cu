@@ -99,8 +99,7 @@ template <class F> static void with_type(int dtype, F f) {
 
 // Rows x 16 elements from which on a thread turns four heads and shares its sines between them: with fewer, one each is as
 // fast or faster (measured, one head / four, us: 40 rows 2.2 / 2.7, 2,560 rows 2.5 / 3.3, 10,240 rows 3.4 / 3.4, 98,304 rows of 64
-// elements 7.1 / 5.4, 163,840 rows 21.1 / 15.4; eight 18.4).  The cache's kernels do no better with more heads than one (98 MB:
-// 19.6, 19.1 with two, 20.5 with four).
+// elements 7.1 / 5.4, 163,840 rows 21.1 / 15.4; eight 18.4). 
 constexpr int64_t kSharedTurns = (int64_t)kPagedSms * 512;
 
 static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream, const int* lengths = nullptr, const int* counts = nullptr) {
@@ -149,13 +148,20 @@ static int run_append(const bob_sm100_cache* c, const bob_sm100_sequences* s, co
         p.in_sb[w] = strides[w][0]; p.in_sh[w] = strides[w][1]; p.in_sn[w] = strides[w][2];
     }
     p.H = c->heads; p.N = N; p.D = c->D;
-    const int64_t threads = (int64_t)s->B * N * (c->D / 16), blocks = (threads + kCacheThreads - 1) / kCacheThreads;
+    const int64_t threads = (int64_t)s->B * N * (c->D / 16);
+    // 4 bits: several heads to a thread, which share its 64-bit sines, where enough threads are left (measured, one / two / four /
+    // eight heads, us: 512 rows of 128 elements 4.6 / 5.8 / 8.4 / 13.4, 96,000 rows 42.7 / 34.2 / 31.3 / 31.0, 128,032 rows of 64
+    // 28.0 / 23.3 / 21.6 / 19.8).  16 bits: one (98 MB 19.5; with two 19.1, four 20.5).
+    p.heads_each = 1;
+    if (c->bits == 4)
+        while (p.heads_each < 8 && threads * c->heads / (2 * p.heads_each) >= kPagedSms * 384) p.heads_each *= 2;
+    const int64_t blocks = (threads + kCacheThreads - 1) / kCacheThreads;
     if (blocks > 0x7fffffffLL) return kBadGeom;
     with_form(rotary_form(r), [&](auto form) {
         with_type(c->dtype, [&](auto bf16) {
             constexpr int F = decltype(form)::value;
             constexpr bool BF = decltype(bf16)::value;
-            const dim3 grid((unsigned)blocks, c->heads);
+            const dim3 grid((unsigned)blocks, (c->heads + p.heads_each - 1) / p.heads_each);
             if (c->bits == 16) append_kernel<F, BF, 16><<<grid, kCacheThreads, 0, stream>>>(p);
             else append_kernel<F, BF, 4><<<grid, kCacheThreads, 0, stream>>>(p);
         });

@@ -30,11 +30,11 @@ inline int rotary_form(const bob_sm100_rotary* r) {
 __device__ __forceinline__ int64_t angle_of(int64_t position, uint64_t turn) {      // 2^-64 turns, in [-1/2, 1/2) turns
     return static_cast<int64_t>(static_cast<uint64_t>(position) * turn);
 }
-__device__ __forceinline__ void turn_factors(int64_t position, uint64_t turn, float factor, float& s, float& c) {
+__device__ __forceinline__ void turn_factors(int64_t position, uint64_t turn, float& s, float& c) {
     // the upper 32 bits: 2^-33 of a turn, 7e-10 radians
     const float x = static_cast<float>(static_cast<int32_t>(angle_of(position, turn) >> 32)) * 1.4629180792671596e-9f;      // 2 pi / 2^32
-    s = __sinf(x) * factor;
-    c = __cosf(x) * factor;
+    s = __sinf(x);
+    c = __cosf(x);
 }
 
 // Sine and cosine of a whole turn's 256 parts.
@@ -65,14 +65,14 @@ __device__ const TurnTable kTurnTable = make_turn_table();
 
 // In 64 bits: the part of a turn from the table, the rest (at most 2^-9 of a turn, x = 0.0123) by the series
 // x - x^3/6 + x^5/120 and 1 - x^2/2 + x^4/24 - x^6/720, which end below 1e-17.
-__device__ __forceinline__ void turn_factors(int64_t position, uint64_t turn, double factor, double& s, double& c) {
+__device__ __forceinline__ void turn_factors(int64_t position, uint64_t turn, double& s, double& c) {
     const uint64_t a = static_cast<uint64_t>(angle_of(position, turn)) + (1ull << 55);      // to the nearest of 256
     const double2 t = kTurnTable.at[a >> 56];
     const double x = static_cast<double>(static_cast<int64_t>(a & ((1ull << 56) - 1)) - (1ll << 55)) * 3.4061215800210806e-19;     // 2 pi / 2^64
     const double x2 = x * x;
     const double sx = fma(x * x2, fma(x2, 1.0 / 120, -1.0 / 6), x), cx = fma(x2, fma(x2, fma(x2, -1.0 / 720, 1.0 / 24), -0.5), 1.0);
-    s = factor * fma(t.x, cx, t.y * sx);
-    c = factor * fma(t.y, cx, -(t.x * sx));
+    s = fma(t.x, cx, t.y * sx);
+    c = fma(t.y, cx, -(t.x * sx));
 }
 
 // Frequencies 2 i and 2 i + 1 of a rotation that is a kernel parameter, by its address: read as constants, which a warp takes
@@ -186,12 +186,16 @@ struct Turner {
     int active;                   // how many of the 8 pairs turn
     __device__ __forceinline__ void set(const bob_sm100_rotary& r, int place, int64_t position) {
         active = min(8, max(0, r.pairs - 8 * place));
+        if (active == 0) return;
         #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
+        for (int j = 0; j < 8; j += 2) {                     // (those that do not turn are not used)
             const ulonglong2 turn = turn_pair(r, 4 * place + j / 2);         // (64 of them are there)
-            s[j] = s[j + 1] = 0; c[j] = c[j + 1] = 1;
-            if (j < active) turn_factors(position, turn.x, static_cast<T>(r.factor), s[j], c[j]);
-            if (j + 1 < active) turn_factors(position, turn.y, static_cast<T>(r.factor), s[j + 1], c[j + 1]);
+            turn_factors(position, turn.x, s[j], c[j]);
+            turn_factors(position, turn.y, s[j + 1], c[j + 1]);
+        }
+        if (r.factor != 1.0) {
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) { s[j] *= static_cast<T>(r.factor); c[j] *= static_cast<T>(r.factor); }
         }
     }
     static constexpr int STEP = FORM == kInterleaved ? 2 : 1, PARTNER = FORM == kInterleaved ? 1 : 8;
