@@ -298,6 +298,8 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
     p.window = std::min(a->window, 1 << 28);
     p.scale = a->scale;
     p.ctas = d.ctas;
+    auto same = [](const int64_t (&x)[2][3]) { return std::equal(x[0], x[0] + 3, x[1]); };
+    p.alike = same(a->cache.strides) && (a->cache.bits == 16 || same(a->cache.scale_strides));
     p.part_ml = static_cast<float*>(workspace);
     p.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + d.acc_offset);
     int rc = 0;

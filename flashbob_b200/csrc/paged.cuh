@@ -32,6 +32,7 @@ struct alignas(16) PagedParams {
     int Hq, Hkv, G, N, form;
     int groups;                   // row groups of ROWS query rows per KV head
     int causal, window;
+    int alike;                    // keys and values (and their scales) have the same strides
     float scale;
     float* part_ml;               // [CTAs][2][ROWS] (reference, sum)
     float* part_acc;              // [CTAs][2][ROWS][D]
@@ -49,14 +50,14 @@ struct PagedConfig {
     static constexpr int LR = ROWS / 8;                          // rows of a thread
     // 16 bits: 4 KB of keys and 4 KB of values per block.  4 bits: 2 to 2.5 KB each, where the work per block counts.
     static constexpr int KB = BITS == 16 ? 2048 / D : (D == 128 ? 32 : 64);
-    static constexpr int SUB = 2048 / D;                         // keys of a block that are computed at a time
+    static constexpr int SUB = BITS == 16 ? KB : 32;             // keys of a block that are computed at a time
     static_assert(KB % SUB == 0 && SUB % 16 == 0, "whole products");
     static constexpr int ROW_BYTES = D * BITS / 8, CHUNKS = ROW_BYTES / 16;
     // 4 bits: a thread reads a word of four rows two apart; these strides put the rows into different banks
     static constexpr int V_STRIDE = BITS == 16 ? ROW_BYTES : (D == 128 ? 80 : (D == 64 ? 48 : 16));
     static constexpr int OFF_V = KB * ROW_BYTES, OFF_SK = OFF_V + KB * V_STRIDE, OFF_SV = OFF_SK + (BITS == 4 ? KB * 8 : 0);
     static constexpr int STAGE = OFF_SV + (BITS == 4 ? KB * 8 : 0);
-    static constexpr int CTAS = ROWS == 8 ? 3 : 2;              // per SM
+    static constexpr int CTAS = ROWS == 8 ? 3 : 2;
     static constexpr int NST = BITS == 16 ? (CTAS == 2 ? 3 : 2) : (CTAS == 2 ? 4 : 3);
     // columns that EX_ROWS rows of an accumulator bring into a ring slot at a time
     static constexpr int EX_ROWS = ROWS == 8 ? 8 : 16;
@@ -65,7 +66,9 @@ struct PagedConfig {
     static constexpr int Q_STRIDE = 2 * D + 16;                  // bytes of a query row; the 16 spread rows over the banks
     static constexpr int OFF_Q = kPagedWarps * NST * STAGE, OFF_ML = OFF_Q + 16 * MT * Q_STRIDE;
     static constexpr int OFF_SLOT = OFF_ML + 2 * kPagedWarps * EX_ROWS * 4;
-    static constexpr int SMEM = OFF_SLOT + 16;
+    static constexpr int OFF_QF = OFF_SLOT + 16;                 // 4 bits: queries as the products' operands, [product][step][lane]
+    static constexpr int SMEM = OFF_QF + (BITS == 4 ? MT * (D / 16) * 512 : 0);
+    static_assert(OFF_QF % 16 == 0, "16-byte loads");
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -273,60 +276,70 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     int fill = 0;                                        // ring slot that is free
     bool more = true;
     src.blk = src.last = 0;
-    int page_ids = -1;                                   // lane i: page of keys 16 i ... of the block
+    // Lane i: where the block's keys 16 i ... lie, from the start of the cache's tensors; -1 where the page is none.
+    long long row_k = -1, row_v = 0, scale_k = 0, scale_v = 0;
+    bool inside = false;                                 // every key of the block is in reach, and its page there
+    constexpr int RPC = 32 / CFG::CHUNKS;                // rows of a warp-wide copy
+    const int copy_row = lane / CFG::CHUNKS, chunk = lane % CFG::CHUNKS;
     auto seek = [&]() {                                  // to this warp's next block, and ask for its pages
         while (more && src.blk >= src.last) {
             more = src.template next<ROWS>(p);
             src.blk += warp;
         }
-        page_ids = -1;
-        if (more) {
-            const int key = src.blk * KB + 16 * lane;
-            if (lane < KB / 16 && key + 15 >= src.lo && key < src.hi) {
-                page_ids = page_of(p.seq, src.b, key);
-                if (page_ids < 0) report(p.seq.sticky, kStatusBadPage);
+        row_k = -1;
+        if (!more) return;
+        const int key = src.blk * KB + 16 * lane;
+        if (lane < KB / 16 && key + 15 >= src.lo && key < src.hi) {
+            const int page = page_of(p.seq, src.b, key);
+            if (page < 0) {
+                report(p.seq.sticky, kStatusBadPage);
+            } else {
+                const int row = key & ((1 << p.seq.page_shift) - 1);
+                auto at = [&](const CacheTensor& c) { return page * c.sp + src.kv_head * c.sh + row * c.sr; };
+                auto scale_at = [&](const CacheTensor& c) { return page * c.ssp + src.kv_head * c.ssh + row * c.ssr; };
+                row_k = row_v = at(p.cache[0]);
+                if constexpr (BITS == 4) scale_k = scale_v = scale_at(p.cache[0]);
+                if (!p.alike) {
+                    row_v = at(p.cache[1]);
+                    if constexpr (BITS == 4) scale_v = scale_at(p.cache[1]);
+                }
             }
         }
+        inside = src.blk * KB >= src.lo && (src.blk + 1) * KB <= src.hi && !__any_sync(0xffffffffu, lane < KB / 16 && row_k < 0);
     };
-    constexpr int RPC = 32 / CFG::CHUNKS;                // rows of a warp-wide copy
     auto swizzled = [](int r, int ch) { return BITS == 4 ? ch : ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3); };
     auto copy_block = [&]() {
         if (more) {
             const uint32_t dst = ring + fill * STAGE;
-            const int key0 = src.blk * KB, mask = (1 << p.seq.page_shift) - 1;
-            const bool inside = key0 >= src.lo && key0 + KB <= src.hi && !__any_sync(0xffffffffu, lane < KB / 16 && page_ids < 0);
+            const int key0 = src.blk * KB;
             #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const CacheTensor& c = p.cache[w];
-                const uint8_t* head = c.data + src.kv_head * c.sh;
-                const int ch = lane % CFG::CHUNKS;
-                auto to = [&](int r) { return dst + (w ? CFG::OFF_V + r * CFG::V_STRIDE : r * CFG::ROW_BYTES) + 16 * swizzled(r, ch); };
+                auto to = [&](int r) { return dst + (w ? CFG::OFF_V + r * CFG::V_STRIDE : r * CFG::ROW_BYTES) + 16 * swizzled(r, chunk); };
                 if (inside) {
                     // rows of 16 keys lie in one page, one after another
                     #pragma unroll
                     for (int sub = 0; sub < KB / 16; sub += RPC > 16 ? RPC / 16 : 1) {
-                        const int r0 = 16 * sub + lane / CFG::CHUNKS;
-                        const int page = __shfl_sync(0xffffffffu, page_ids, r0 / 16);
-                        const uint8_t* from = head + page * c.sp + ((key0 + r0) & mask) * c.sr + 16 * ch;
+                        const long long at = __shfl_sync(0xffffffffu, w ? row_v : row_k, sub + copy_row / 16);
+                        const uint8_t* from = c.data + at + (copy_row % 16) * c.sr + 16 * chunk;
                         #pragma unroll
-                        for (int k = 0; k < (RPC > 16 ? 1 : 16 / RPC); ++k) copy16(to(r0 + k * RPC), from + k * RPC * c.sr);
+                        for (int k = 0; k < (RPC > 16 ? 1 : 16 / RPC); ++k) copy16(to(16 * sub + copy_row + k * RPC), from + k * RPC * c.sr);
                     }
                 } else {
                     #pragma unroll 1
-                    for (int r = lane / CFG::CHUNKS; r < KB; r += RPC) {
-                        const int page = __shfl_sync(0xffffffffu, page_ids, r / 16), key = key0 + r;
-                        const bool there = key >= src.lo && key < src.hi && page >= 0;
-                        copy16(to(r), there ? head + page * c.sp + (key & mask) * c.sr + 16 * ch : c.data, there);
+                    for (int r = copy_row; r < KB; r += RPC) {
+                        const long long first = __shfl_sync(0xffffffffu, row_k, r / 16), at = __shfl_sync(0xffffffffu, w ? row_v : row_k, r / 16);
+                        const bool there = key0 + r >= src.lo && key0 + r < src.hi && first >= 0;
+                        copy16(to(r), there ? c.data + at + (r % 16) * c.sr + 16 * chunk : c.data, there);
                     }
                 }
                 if constexpr (BITS == 4) {
                     #pragma unroll
                     for (int k = 0; k < KB / 32; ++k) {
                         const int r = k * 32 + lane, key = key0 + r;
-                        const int page = __shfl_sync(0xffffffffu, page_ids, r / 16);
-                        const bool there = inside || (key >= src.lo && key < src.hi && page >= 0);
-                        const float* from = there ? c.scales + page * c.ssp + src.kv_head * c.ssh + (key & mask) * c.ssr : c.scales;
-                        copy8(dst + (w ? CFG::OFF_SV : CFG::OFF_SK) + 8 * r, from, there);
+                        const long long first = __shfl_sync(0xffffffffu, row_k, r / 16), at = __shfl_sync(0xffffffffu, w ? scale_v : scale_k, r / 16);
+                        const bool there = inside || (key >= src.lo && key < src.hi && first >= 0);
+                        copy8(dst + (w ? CFG::OFF_SV : CFG::OFF_SK) + 8 * r, there ? c.scales + at + (r % 16) * c.ssr : c.scales, there);
                     }
                 }
             }
@@ -368,47 +381,51 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             }
         }
         __syncthreads();
-        uint32_t qa[MT][KS][4];
         float q_sum[LR];                                 // 4 bits: sum of a row's elements
         (void)q_sum;
         // row of mine (LR of them) that half hr of product mt has, or a part of
         auto my_row = [](int mt, int hr) { return ROWS == 8 ? 0 : ROWS == 16 ? hr : 2 * mt + hr; };
+        const uint32_t q_rows = smem_u32(paged_smem) + CFG::OFF_Q, q_frags = smem_u32(paged_smem) + CFG::OFF_QF + 16 * lane;
         if constexpr (BITS == 4) {
+            // the elements in the order in which a word of codes yields them: thread t holds words NWD t ... of a
+            // key row, and a word's pairs are (e, e + 4).  Kept in shared memory: in registers they leave room for 12
+            // warps per SM instead of 16.
             #pragma unroll
             for (int k = 0; k < LR; ++k) q_sum[k] = 0.f;
-        }
-        #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const uint32_t base = smem_u32(paged_smem) + CFG::OFF_Q + mt * 16 * CFG::Q_STRIDE;
-            if constexpr (BITS == 16) {
-                #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) ldsm4(base + (lane % 16) * CFG::Q_STRIDE + ks * 32 + (lane / 16) * 16, qa[mt][ks]);
-            } else {
-                // the elements in the order in which a word of codes yields them: thread t holds words NWD t ... of a
-                // key row, and a word's pairs are (e, e + 4)
-                constexpr int NWD = D / 32;
+            constexpr int NWD = D / 32;
+            #pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                uint32_t frag[KS][4];
                 #pragma unroll
                 for (int hr = 0; hr < 2; ++hr) {
                     float sum = 0.f;
                     #pragma unroll
                     for (int j = 0; j < NWD; ++j) {
                         uint32_t w[4];
-                        lds_words<4>(base + (g + 8 * hr) * CFG::Q_STRIDE + 16 * (NWD * t + j), w);
+                        lds_words<4>(q_rows + (mt * 16 + g + 8 * hr) * CFG::Q_STRIDE + 16 * (NWD * t + j), w);
                         float f[8];
                         widen8<BF16>(make_uint4(w[0], w[1], w[2], w[3]), f);
                         #pragma unroll
                         for (int e = 0; e < 8; ++e) sum += f[e];
                         #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            qa[mt][2 * j + half][hr] = __byte_perm(w[half], w[2 + half], 0x5410);
-                            qa[mt][2 * j + half][2 + hr] = __byte_perm(w[half], w[2 + half], 0x7632);
+                            frag[2 * j + half][hr] = __byte_perm(w[half], w[2 + half], 0x5410);
+                            frag[2 * j + half][2 + hr] = __byte_perm(w[half], w[2 + half], 0x7632);
                         }
                     }
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                     q_sum[my_row(mt, hr)] += sum + __shfl_xor_sync(0xffffffffu, sum, 2);
                 }
+                #pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    if (ks % kPagedWarps == warp) st_shared_v4(q_frags + (mt * KS + ks) * 512, frag[ks][0], frag[ks][1], frag[ks][2], frag[ks][3]);
             }
+            __syncthreads();
         }
+        auto query = [&](int mt, int ks, uint32_t (&a)[4]) {
+            if constexpr (BITS == 16) ldsm4(q_rows + (mt * 16 + lane % 16) * CFG::Q_STRIDE + ks * 32 + (lane / 16) * 16, a);
+            else lds_words<4>(q_frags + (mt * KS + ks) * 512, a);
+        };
         int lo[LR], hi[LR];                              // keys that my rows attend to
         #pragma unroll
         for (int k = 0; k < LR; ++k) {
@@ -452,6 +469,9 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             if constexpr (BITS == 16) {
                 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
+                    uint32_t qa[MT][4];
+                    #pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) query(mt, ks, qa[mt]);
                     #pragma unroll
                     for (int pr = 0; pr < NT / 2; ++pr) {
                         const int r = pr * 16 + (lane / 16) * 8 + lane % 8, ch = 2 * ks + (lane / 8) % 2;
@@ -459,8 +479,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         ldsm4(base + r * CFG::ROW_BYTES + 16 * swizzled(r, ch), kf);
                         #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            mma16816<BF16>(sc[mt][2 * pr], qa[mt][ks], kf[0], kf[1]);
-                            mma16816<BF16>(sc[mt][2 * pr + 1], qa[mt][ks], kf[2], kf[3]);
+                            mma16816<BF16>(sc[mt][2 * pr], qa[mt], kf[0], kf[1]);
+                            mma16816<BF16>(sc[mt][2 * pr + 1], qa[mt], kf[2], kf[3]);
                         }
                     }
                 }
@@ -468,17 +488,21 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                 // codes as 16-bit numbers b = 1 + c / 16, exactly: a shift and one operation on a pair.  A score is
                 // scale q . c + zero sum q = 16 scale q . b + (zero - 16 scale) sum q.
                 constexpr int NWD = D / 32;
+                uint32_t w[NT][NWD];
                 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    uint32_t w[NWD];
-                    lds_words<NWD>(base + (8 * nt + g) * CFG::ROW_BYTES + 4 * NWD * t, w);
+                for (int nt = 0; nt < NT; ++nt) lds_words<NWD>(base + (8 * nt + g) * CFG::ROW_BYTES + 4 * NWD * t, w[nt]);
+                #pragma unroll
+                for (int j = 0; j < NWD; ++j) {
                     #pragma unroll
-                    for (int j = 0; j < NWD; ++j) {
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t qa[MT][4];
                         #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint32_t b0 = key_codes(w[j], 2 * half), b1 = key_codes(w[j], 2 * half + 1);
+                        for (int mt = 0; mt < MT; ++mt) query(mt, 2 * j + half, qa[mt]);
+                        #pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint32_t b0 = key_codes(w[nt][j], 2 * half), b1 = key_codes(w[nt][j], 2 * half + 1);
                             #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) mma16816<BF16>(sc[mt][nt], qa[mt][2 * j + half], b0, b1);
+                            for (int mt = 0; mt < MT; ++mt) mma16816<BF16>(sc[mt][nt], qa[mt], b0, b1);
                         }
                     }
                 }
