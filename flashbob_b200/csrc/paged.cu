@@ -256,13 +256,19 @@ static int launch_paged(PagedParams& p, int device, cudaStream_t stream) {
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
+    const int64_t items = (int64_t)p.seq.B * p.Hkv * p.groups;
     const int rows = std::min(ROWS, p.N * p.G);
-    cfg.gridDim = dim3((unsigned)(p.seq.B * p.Hkv * p.groups), (unsigned)((rows + kPagedWarps - 1) / kPagedWarps));
     cfg.blockDim = dim3(kPagedThreads);
     cfg.stream = stream;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, combine_kernel<D, ROWS, BF16, BITS>, p) == cudaSuccess ? 0 : kBadLaunch;
+    // a CTA to a row while all of them run at once (512 rows in 37 parts each 31 us with a warp, 29 with four)
+    if (items * rows <= kPagedSms * 8) {
+        cfg.gridDim = dim3((unsigned)items, (unsigned)rows);
+        return cudaLaunchKernelEx(&cfg, combine_kernel<D, ROWS, BF16, BITS, 4>, p) == cudaSuccess ? 0 : kBadLaunch;
+    }
+    cfg.gridDim = dim3((unsigned)items, (unsigned)((rows + kPagedWarps - 1) / kPagedWarps));
+    return cudaLaunchKernelEx(&cfg, combine_kernel<D, ROWS, BF16, BITS, 1>, p) == cudaSuccess ? 0 : kBadLaunch;
 }
 
 static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_t stream) {

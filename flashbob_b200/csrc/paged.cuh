@@ -149,19 +149,49 @@ __device__ __forceinline__ BlockRange blocks_of(const PagedParams& p, int b) {
     return {first, (s.length + KB - 1) / KB - first};
 }
 
-// The line of all blocks: its length, and where it is cut.
-template <int KB>
-__device__ __forceinline__ long long line_length(const PagedParams& p, int lane) {
-    long long total = 0;
-    for (int b = lane; b < p.seq.B; b += 32) total += blocks_of<KB>(p, b).n;
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    return total * p.Hkv * p.groups;
+__device__ __forceinline__ long long quotient(long long a, long long b) {       // both not negative; 32 bits where they do
+    return (a | b) >> 32 ? a / b : static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
 }
-__device__ __forceinline__ int line_parts(const PagedParams& p, long long total) {
-    return static_cast<int>(min((long long)p.ctas, max(1LL, total / kPagedMinBlocks)));
-}
-__device__ __forceinline__ long long cut(long long total, int parts, int i) { return total * i / parts; }
+
+// The line of all blocks, and where it is cut: into stretches of equal length, one for each CTA.  With fewer items than CTAs
+// and little work every item is cut into the same number of stretches, so that none has parts of two items (their queries,
+// sums and parts to add cost as much as a few blocks: 128 items of 33 blocks 17.6 us without, 14.8 with).
+struct Line {
+    long long total, base;        // blocks; blocks of a stretch, the first `rest` have one more
+    int parts, rest, lane_n;
+    // lane_n: the blocks of sequence `lane` (of the first 32)
+    template <int KB>
+    __device__ __forceinline__ void measure(const PagedParams& p, int lane) {
+        lane_n = lane < p.seq.B ? blocks_of<KB>(p, lane).n : 0;
+        long long sum = lane_n;
+        int items = lane_n > 0;
+        for (int b = lane + 32; b < p.seq.B; b += 32) {
+            const int n = blocks_of<KB>(p, b).n;
+            sum += n;
+            items += n > 0;
+        }
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            items += __shfl_xor_sync(0xffffffffu, items, o);
+        }
+        const long long per = p.Hkv * p.groups;
+        total = sum * per;
+        parts = static_cast<int>(min((long long)p.ctas, max(1LL, total / kPagedMinBlocks)));
+        if (total > 0 && items * per <= parts && total < 32LL * parts) {
+            const int whole = static_cast<int>(items * per), equal = parts / whole * whole;
+            if (5 * equal >= 4 * parts) parts = equal;
+        }
+        base = quotient(total, parts);
+        rest = static_cast<int>(total - base * parts);
+    }
+    __device__ __forceinline__ long long cut(int i) const { return base * i + min(i, rest); }
+    // the stretch that block `at` lies in
+    __device__ __forceinline__ int stretch(long long at) const {
+        const long long longer = (base + 1) * rest;
+        return static_cast<int>(at < longer ? quotient(at, base + 1) : rest + quotient(at - longer, max(1LL, base)));
+    }
+};
 
 // Walks the items of a CTA's stretch of the line.
 template <int KB>
@@ -172,20 +202,21 @@ struct Cursor {
     int kv_head, group, blk, last, lo, hi;
     bool whole, begins;           // the segment is the whole item; ... has its first block
 
-    // Finds the sequence that `begin` lies in.
-    __device__ __forceinline__ void start(const PagedParams& p, long long begin, long long end_, int lane) {
-        pos = begin; end = end_; base = 0; b = 0; first = 0; n = 0;
-        if (begin >= end_) return;
+
+    // Finds the sequence that a stretch begins in.
+    __device__ __forceinline__ void start(const PagedParams& p, const Line& line, int part, int lane) {
+        pos = line.cut(part); end = line.cut(part + 1); base = 0; b = 0; first = 0; n = 0;
+        if (pos >= end) return;
         const int per = p.Hkv * p.groups;
         for (int b0 = 0;; b0 += 32) {
-            const int mine = b0 + lane < p.seq.B ? blocks_of<KB>(p, b0 + lane).n : 0;
+            const int mine = b0 == 0 ? line.lane_n : (b0 + lane < p.seq.B ? blocks_of<KB>(p, b0 + lane).n : 0);
             int upto = mine;
             #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int t = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += t;
             }
-            const uint32_t past = __ballot_sync(0xffffffffu, base + (long long)upto * per > begin);
+            const uint32_t past = __ballot_sync(0xffffffffu, base + (long long)upto * per > pos);
             if (past || b0 + 32 >= p.seq.B) {
                 const int l = past ? __ffs(past) - 1 : 31;
                 b = b0 + l;
@@ -264,14 +295,15 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
         for (int b = lane; b < p.seq.B; b += 32)
             if (!sequence_of(p.seq, b, p.N).ok) report(p.seq.sticky, kStatusBadLength);
     }
-    const long long total = line_length<KB>(p, lane);
-    const int parts = line_parts(p, total);
-    if (static_cast<int>(blockIdx.x) >= parts) return;
-    const long long begin = cut(total, parts, blockIdx.x), end = cut(total, parts, blockIdx.x + 1);
+    Cursor<KB> src, seg;
+    {
+        Line line;
+        line.measure<KB>(p, lane);
+        if (static_cast<int>(blockIdx.x) >= line.parts) return;
+        src.start(p, line, blockIdx.x, lane);
+    }
 
     // ---- copies: block `blk` of the copying cursor, a warp's every fourth of a segment ----------------------
-    Cursor<KB> src, seg;
-    src.start(p, begin, end, lane);
     seg = src;
     int fill = 0;                                        // ring slot that is free
     bool more = true;
@@ -741,77 +773,93 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     }
 }
 
-// Adds the parts of the items that paged_kernel divided, and writes the zeros of those without keys.  One warp per query row.
-template <int D, int ROWS, bool BF16, int BITS>
+// Adds the parts of the items that paged_kernel divided, and writes the zeros of those without keys.  WARPS warps to a query
+// row (4, or 1 where there are many rows): D / 4 lanes have a part's columns, and up to 4 * WARPS * 128 / D parts are on
+// their way at once.
+template <int D, int ROWS, bool BF16, int BITS, int WARPS>
 __global__ void __launch_bounds__(kPagedThreads) combine_kernel(const __grid_constant__ PagedParams p) {
     using CFG = PagedConfig<D, ROWS, BITS>;
-    constexpr int KB = CFG::KB, LPR = D / 4, PER = 32 / LPR;   // lanes of a row; parts taken at a time
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int per = p.Hkv * p.groups, b = blockIdx.x / per, item = blockIdx.x % per;
-    const int r = blockIdx.y * kPagedWarps + warp, row = (item % p.groups) * ROWS + r;
-    const bool row_ok = row < p.N * p.G;
+    constexpr int KB = CFG::KB, LPR = D / 4, PER = 32 / LPR, BATCH = 4, STEP = WARPS * PER;
+    __shared__ float2 sm_ml[kPagedWarps * PER];
+    __shared__ float4 sm_acc[kPagedWarps * PER][LPR];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = (lane % LPR) * 4;
+    const int group = warp / WARPS * STEP, mine = (warp % WARPS) * PER + lane / LPR;     // the row's place in shared memory; which of its parts
+    const int per = p.Hkv * p.groups, b = blockIdx.x / per, item = blockIdx.x - b * per;
+    const int r = blockIdx.y * (kPagedWarps / WARPS) + warp / WARPS, row = (item % p.groups) * ROWS + r;
+    const bool row_ok = r < ROWS && row < p.N * p.G;
     // (lengths are inputs: they were there before paged_kernel started)
-    long long before = 0, total = 0;
-    for (int i = lane; i < p.seq.B; i += 32) {
-        const int n = blocks_of<KB>(p, i).n;
-        total += n;
-        if (i < b) before += n;
-    }
+    Line line;
+    line.measure<KB>(p, lane);
+    long long before = 0;
+    for (int i = lane; i < b; i += 32) before += i < 32 ? line.lane_n : blocks_of<KB>(p, i).n;
     #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    total *= per;
-    const int n = blocks_of<KB>(p, b).n, parts = line_parts(p, total);
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    const int n = blocks_of<KB>(p, b).n;
     const long long first = before * per + (long long)item * n;
-    const int col = (lane % LPR) * 4;
-    uint16_t* out = p.out + (((long long)b * p.Hq + (item / p.groups) * p.G + row % p.G) * p.N + row / p.G) * D + col;
     int c0 = 0, c1 = 0;                                  // the CTAs that have its blocks
     if (n > 0) {
-        auto holder = [&](long long at) {
-            int c = static_cast<int>(min((long long)parts - 1, at * parts / total));
-            while (cut(total, parts, c) > at) --c;
-            while (cut(total, parts, c + 1) <= at) ++c;
-            return c;
-        };
-        c0 = holder(first);
-        c1 = holder(first + n - 1);
+        c0 = line.stretch(first);
+        c1 = line.stretch(first + n - 1);
     }
     // (every CTA waits: this grid must not end, and let the stream go on, before paged_kernel has)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (!row_ok || (n > 0 && c0 == c1)) return;          // no row, or finished in paged_kernel
+    if (n > 0 && c0 == c1) return;                       // finished in paged_kernel
+    uint16_t* out = p.out + (((long long)b * p.Hq + (item / p.groups) * p.G + row % p.G) * p.N + row / p.G) * D + col;
     if (n == 0) {
-        if (lane < LPR) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
+        if (row_ok && mine == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
         return;
     }
-    // slot 1 of the CTA where the item begins, slot 0 of those where it goes on
-    auto slot = [&](int c) { return (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r; };
     float ref = -1e30f, sum = 0.f;
-    for (int c = c0 + lane; c <= c1; c += 32) ref = fmaxf(ref, __ldcg(p.part_ml + 2 * slot(c)));
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ref = fmaxf(ref, __shfl_xor_sync(0xffffffffu, ref, o));
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    #pragma unroll 8
-    for (int c = c0 + lane / LPR; c <= c1; c += PER) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot(c)));
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_acc + slot(c) * D + col));
-        const float f = exp2_ftz(ml.x - ref);
-        sum = fmaf(f, ml.y, sum);
+    for (int c = c0 + mine; row_ok && c <= c1; c += BATCH * STEP) {
+        float2 ml[BATCH];
+        float4 x[BATCH];
+        #pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const int part = c + k * STEP;
+            ml[k] = make_float2(-1e30f, 0.f);
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (part <= c1) {
+                // slot 1 of the CTA where the item begins, slot 0 of those where it goes on
+                const long long slot = (2LL * part + (part == c0 ? 1 : 0)) * ROWS + r;
+                ml[k] = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot));
+                x[k] = __ldcg(reinterpret_cast<const float4*>(p.part_acc + slot * D + col));
+            }
+        }
+        float top = ref;
+        #pragma unroll
+        for (int k = 0; k < BATCH; ++k) top = fmaxf(top, ml[k].x);
+        const float back = exp2_ftz(ref - top);
+        ref = top;
+        sum *= back;
+        v.x *= back; v.y *= back; v.z *= back; v.w *= back;
+        #pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            const float f = exp2_ftz(ml[k].x - top);
+            sum = fmaf(f, ml[k].y, sum);
+            v.x = fmaf(f, x[k].x, v.x); v.y = fmaf(f, x[k].y, v.y); v.z = fmaf(f, x[k].z, v.z); v.w = fmaf(f, x[k].w, v.w);
+        }
+    }
+    if (lane % LPR == 0) sm_ml[group + mine] = make_float2(ref, sum);
+    sm_acc[group + mine][lane % LPR] = v;
+    __syncthreads();
+    if (mine > 0 || !row_ok) return;
+    float top = ref;
+    #pragma unroll
+    for (int k = 1; k < STEP; ++k) top = fmaxf(top, sm_ml[group + k].x);
+    sum = 0.f;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    #pragma unroll
+    for (int k = 0; k < STEP; ++k) {
+        const float f = exp2_ftz(sm_ml[group + k].x - top);
+        const float4 x = sm_acc[group + k][lane % LPR];
+        sum = fmaf(f, sm_ml[group + k].y, sum);
         v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
     }
-    #pragma unroll
-    for (int o = LPR; o < 32; o <<= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-        v.z += __shfl_xor_sync(0xffffffffu, v.z, o); v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
-    }
-    if (lane < LPR) {
-        const float inv = 1.f / sum;
-        uint2 o = make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
-        if (sum == 0.f) o = make_uint2(0, 0);
-        *reinterpret_cast<uint2*>(out) = o;
-    }
+    const float inv = 1.f / sum;
+    uint2 o = make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
+    if (sum == 0.f) o = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(out) = o;
 }
 
 }  // namespace bob
