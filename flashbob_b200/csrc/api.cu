@@ -151,7 +151,7 @@ static int launch_sweep(const bob_sm100_geom* g, SweepParams& prm, const TensorA
                        : sweep_kernel<MODE, DPAD, TN, BF16, NG, CW, ALIAS, false>;
     static std::atomic<uint64_t> done[2];
     if (int rc = prepare_kernel<CFG>(kernel, g->device, done[allt])) return rc;
-    const long long items = (long long)((n_own + 127) / 128) * heads * g->B;
+    const long long items = (long long)((n_own + 127) / 128) * heads * g->B * (MODE == kFwdPaged ? prm.splits : 1);
     if (items > 0x7fffffffLL) return kErrGeom;
     const int sms = sm_count(g->device);
     if (sms <= 0) return kErrDevice;
@@ -460,12 +460,13 @@ extern "C" int bob_sm100_fwd(const bob_sm100_geom* g, const void* q, const void*
 }
 
 // Forward over a paged cache for many query rows; `q` and its strides may be those of turned queries in the workspace.
-int bob::sweep_paged(const bob_sm100_paged_args* a, const SequenceParams& seq, const void* q, const int64_t* q_strides, void* workspace, cudaStream_t s) {
+int bob::sweep_paged(const bob_sm100_paged_args* a, const SequenceParams& seq, const void* q, const int64_t* q_strides, int pack, int splits, float* part_acc,
+                     float* part_ml, void* workspace, cudaStream_t s) {
     int rc = begin_call(workspace, s);
     if (rc) return rc;
     const bob_sm100_cache& c = a->cache;
     bob_sm100_geom g = {};
-    g.B = seq.B; g.Hq = a->Hq; g.Hkv = c.heads; g.Nq = a->N; g.Nk = 1; g.D = c.D;       // (every sequence has its own length)
+    g.B = seq.B; g.Hq = a->Hq / pack; g.Hkv = c.heads; g.Nq = a->N * pack; g.Nk = 1; g.D = c.D;       // (every sequence has its own length)
     g.dtype = c.dtype;
     g.is_causal = a->is_causal;
     g.device = c.device;
@@ -476,6 +477,7 @@ int bob::sweep_paged(const bob_sm100_paged_args* a, const SequenceParams& seq, c
     p.sticky = seq.sticky;
     p.seq = seq;
     p.box_rows = std::min(c.page_size, 128);
+    p.pack = pack; p.splits = splits; p.part_acc = part_acc; p.part_ml = part_ml;
     p.res0 = a->out;
     int64_t strides[2][3];
     for (int w = 0; w < 2; ++w)

@@ -35,6 +35,7 @@ struct ReadParams {
     CacheTensor cache[2];
     uint16_t* out[2];                                            // contiguous [B, H, N, D]
     int H, N, D;
+    int unpack, window;           // out is [B * max_pages, H, page_size, D], only rows that a paged call looks at are written
 };
 
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
@@ -169,8 +170,12 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_consta
     const long long id = (long long)blockIdx.x * kCacheThreads + threadIdx.x, token = id / per_row;
     if (token >= (long long)p.seq.B * p.N) return;
     const int c = static_cast<int>(id % per_row), b = static_cast<int>(token / p.N), n = static_cast<int>(token % p.N);
-    const Sequence s = sequence_of(p.seq, b, 0);
+    const Sequence s = sequence_of(p.seq, b, p.unpack);
     if (n == 0 && c == 0 && h == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
+    if (p.unpack) {
+        const int first = p.window > 0 ? s.length - (p.seq.counts ? __ldg(p.seq.counts + b) : p.unpack) - p.window + 1 : 0;
+        if (n >= s.length || n < first) return;
+    }
     int page = -1;
     if (n < s.length) {
         page = page_of(p.seq, b, n);
@@ -203,7 +208,9 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_consta
             x[w].a = narrow8<BF16>(v);
             x[w].b = narrow8<BF16>(v + 8);
         }
-        uint4* dst = reinterpret_cast<uint4*>(p.out[w] + (((long long)b * p.H + h) * p.N + n) * p.D) + 2 * c;
+        const long long at = p.unpack ? (((long long)b * p.seq.max_pages + (n >> p.seq.page_shift)) * p.H + h << p.seq.page_shift) + row
+                                      : ((long long)b * p.H + h) * p.N + n;
+        uint4* dst = reinterpret_cast<uint4*>(p.out[w] + at * p.D) + 2 * c;
         dst[0] = x[w].a;
         dst[1] = x[w].b;
     }

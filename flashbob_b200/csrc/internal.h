@@ -19,8 +19,10 @@ int bwd2_impl(const bob_sm100_geom* g, const void* q, const void* k, const void*
               void* dObar, void* workspace, void* stream, int* sticky, int part);
 
 // Forward over a 16-bit paged cache through the kernel for many rows (arguments checked, the device is current): clears the
-// workspace's status block, which is all of the workspace that it uses.
-int sweep_paged(const bob_sm100_paged_args* a, const SequenceParams& seq, const void* q, const int64_t* q_strides, void* workspace, cudaStream_t stream);
+// workspace's status block, which is all of the workspace that it uses.  pack: query heads that
+// share a head's rows (SweepParams::pack); pack or splits > 1: to part_acc and part_ml, not `out`.
+int sweep_paged(const bob_sm100_paged_args* a, const SequenceParams& seq, const void* q, const int64_t* q_strides, int pack, int splits, float* part_acc,
+                float* part_ml, void* workspace, cudaStream_t stream);
 
 // The per-device host-visible status word: its device address (create = true: page-locks it on first
 // use; null if that failed) or its host address (create = false; null before first use).

@@ -102,9 +102,9 @@ template <class F> static void with_type(int dtype, F f) {
 // elements 7.1 / 5.4, 163,840 rows 21.1 / 15.4; eight 18.4). 
 constexpr int64_t kSharedTurns = (int64_t)kPagedSms * 512;
 
-static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream, const int* lengths = nullptr, const int* counts = nullptr) {
+static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream, const int* lengths = nullptr, const int* counts = nullptr, int pack = 1) {
     RotateParams p = {};
-    p.lengths = lengths; p.counts = counts;
+    p.lengths = lengths; p.counts = counts; p.pack = pack;
     p.rotary = a->rotary;
     if (a->inverse)
         for (uint64_t& x : p.rotary.turns) x = 0 - x;
@@ -169,10 +169,13 @@ static int run_append(const bob_sm100_cache* c, const bob_sm100_sequences* s, co
     return launched();
 }
 
-static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int n, void* const* out, cudaStream_t stream) {
+// unpack > 0: for a paged call of that many rows per sequence (ReadParams::unpack).
+static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int n, void* const* out, cudaStream_t stream, int unpack = 0, int window = 0) {
     ReadParams p = {};
     p.seq = sequences(c, s);
-    p.seq.counts = nullptr;
+    if (!unpack) p.seq.counts = nullptr;
+    p.unpack = unpack;
+    p.window = window;
     for (int w = 0; w < 2; ++w) { p.cache[w] = cache_tensor(c, w); p.out[w] = static_cast<uint16_t*>(out[w]); }
     p.H = c->heads; p.N = n; p.D = c->D;
     const int64_t threads = (int64_t)s->B * n * (c->D / 16), blocks = (threads + kCacheThreads - 1) / kCacheThreads;
@@ -189,26 +192,46 @@ static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int 
 // ---- attention --------------------------------------------------------------------------------------------------
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// sweep: through the kernel for many rows, after a kernel that turns the queries into the workspace.
-struct PagedPlan { bool sweep; int rows, groups, ctas; size_t q_offset, acc_offset, bytes; };
+// sweep: through the kernel for many rows, after a kernel that turns the queries into the workspace (and, in 4 bits, one that
+// unpacks the cache there), and with splits > 1 before one that adds the parts.
+struct PagedPlan { bool sweep; int pack, splits, rows, groups, ctas; size_t q_offset, ml_offset, acc_offset, kv_offset, kv_bytes, bytes; };
 
-constexpr int kPagedRows = 32;         // most rows of a KV head's queries that a 16-bit cache's paged_kernel takes
+// Most rows of a KV head's queries that paged_kernel takes.
+constexpr int kPagedRows = 32, kPagedRows4 = 64;
+// ... in 4 bits, while the unpacked cache (as much as the page table has room for) takes no more than this.
+constexpr int64_t kMostUnpacked = (int64_t)1 << 30;
+constexpr int kMostSplits = 16;
 
 static int block_keys(int D, int bits) { return bits == 16 ? 2048 / D : (D == 128 ? 32 : 64); }
 
-// The kernel for many rows takes its queries as tiles: those to be turned, and expanded ones, are written out first.
+// The kernel for many rows takes its queries as tiles of 128 rows of a head: those to be turned, and expanded ones, are written
+// out first, and so are those of heads that share keys where that makes at most half as many tiles.
+static int packed_heads(const bob_sm100_paged_args* a) {
+    const int64_t G = a->Hq / a->cache.heads, apart = (a->N + 127) / 128 * G, together = (a->N * G + 127) / 128;
+    return 2 * together <= apart ? (int)G : 1;
+}
 static bool copies_queries(const bob_sm100_paged_args* a) {
     const int64_t* s = a->q_strides;
-    return a->rotary.pairs || (s[0] == 0 && a->seq.B > 1) || (s[1] == 0 && a->Hq > 1) || (s[2] == 0 && a->N > 1);
+    return a->rotary.pairs || packed_heads(a) > 1 || (s[0] == 0 && a->seq.B > 1) || (s[1] == 0 && a->Hq > 1) || (s[2] == 0 && a->N > 1);
 }
 
 static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
     PagedPlan d = {};
     const int64_t R = (int64_t)a->N * (a->Hq / a->cache.heads);
-    d.sweep = a->cache.bits == 16 && R > kPagedRows;
+    const int64_t rows = (int64_t)a->seq.B * a->Hq * a->N, unpacked = (int64_t)a->seq.B * a->seq.max_pages * a->cache.page_size * a->cache.heads * a->cache.D * 2;
+    d.sweep = a->cache.bits == 16 ? R > kPagedRows : R > kPagedRows4 && 2 * unpacked <= kMostUnpacked;
     if (d.sweep) {
+        // with a tile for fewer than half of the SMs, the keys are divided too (whatever the lengths are)
+        d.pack = packed_heads(a);
+        const int64_t items = ((int64_t)a->N * d.pack + 127) / 128 * (a->Hq / d.pack) * a->seq.B;
+        d.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMostSplits, kPagedSms / items));
+        const bool parted = d.splits > 1 || d.pack > 1;
         d.q_offset = 256;
-        d.bytes = d.q_offset + (copies_queries(a) ? (size_t)a->seq.B * a->Hq * a->N * a->cache.D * 2 : 0);
+        d.ml_offset = d.q_offset + (copies_queries(a) ? up256(rows * a->cache.D * 2) : 0);
+        d.acc_offset = d.ml_offset + (parted ? up256(d.splits * rows * 2 * sizeof(float)) : 0);
+        d.kv_offset = d.acc_offset + (parted ? up256(d.splits * rows * a->cache.D * sizeof(float)) : 0);
+        d.kv_bytes = a->cache.bits == 4 ? up256(unpacked) : 0;
+        d.bytes = d.kv_offset + 2 * d.kv_bytes;
         return d;
     }
     d.rows = R <= 8 ? 8 : (R <= 16 ? 16 : 32);
@@ -217,9 +240,9 @@ static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
     const int64_t kb = block_keys(a->cache.D, a->cache.bits), most = ((int64_t)a->seq.max_pages * a->cache.page_size + kb - 1) / kb;
     const int64_t line = most * a->seq.B * a->cache.heads * d.groups;
     d.ctas = (int)std::min<int64_t>((d.rows == 8 ? 3 : 2) * kPagedSms, std::max<int64_t>(1, line / kPagedMinBlocks));
-    const size_t rows = (size_t)d.ctas * 2 * d.rows;
-    d.acc_offset = up256(rows * 2 * sizeof(float));
-    d.bytes = d.acc_offset + rows * a->cache.D * sizeof(float);
+    const size_t slots = (size_t)d.ctas * 2 * d.rows;
+    d.acc_offset = up256(slots * 2 * sizeof(float));
+    d.bytes = d.acc_offset + slots * a->cache.D * sizeof(float);
     return d;
 }
 
@@ -274,7 +297,9 @@ static int launch_paged(PagedParams& p, int device, cudaStream_t stream) {
 static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_t stream) {
     const PagedPlan d = paged_plan(a);
     if (d.sweep) {
-        const SequenceParams seq = sequences(&a->cache, &a->seq);
+        char* ws = static_cast<char*>(workspace);
+        bob_sm100_paged_args b = *a;
+        SequenceParams seq = sequences(&a->cache, &a->seq);
         const void* q = a->q;
         int64_t strides[3] = {a->q_strides[0], a->q_strides[1], a->q_strides[2]};
         if (copies_queries(a)) {
@@ -283,13 +308,32 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
             r.heads[0] = a->Hq;
             r.in[0] = q;
             for (int i = 0; i < 3; ++i) r.in_strides[0][i] = strides[i];
-            r.out[0] = static_cast<char*>(workspace) + d.q_offset;
+            r.out[0] = ws + d.q_offset;
             r.rotary = a->rotary;
-            if (int rc = run_rotate(&r, stream, a->seq.lengths, a->seq.counts)) return rc;
+            if (int rc = run_rotate(&r, stream, a->seq.lengths, a->seq.counts, d.pack)) return rc;
             q = r.out[0];
-            strides[2] = a->cache.D; strides[1] = strides[2] * a->N; strides[0] = strides[1] * a->Hq;
+            strides[2] = a->cache.D; strides[1] = strides[2] * a->N * d.pack; strides[0] = strides[1] * (a->Hq / d.pack);
         }
-        return sweep_paged(a, seq, q, strides, workspace, stream);
+        if (a->cache.bits == 4) {
+            bob_sm100_cache& c = b.cache;
+            for (int w = 0; w < 2; ++w) {
+                c.data[w] = ws + d.kv_offset + w * d.kv_bytes;
+                c.strides[w][2] = 2 * c.D; c.strides[w][1] = c.strides[w][2] * c.page_size; c.strides[w][0] = c.strides[w][1] * c.heads;
+            }
+            if (int rc = run_read(&a->cache, &a->seq, a->seq.max_pages * c.page_size, c.data, stream, a->N, std::min(a->window, 1 << 28))) return rc;
+            c.bits = 16;
+            c.pages = seq.pages = seq.B * seq.max_pages;
+            seq.table = nullptr;
+        }
+        float* ml = reinterpret_cast<float*>(ws + d.ml_offset);
+        float* acc = reinterpret_cast<float*>(ws + d.acc_offset);
+        if (int rc = sweep_paged(&b, seq, q, strides, d.pack, d.splits, acc, ml, workspace, stream)) return rc;
+        if (d.splits == 1 && d.pack == 1) return 0;
+        const int64_t rows = (int64_t)a->seq.B * a->Hq * a->N, blocks = (rows * (a->cache.D / 4) + 255) / 256;
+        with_type(a->cache.dtype, [&](auto bf16) {
+            add_splits_kernel<decltype(bf16)::value><<<(unsigned)blocks, 256, 0, stream>>>(ml, acc, static_cast<uint16_t*>(a->out), d.splits, rows, a->cache.D, a->N, d.pack);
+        });
+        return launched();
     }
     PagedParams p = {};
     p.rotary = a->rotary;

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     }
     Cursor<KB> src, seg;
     {
-        Line line;
+        Line line = {};
         line.measure<KB>(p, lane);
         if (static_cast<int>(blockIdx.x) >= line.parts) return;
         src.start(p, line, blockIdx.x, lane);
@@ -773,6 +773,33 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     }
 }
 
+// Adds the parts of a forward whose tiles were divided (SweepParams::splits, pack): one thread per four columns of a row.
+template <bool BF16>
+__global__ void __launch_bounds__(256) add_splits_kernel(const float* part_ml, const float* part_acc, uint16_t* out, int splits, long long rows, int D, int N, int pack) {
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / (D / 4);
+    const int col = static_cast<int>(id % (D / 4)) * 4;
+    if (row >= rows) return;
+    float ref = -1e30f;
+    for (int s = 0; s < splits; ++s) ref = fmaxf(ref, __ldcg(part_ml + 2 * (s * rows + row)));
+    float sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    #pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * (s * rows + row)));
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(part_acc + (s * rows + row) * D + col));
+        const float f = exp2_ftz(ml.x - ref);
+        sum = fmaf(f, ml.y, sum);
+        v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
+    }
+    const float inv = 1.f / sum;
+    uint2 o = make_uint2(pack2<BF16>(v.x * inv, v.y * inv), pack2<BF16>(v.z * inv, v.w * inv));
+    if (sum == 0.f) o = make_uint2(0, 0);
+    // row (head, i, g) of [B * heads, N, pack]
+    const long long head = row / (N * pack);
+    const int in = static_cast<int>(row - head * (N * pack)), i = in / pack, g = in - i * pack;
+    *reinterpret_cast<uint2*>(out + ((head * pack + g) * N + i) * D + col) = o;
+}
+
 // Adds the parts of the items that paged_kernel divided, and writes the zeros of those without keys.  WARPS warps to a query
 // row (4, or 1 where there are many rows): D / 4 lanes have a part's columns, and up to 4 * WARPS * 128 / D parts are on
 // their way at once.
@@ -788,7 +815,7 @@ __global__ void __launch_bounds__(kPagedThreads) combine_kernel(const __grid_con
     const int r = blockIdx.y * (kPagedWarps / WARPS) + warp / WARPS, row = (item % p.groups) * ROWS + r;
     const bool row_ok = r < ROWS && row < p.N * p.G;
     // (lengths are inputs: they were there before paged_kernel started)
-    Line line;
+    Line line = {};
     line.measure<KB>(p, lane);
     long long before = 0;
     for (int i = lane; i < b; i += 32) before += i < 32 ? line.lane_n : blocks_of<KB>(p, i).n;

@@ -272,6 +272,7 @@ struct alignas(16) RotateParams {
     int B, N, D;
     const void* positions; int wide; long long pos_sb, pos_sn;   // int64 or int32; null: first + row
     int64_t first;
+    int pack;                     // > 1: out is [B, H / pack, N, pack, D]
     const int *lengths, *counts;  // not null: the positions of a paged call's rows (counts null: all N), not the above
 };
 
@@ -316,7 +317,7 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(const __grid_con
         const RotateTensor& t = p.t[second];
         const int th = second ? h - p.t[0].H : h;
         const Chunks y = turned<FORM>(turn, place, plain, x[k], stage + threadIdx.x / per_row * p.D);
-        if (there && th < t.H) outer.store(t.out + (((long long)b * t.H + th) * p.N + n) * p.D, y);
+        if (there && th < t.H) outer.store(t.out + ((((long long)b * (t.H / p.pack) + th / p.pack) * p.N + n) * p.pack + th % p.pack) * p.D, y);
     }
 }
 

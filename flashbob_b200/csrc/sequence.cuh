@@ -8,7 +8,7 @@ namespace bob {
 enum : int { kStatusBadPage = 21, kStatusBadLength = 22 };
 
 struct SequenceParams {
-    const int* table; long long table_stride;
+    const int* table; long long table_stride;      // null: page i of sequence b is page b * max_pages + i
     const int* lengths;
     const int* counts;            // null: every row of the call
     int B, max_pages, pages, page_shift;
@@ -34,6 +34,7 @@ __device__ __forceinline__ Sequence sequence_of(const SequenceParams& p, int b, 
 
 // The page of a position below its sequence's length; -1 if the table's entry is no page.
 __device__ __forceinline__ int page_of(const SequenceParams& p, int b, int position) {
+    if (!p.table) return b * p.max_pages + (position >> p.page_shift);
     const int page = __ldg(p.table + b * p.table_stride + (position >> p.page_shift));
     return static_cast<unsigned>(page) < static_cast<unsigned>(p.pages) ? page : -1;
 }

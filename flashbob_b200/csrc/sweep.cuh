@@ -82,6 +82,12 @@ struct SweepParams {
     long long* trace;             // development builds with BOB_TRACE
     SequenceParams seq;           // kFwdPaged: map[kTK] and map[kTV] are of pages [pages, Hkv, page_size, D]
     int box_rows;                 // ... rows of a page that one copy takes: a page, or a tile of it
+    // kFwdPaged: with splits > 1 an item's tiles are divided between that many items, whose unnormalised results and
+    // (reference, sum) are added afterwards: [splits][B, Hq, Nq] rows of D, and of two.
+    // pack > 1: a head's rows are those of `pack` query heads, row i * pack + g the i-th query of head g; results go to the parts.
+    int splits, pack;
+    float* part_acc;
+    float* part_ml;
 };
 
 template <int MODE> struct ModeTraits;
@@ -323,7 +329,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
     const int n_own_tiles = (n_own + 127) / 128;
     const int grid_heads = COL ? p.Hkv : p.Hq;
     const int per_rank = grid_heads * p.B;
-    const int n_items = n_own_tiles * per_rank;
+    const int n_items = n_own_tiles * per_rank * (MODE == kFwdPaged ? p.splits : 1);
     const int n_outer = COL ? p.G : 1;
     const int doff_all = p.delta_off;            // q_offset - k_offset, within +-2^29 (see the host's fill_mask)
     // kernel parameters that the per-tile code needs, read once
@@ -334,10 +340,12 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
     // predicated on values only known at run time.
     const bool has_uq = ALLT || p.has_uq != 0, has_uk = ALLT || p.has_uk != 0, has_uv = ALLT || p.has_uv != 0;
     // lo, hi: other-side positions that can be unmasked; n_own, n_oth, doff: the sequence's own (kFwdPaged only)
-    struct Item { int own0, head, batch, kv_head, t_lo, t_hi, T, total, lo, hi, n_own, n_oth, doff; };
+    struct Item { int own0, head, batch, kv_head, t_lo, t_hi, T, total, lo, hi, n_own, n_oth, doff, split; };
     constexpr bool PAGED = MODE == kFwdPaged;
     auto decode = [&](int item) {
         Item w;
+        w.split = 0;
+        if (PAGED && p.splits > 1) { w.split = item % p.splits; item /= p.splits; }
         const int tile_rank = item / per_rank;
         const int rem = item % per_rank;
         w.head = rem % grid_heads;               // query head (row-owned) or KV head (column-owned)
@@ -348,8 +356,8 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         w.kv_head = COL ? w.head : w.head / p.G;
         w.n_own = n_own; w.n_oth = n_oth; w.doff = doff_all;
         if constexpr (PAGED) {
-            const Sequence q = sequence_of(p.seq, w.batch, p.Nq);
-            w.n_own = q.count; w.n_oth = q.length; w.doff = q.start;
+            const Sequence q = sequence_of(p.seq, w.batch, p.Nq / p.pack);
+            w.n_own = q.count * p.pack; w.n_oth = q.length; w.doff = q.start;
         }
         const int doff = w.doff;
         int lo = 0, hi = w.n_oth;                // other-side positions [lo, hi) that can be unmasked
@@ -357,8 +365,8 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         // (lengths are at most 2^28, |doff| 2^29 and the window 2^30: 32-bit sums cannot overflow)
         if (causal) {
             if (!COL) {
-                hi = min(w.n_oth, own_last + doff + 1);
-                if (window > 0) lo = max(0, w.own0 + doff - window + 1);
+                hi = min(w.n_oth, (PAGED ? own_last / p.pack : own_last) + doff + 1);
+                if (window > 0) lo = max(0, (PAGED ? w.own0 / p.pack : w.own0) + doff - window + 1);
             } else {
                 lo = max(0, w.own0 - doff);
                 if (window > 0) hi = min(n_oth, own_last - doff + window);
@@ -368,6 +376,11 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         w.lo = lo; w.hi = hi;
         w.t_lo = (hi > lo) ? lo / TN : 0;
         w.t_hi = (hi > lo) ? (hi + TN - 1) / TN : 0;
+        if (PAGED && p.splits > 1) {
+            const int tiles = w.t_hi - w.t_lo;
+            w.t_hi = w.t_lo + tiles * (w.split + 1) / p.splits;
+            w.t_lo += tiles * w.split / p.splits;
+        }
         w.T = w.t_hi - w.t_lo;
         w.total = w.T * n_outer;
         return w;
@@ -514,7 +527,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         if constexpr (PAGED) {
             if (blockIdx.x == 0) {
                 for (int b = lane; b < p.B; b += 32)
-                    if (!sequence_of(p.seq, b, p.Nq).ok) give_up(kStatusBadLength);
+                    if (!sequence_of(p.seq, b, p.Nq / p.pack).ok) give_up(kStatusBadLength);
             }
         }
         for (int k_item = 0; alive; ++k_item) {
@@ -654,6 +667,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
             if (lane == 0) {
                 #pragma unroll
                 for (int i = 0; i < CFG::N_STAGED; ++i) {
+                    if (PAGED && (p.splits > 1 || p.pack > 1)) break;        // (stored by the threads that have them)
                     #pragma unroll
                     for (int ks = 0; ks < KSUB; ++ks)
                         if (ks * 64 < p.D) tma_store_4d(&p.res_map[i], io + i * CFG::OWN_TILE_BYTES + ks * (128 * 128), ks * 64, own0, head, batch);
@@ -950,7 +964,12 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         BOB_ITEM_LOCALS(w)
         const int own_idx = own0 + row;
         const bool own_ok = own_idx < item_own;
+        const bool parted = PAGED && (p.splits > 1 || p.pack > 1);                      // results go to the parts
+        const int own_pos = PAGED ? own_idx / p.pack : own_idx;                         // (row-owned) position, from q_offset
+        (void)parted; (void)own_pos;
         const long long row_stat = ((long long)batch * p.Hq + head) * p.Nq + own_idx;   // row-owned only
+        const long long part_rows = (long long)p.B * p.Hq * p.Nq;                       // kFwdPaged: rows of a split
+        (void)part_rows;
 
         // per-row state (row-owned modes): -lse*log2e and -delta of my row
         float nL2 = 0.f, ndlt = 0.f;
@@ -1062,7 +1081,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                 int mlo = 0, mhi = min(CW - 1, item_oth - (oth0 + col0) - 1);
                 if (causal) {
                     if constexpr (!COL) {
-                        const int d0 = own_idx + doff - (oth0 + col0);       // dist falls with the column
+                        const int d0 = own_pos + doff - (oth0 + col0);       // dist falls with the column
                         mhi = min(mhi, d0);
                         if (window > 0) mlo = max(mlo, d0 - window + 1);
                     } else {
@@ -1332,9 +1351,9 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                 if (causal) {
                     // oldest and newest own position of the tile pair against the swept tile's extremes
                     if constexpr (!COL) {
-                        hi = min(hi, (own0 + doff + 1) / TN);                           // dist >= 0 everywhere
+                        hi = min(hi, ((PAGED ? own0 / p.pack : own0) + doff + 1) / TN); // dist >= 0 everywhere
                         if (window > 0) {
-                            const int x = own0 + 127 + doff - window;                   // last swept position with dist >= window
+                            const int x = (PAGED ? (own0 + 127) / p.pack : own0 + 127) + doff - window; // last swept position with dist >= window
                             lo = max(lo, x < 0 ? 0 : (x + TN) / TN);
                         }
                     } else {
@@ -1384,7 +1403,13 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
             const float m = fmaxf(m0, m1);
             const float a0 = fast_exp2(m0 - m), a1 = fast_exp2(m1 - m);
             const float l = a0 * xb[2 * 128 + row] + a1 * xb[3 * 128 + row];
-            const float inv = (l > 0.f) ? 1.f / l : 0.f;
+            float inv = (l > 0.f) ? 1.f / l : 0.f;
+            if constexpr (PAGED) {
+                if (parted) {
+                    inv = 1.f;
+                    if (grp == 0 && own_idx < n_own) *reinterpret_cast<float2*>(p.part_ml + 2 * (w.split * part_rows + row_stat)) = make_float2(m, l);
+                }
+            }
             // a group that took no tile of this item has never written its accumulator
             fwd_k0 = (total >= 1) ? a0 * inv : 0.f;
             fwd_k1 = (total >= 2) ? a1 * inv : 0.f;
@@ -1529,7 +1554,15 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                     #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         a0[i] = (fwd_k0 != 0.f ? fwd_k0 * a0[i] : 0.f) + (fwd_k1 != 0.f ? fwd_k1 * a1[i] : 0.f);
-                    stage16(io_out, col, a0);
+                    if (PAGED && parted) {
+                        float4* dst = reinterpret_cast<float4*>(p.part_acc + (w.split * part_rows + row_stat) * p.D + col);
+                        if (own_idx < n_own) {
+                            #pragma unroll
+                            for (int i = 0; i < 4; ++i) dst[i] = make_float4(a0[4 * i], a0[4 * i + 1], a0[4 * i + 2], a0[4 * i + 3]);
+                        }
+                    } else {
+                        stage16(io_out, col, a0);
+                    }
                 } else if constexpr (MODE == kBwd1Row) {
                     #pragma unroll
                     for (int i = 0; i < 16; ++i) a0[i] *= p.scale;
