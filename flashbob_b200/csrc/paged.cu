@@ -196,7 +196,11 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // unpacks the cache there), and with splits > 1 before one that adds the parts.
 struct PagedPlan { bool sweep; int pack, splits, rows, groups, ctas; size_t q_offset, ml_offset, acc_offset, kv_offset, kv_bytes, bytes; };
 
-// Most rows of a KV head's queries that paged_kernel takes.
+// Most rows of a KV head's queries that paged_kernel takes: 32 in 16 bits (16 but for fewer than 4 heads in all), 64 in 4 bits.
+// Measured, paged_kernel / tiles of 128 rows, us: 40 rows of 8 heads in 16 bits 300 keys 20.0 / 20.8, 3000 25.2 / 22.7, of 64
+// heads 25.1 / 20.5 and 49.8 / 37.4; 32 rows of one head 14.2 / 20.9 and 15.9 / 21.0.  In 4 bits unpacking costs what tiles
+// gain: 20 rows of 64 heads 1000 keys 29.7 / 33.1, 8192 97.9 / 139.5 (8 heads 45.3 / 35.6), 64 rows of 32 heads 4096 keys 51 / 55;
+// 100 rows of 48 heads 2500 keys 41 / 33, 1024 rows of 16 heads 4096 keys 259 / 63.
 constexpr int kPagedRows = 32, kPagedRows4 = 64;
 // ... in 4 bits, while the unpacked cache (as much as the page table has room for) takes no more than this.
 constexpr int64_t kMostUnpacked = (int64_t)1 << 30;
@@ -219,7 +223,7 @@ static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
     PagedPlan d = {};
     const int64_t R = (int64_t)a->N * (a->Hq / a->cache.heads);
     const int64_t rows = (int64_t)a->seq.B * a->Hq * a->N, unpacked = (int64_t)a->seq.B * a->seq.max_pages * a->cache.page_size * a->cache.heads * a->cache.D * 2;
-    d.sweep = a->cache.bits == 16 ? R > kPagedRows : R > kPagedRows4 && 2 * unpacked <= kMostUnpacked;
+    d.sweep = a->cache.bits == 16 ? R > kPagedRows || (R > 16 && (int64_t)a->seq.B * a->cache.heads >= 4) : R > kPagedRows4 && 2 * unpacked <= kMostUnpacked;
     if (d.sweep) {
         // with a tile for fewer than half of the SMs, the keys are divided too (whatever the lengths are)
         d.pack = packed_heads(a);
@@ -342,6 +346,7 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
     p.q = static_cast<const uint16_t*>(a->q); p.q_sb = a->q_strides[0]; p.q_sh = a->q_strides[1]; p.q_sn = a->q_strides[2];
     p.out = static_cast<uint16_t*>(a->out);
     p.Hq = a->Hq; p.Hkv = a->cache.heads; p.G = a->Hq / a->cache.heads; p.N = a->N;
+    p.g_part = 65536 / p.G + 1;
     p.form = rotary_form(&a->rotary);
     p.groups = d.groups;
     p.causal = a->is_causal != 0;

@@ -30,6 +30,7 @@ struct alignas(16) PagedParams {
     const uint16_t* q; long long q_sb, q_sh, q_sn;
     uint16_t* out;                // contiguous [B, Hq, N, D]
     int Hq, Hkv, G, N, form;
+    int g_part;                   // 65536 / G + 1: x / G = x * g_part / 65536 for x < 2048
     int groups;                   // row groups of ROWS query rows per KV head
     int causal, window;
     int alike;                    // keys and values (and their scales) have the same strides
@@ -240,15 +241,23 @@ struct Cursor {
         }
         const int at = static_cast<int>(pos - base), item = at / n, off = at - item * n;
         const int take = static_cast<int>(min((long long)(n - off), end - pos));
-        kv_head = item / p.groups;
-        group = item - kv_head * p.groups;
+        kv_head = item;
+        group = 0;
+        if (p.groups > 1) {
+            kv_head = item / p.groups;
+            group = item - kv_head * p.groups;
+        }
         blk = first + off;
         last = blk + take;
         whole = take == n;
         begins = off == 0;
         pos += take;
         const Sequence s = sequence_of(p.seq, b, p.N);
-        const int i0 = group * ROWS / p.G, i1 = min((min((group + 1) * ROWS, p.N * p.G) - 1) / p.G, s.count - 1);
+        int i0 = 0, i1 = min(p.N, s.count) - 1;          // its tokens
+        if (p.groups > 1) {
+            i0 = group * ROWS / p.G;
+            i1 = min(i1, (min((group + 1) * ROWS, p.N * p.G) - 1) / p.G);
+        }
         lo = p.window > 0 ? max(0, s.start + i0 - p.window + 1) : 0;
         hi = i0 > i1 ? 0 : (p.causal ? min(s.length, s.start + i1 + 1) : s.length);
         blk = max(blk, lo / KB);
@@ -393,15 +402,17 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     #pragma unroll 1
     while (seg.template next<ROWS>(p)) {
         const Sequence s = sequence_of(p.seq, seg.b, p.N);
-        const int row0 = seg.group * ROWS;
+        // row r of the item is head (r + skip) % G of token i0 + (r + skip) / G
+        const int row0 = seg.group * ROWS, i0 = seg.group ? row0 / p.G : 0, skip = row0 - i0 * p.G;
+        auto token_of = [&](int r) { return (r + skip) * p.g_part >> 16; };
         // ---- the item's queries ---------------------------------------------------------------------------
         __syncthreads();                                 // (the last item's are in registers, its sums written)
         #pragma unroll 1
         for (int id = tid; id < ROWS * (D / 16); id += kPagedThreads) {
-            const int r = row0 + id / (D / 16), c = id % (D / 16), i = r / p.G, h = seg.kv_head * p.G + r % p.G;
+            const int r = id / (D / 16), c = id % (D / 16), k = token_of(r), i = i0 + k, h = seg.kv_head * p.G + r + skip - k * p.G;
             uint16_t* dst = reinterpret_cast<uint16_t*>(paged_smem + CFG::OFF_Q + (id / (D / 16)) * CFG::Q_STRIDE);
             uint16_t* rest = PARTS ? dst + ROWS * CFG::Q_STRIDE / 2 : nullptr;
-            if (r < R && i < s.count) {
+            if (row0 + r < R && i < s.count) {
                 const uint16_t* from = p.q + seg.b * p.q_sb + h * p.q_sh + i * p.q_sn;
                 if (p.form == kHalf) bring_query<D, BF16, kHalf>(p, dst, rest, from, c, s.start + i);
                 else if (p.form == kInterleaved) bring_query<D, BF16, kInterleaved>(p, dst, rest, from, c, s.start + i);
@@ -461,13 +472,13 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
         int lo[LR], hi[LR];                              // keys that my rows attend to
         #pragma unroll
         for (int k = 0; k < LR; ++k) {
-            const int i = (row0 + 8 * k + g) / p.G;
+            const int i = i0 + token_of(8 * k + g);
             hi[k] = p.causal ? min(s.length, s.start + i + 1) : s.length;
             lo[k] = p.window > 0 ? s.start + i - p.window + 1 : 0;
         }
         // ... that every row of the item does
-        const int all_hi = p.causal ? min(s.length, s.start + row0 / p.G + 1) : s.length;
-        const int all_lo = p.window > 0 ? s.start + (row0 + ROWS - 1) / p.G - p.window + 1 : 0;
+        const int all_hi = p.causal ? min(s.length, s.start + i0 + 1) : s.length;
+        const int all_lo = p.window > 0 ? s.start + i0 + token_of(ROWS - 1) - p.window + 1 : 0;
         float acc[MT][D / 8][4], m[LR], l[LR], z[LR];    // z: 4 bits, what every column gains
         #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -739,10 +750,11 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     }
                 }
                 __syncthreads();
-                #pragma unroll 1
-                for (int id = tid; id < EXR * EXC / 4; id += kPagedThreads) {
+                #pragma unroll
+                for (int k = 0; k < (EXR * EXC / 4 + kPagedThreads - 1) / kPagedThreads; ++k) {
+                    const int id = k * kPagedThreads + tid;
                     const int r = id / (EXC / 4), col = (id % (EXC / 4)) * 4, row = row0 + pass * EXR + r;
-                    if (row >= R) continue;
+                    if (row >= R || (EXR * EXC / 4 < kPagedThreads && id >= EXR * EXC / 4)) continue;
                     float ref = sm_m[r];
                     #pragma unroll
                     for (int w = 1; w < kPagedWarps; ++w) ref = fmaxf(ref, sm_m[w * EXR + r]);
@@ -755,7 +767,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         sum = fmaf(f, sm_l[w * EXR + r], sum);
                         v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
                     }
-                    const int i = row / p.G, h = seg.kv_head * p.G + row % p.G;
+                    const int tk = token_of(pass * EXR + r), i = i0 + tk, h = seg.kv_head * p.G + pass * EXR + r + skip - tk * p.G;
                     if (i >= s.count) sum = 0.f;         // a row behind the sequence's new tokens
                     if (seg.whole) {
                         const float inv = sum == 0.f ? 0.f : 1.f / sum;      // (a row without keys is zero; NaN stays NaN)
