@@ -72,12 +72,6 @@ struct PagedConfig {
     static_assert(OFF_QF % 16 == 0, "16-byte loads");
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy8(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -317,9 +311,9 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     int fill = 0;                                        // ring slot that is free
     bool more = true;
     src.blk = src.last = 0;
-    // Lane i: where the block's keys 16 i ... lie, from the start of the cache's tensors; -1 where the page is none.
-    long long row_k = -1, row_v = 0, scale_k = 0, scale_v = 0;
-    bool inside = false;                                 // every key of the block is in reach, and its page there
+    // Lane i: where the block's keys 16 i ... lie, from the start of the cache's tensors.
+    long long row_k = 0, row_v = 0, scale_k = 0, scale_v = 0;
+    uint32_t pages = 0;                                  // bit i: ... if they do
     constexpr int RPC = 32 / CFG::CHUNKS;                // rows of a warp-wide copy
     const int copy_row = lane / CFG::CHUNKS, chunk = lane % CFG::CHUNKS;
     auto seek = [&]() {                                  // to this warp's next block, and ask for its pages
@@ -327,14 +321,15 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             more = src.template next<ROWS>(p);
             src.blk += warp;
         }
-        row_k = -1;
         if (!more) return;
+        bool there = false;
         const int key = src.blk * KB + 16 * lane;
         if (lane < KB / 16 && key + 15 >= src.lo && key < src.hi) {
             const int page = page_of(p.seq, src.b, key);
             if (page < 0) {
                 report(p.seq.sticky, kStatusBadPage);
             } else {
+                there = true;
                 const int row = key & ((1 << p.seq.page_shift) - 1);
                 auto at = [&](const CacheTensor& c) { return page * c.sp + src.kv_head * c.sh + row * c.sr; };
                 auto scale_at = [&](const CacheTensor& c) { return page * c.ssp + src.kv_head * c.ssh + row * c.ssr; };
@@ -346,41 +341,34 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                 }
             }
         }
-        inside = src.blk * KB >= src.lo && (src.blk + 1) * KB <= src.hi && !__any_sync(0xffffffffu, lane < KB / 16 && row_k < 0);
+        pages = __ballot_sync(0xffffffffu, there);
     };
     auto swizzled = [](int r, int ch) { return BITS == 4 ? ch : ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3); };
     auto copy_block = [&]() {
         if (more) {
             const uint32_t dst = ring + fill * STAGE;
-            const int key0 = src.blk * KB;
+            const int from_lo = src.blk * KB - src.lo, reach = src.hi - src.lo;
+            // rows of 16 keys lie in one page, one after another
+            auto there = [&](int r) { return static_cast<unsigned>(from_lo + r) < static_cast<unsigned>(reach) && (pages >> (r / 16) & 1); };
             #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const CacheTensor& c = p.cache[w];
-                auto to = [&](int r) { return dst + (w ? CFG::OFF_V + r * CFG::V_STRIDE : r * CFG::ROW_BYTES) + 16 * swizzled(r, chunk); };
-                if (inside) {
-                    // rows of 16 keys lie in one page, one after another
+                #pragma unroll
+                for (int sub = 0; sub < KB / 16; sub += RPC > 16 ? RPC / 16 : 1) {
+                    const long long at = __shfl_sync(0xffffffffu, w ? row_v : row_k, sub + copy_row / 16);
+                    const uint8_t* from = c.data + at + (copy_row % 16) * c.sr + 16 * chunk;
                     #pragma unroll
-                    for (int sub = 0; sub < KB / 16; sub += RPC > 16 ? RPC / 16 : 1) {
-                        const long long at = __shfl_sync(0xffffffffu, w ? row_v : row_k, sub + copy_row / 16);
-                        const uint8_t* from = c.data + at + (copy_row % 16) * c.sr + 16 * chunk;
-                        #pragma unroll
-                        for (int k = 0; k < (RPC > 16 ? 1 : 16 / RPC); ++k) copy16(to(16 * sub + copy_row + k * RPC), from + k * RPC * c.sr);
-                    }
-                } else {
-                    #pragma unroll 1
-                    for (int r = copy_row; r < KB; r += RPC) {
-                        const long long first = __shfl_sync(0xffffffffu, row_k, r / 16), at = __shfl_sync(0xffffffffu, w ? row_v : row_k, r / 16);
-                        const bool there = key0 + r >= src.lo && key0 + r < src.hi && first >= 0;
-                        copy16(to(r), there ? c.data + at + (r % 16) * c.sr + 16 * chunk : c.data, there);
+                    for (int k = 0; k < (RPC > 16 ? 1 : 16 / RPC); ++k) {
+                        const int r = 16 * sub + copy_row + k * RPC;
+                        copy16(dst + (w ? CFG::OFF_V + r * CFG::V_STRIDE : r * CFG::ROW_BYTES) + 16 * swizzled(r, chunk), from + k * RPC * c.sr, there(r));
                     }
                 }
                 if constexpr (BITS == 4) {
                     #pragma unroll
                     for (int k = 0; k < KB / 32; ++k) {
-                        const int r = k * 32 + lane, key = key0 + r;
-                        const long long first = __shfl_sync(0xffffffffu, row_k, r / 16), at = __shfl_sync(0xffffffffu, w ? scale_v : scale_k, r / 16);
-                        const bool there = inside || (key >= src.lo && key < src.hi && first >= 0);
-                        copy8(dst + (w ? CFG::OFF_SV : CFG::OFF_SK) + 8 * r, there ? c.scales + at + (r % 16) * c.ssr : c.scales, there);
+                        const int r = k * 32 + lane;
+                        const long long at = __shfl_sync(0xffffffffu, w ? scale_v : scale_k, r / 16);
+                        copy8(dst + (w ? CFG::OFF_SV : CFG::OFF_SK) + 8 * r, c.scales + at + (r % 16) * c.ssr, there(r));
                     }
                 }
             }
