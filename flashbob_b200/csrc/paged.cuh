@@ -112,7 +112,7 @@ __device__ __forceinline__ float exp2_ftz(float x) {
 template <int BITS>
 __device__ __forceinline__ float whole(float first, float rest) { return BITS == 4 || fabsf(rest) < INFINITY ? first + rest : first; }
 
-// Pairs of codes as pairs of 16-bit numbers 1 + c / 16: a shift and one logic operation, if mask and exponent come from
+// Pairs of codes as pairs of 16-bit numbers 16 + c: a shift and one logic operation, if mask and exponent come from
 // registers (with both as constants the compiler takes two operations).
 template <bool BF16>
 struct CodePairs {
@@ -120,7 +120,7 @@ struct CodePairs {
     uint32_t mask, one;
     __device__ __forceinline__ CodePairs() {
         asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(0x000f000fu << AT));
-        asm volatile("mov.b32 %0, %1;" : "=r"(one) : "n"(BF16 ? 0x3f803f80u : 0x3c003c00u));
+        asm volatile("mov.b32 %0, %1;" : "=r"(one) : "n"(BF16 ? 0x41804180u : 0x4c004c00u));
     }
     // nibbles i and i + 4 of a word
     __device__ __forceinline__ uint32_t operator()(uint32_t w, int i) const {
@@ -516,8 +516,16 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     }
                 }
             } else {
-                // codes as 16-bit numbers b = 1 + c / 16, exactly: a shift and one operation on a pair.  A score is
-                // scale q . c + zero sum q = 16 scale q . b + (zero - 16 scale) sum q.
+                // codes as 16-bit numbers b = 16 + c, exactly: a shift and one operation on a pair.  A score is
+                // scale q . c + zero sum q, with q . c = q . b - 16 sum q: the accumulators begin at that.
+                #pragma unroll
+                for (int mt = 0; mt < (ROWS == 16 ? 1 : MT); ++mt) {
+                    #pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        #pragma unroll
+                        for (int e = 0; e < (ROWS == 8 ? 2 : 4); ++e) sc[mt][i][e] = -16.f * q_sum[my_row(mt, e >> 1)];
+                    }
+                }
                 constexpr int NWD = D / 32;
                 uint32_t w[NT][NWD];
                 #pragma unroll
@@ -551,9 +559,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         if constexpr (ROWS == 32) { x[hr][i][e] = sc[0][i][2 * hr + e]; x[2 + hr][i][e] = sc[MT - 1][i][2 * hr + e]; }
                     }
                     if constexpr (BITS == 4) {
-                        const float scale = 16.f * __uint_as_float(raw[2 * e]), add = __uint_as_float(raw[2 * e + 1]) - scale;
                         #pragma unroll
-                        for (int k = 0; k < LR; ++k) x[k][i][e] = fmaf(x[k][i][e], scale, add * q_sum[k]);
+                        for (int k = 0; k < LR; ++k) x[k][i][e] = fmaf(x[k][i][e], __uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1]) * q_sum[k]);
                     }
                 }
             }
@@ -620,12 +627,12 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         pr[e] = exp2_ftz(fmaf(x[k][i][e], c_exp, -m[k]));
                         l[k] += pr[e];
                         if constexpr (BITS == 4) {
-                            // value = 16 scale b + (zero - 16 scale): the first part goes through the product, with 16 scale
+                            // value = scale b + (zero - 16 scale): the first part goes through the product, with the scale
                             // in the probability, the second is the same for every column.  In bf16 for both
                             // types: a scale may lie outside fp16.
-                            const float scale = 16.f * __uint_as_float(raw[2 * e]), add = __uint_as_float(raw[2 * e + 1]) - scale;
-                            // (one part: about the middle, so that its rounding, 2^-9, meets b - 3/2 and not b)
-                            z[k] = fmaf(pr[e], PARTS ? add : fmaf(1.5f, scale, add), z[k]);
+                            // (one part: about the middle, so that its rounding, 2^-9, meets b - 24 and not b)
+                            const float scale = __uint_as_float(raw[2 * e]);
+                            z[k] = fmaf(pr[e], fmaf(PARTS ? -16.f : 8.f, scale, __uint_as_float(raw[2 * e + 1])), z[k]);
                             pr[e] *= scale;
                         }
                     }
@@ -633,7 +640,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     float back[2];
                     if constexpr (PB) { back[0] = __uint_as_float(first << 16); back[1] = __uint_as_float(first & 0xffff0000u); }
                     else { const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&first)); back[0] = f2.x; back[1] = f2.y; }
-                    if constexpr (BITS == 4 && !PARTS) z[k] = fmaf(-1.5f, back[0] + back[1], z[k]);
+                    if constexpr (BITS == 4 && !PARTS) z[k] = fmaf(-24.f, back[0] + back[1], z[k]);
                     if constexpr (PARTS) {
                         const uint32_t rest = pack2<PB>(pr[0] - back[0], pr[1] - back[1]);
                         if constexpr (ROWS == 8) { pa[0][i / 2][2 * (i % 2)] = first; pa[0][i / 2][2 * (i % 2) + 1] = rest; }
