@@ -381,10 +381,8 @@ void run_append(const Tensor& k_, const Tensor& v_, Cache& cache, const Sequence
     set_strides(ks, k);
     set_strides(vs, v);
     const int rc = lib.cache_append(&cache.c, &seq.s, &rotary, static_cast<int>(k.size(2)), ptr(k), ks, ptr(v), vs, stream_of(k));
-    for (int i = 0; i < 2; ++i) {                // (written to: what autograd has saved of them is stale)
-        cache.data[i].unsafeGetTensorImpl()->bump_version();
-        if (cache.scales[i].defined()) cache.scales[i].unsafeGetTensorImpl()->bump_version();
-    }
+    for (const Tensor& t : {cache.data[0], cache.data[1], cache.scales[0], cache.scales[1]})
+        if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();      // what autograd has saved of them is stale
     finish_reported(rc, "bob_sm100_cache_append", cache.c.device, check_status);
 }
 

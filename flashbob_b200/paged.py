@@ -8,7 +8,7 @@
 Position t of sequence b lies in page page_table[b, t // page_size], row t % page_size.  `lengths` counts the positions
 that are there with the call's new tokens, `counts` (default: all rows of the call) the new ones: row i of sequence b sits
 at position lengths[b] - counts[b] + i in `append_kv` and in `sdpa_paged` alike.  Both live on the GPU and are never
-read by the host, so a step can be captured in a CUDA graph and replayed as sequences grow.
+read by the host, so a step can be captured in a CUDA graph (after one eager call on the device) and replayed as sequences grow.
 
 A cache of 4 bits keeps a row of a head as codes 0 ... 15 (element 2 j in the low half of byte j) and fp32 (scale, zero):
 value = code * scale + zero, with zero the row's minimum and scale 1/15 of its range (1 where that is nothing), fp32 throughout.  Keys
@@ -94,6 +94,8 @@ class PagedCache:
                 if s < reach:
                     raise ValueError(f"{name} has rows that overlap, got strides {t.stride()}")
                 reach = s * (n - 1) + reach
+        if len({t.data_ptr() for _, t, _ in checked}) < len(checked):
+            raise ValueError("keys and values (and their scales) must not lie in one place")
         self.k, self.v, self.k_scales, self.v_scales, self.dtype = k, v, k_scales, v_scales, dtype
         self._args = (k, v, k_scales, v_scales, dtype == torch.bfloat16)
         self._on_gpu = k.is_cuda
@@ -296,8 +298,12 @@ def sdpa_paged(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, len
     keeps keys at positions up to the query's, `window_size` w > 0 further keeps only the last w of them; without
     `is_causal` every query sees all lengths[b] keys, as in cross attention to cached encoder states (and `rotary` is
     refused: such queries have no position among the keys).  Rows from counts[b] on, and rows without keys, are zero.
-    Key and value rows that no query of its sequence attends to have no part in the result, whatever they hold.  H_Q is a multiple of
-    H_KV, up to 32 times.
+    Key and value rows that no query of its sequence attends to have no part in the result, whatever they hold; a NaN or infinity
+    among the values that some queries of a sequence attend to may reach its other queries of the same call, as in any
+    product of probabilities and values.  H_Q is a multiple of H_KV, up to 32 times.
+
+    Up to 16 rows (tokens of the call x H_Q / H_KV) only the result is rounded to 16 bits; beyond, turned queries and
+    probabilities are too, as in `apply_rotary` followed by `sdpa_bob`.
     """
     turn_args = _plain_rotary(rotary)
     if _native_call(cache, turn_args):

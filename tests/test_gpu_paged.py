@@ -271,6 +271,50 @@ def test_many_expanded_queries(rotary):
     R.close(a, want, bound, 0)
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("Hq,Hkv,N,lengths", [(14, 2, 33, [900, 0, 40]), (8, 8, 129, [4000]), (32, 1, 3, [50, 777]), (6, 2, 64, [64] * 5), (4, 1, 260, [3000, 260])])
+@pytest.mark.parametrize("kw", [dict(), dict(window_size=70), dict(is_causal=False)])
+def test_rows_packed_and_keys_divided(bits, Hq, Hkv, N, lengths, kw):
+    """Several heads in a tile of rows, a head's keys divided between CTAs, 4-bit caches unpacked: every way through the tiles,
+    with sequences without queries and rows behind them."""
+    counts = [max(0, min(n, N - 5 * (b % 2))) for b, n in enumerate(lengths)]
+    for D, dtype, page in ((64, torch.bfloat16, 16), (128, torch.float16, 256)):
+        rotary = None if "is_causal" in kw else Rotary(D, interleaved=D == 64)
+        _check(lengths, counts, N, Hq, Hkv, D, dtype, bits, page, rotary=rotary, **kw)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_many_rows_over_other_layouts_and_freed_pages(bits):
+    """Tiles over [page, row, head, element] storage; pages before the window are none any more."""
+    D, H, dtype = 64, 2, torch.bfloat16
+    seqs = R.Sequences([1000, 150], 32)
+    plain = _cache(seqs, H, D, dtype, bits)
+    names = ("k", "v") if bits == 16 else ("k", "v", "k_scales", "v_scales")
+    turned = [getattr(plain, n).transpose(1, 2).contiguous().transpose(1, 2) for n in names]
+    other = PagedCache(*turned[:2], **(dict(k_scales=turned[2], v_scales=turned[3], dtype=dtype) if bits == 4 else {}))
+    q = _heads((2, 4, 100, D), dtype, 2)
+    want, bound = R.attention(q, plain, seqs, window_size=60, rotary=Rotary(D))
+    seqs.table[0, : (1000 - 100 - 59) // 32] = -5
+    a = sdpa_paged(q, plain, seqs.table, seqs.lengths, window_size=60, rotary=Rotary(D))
+    R.close(a, want, bound, 0)
+    assert torch.equal(a, sdpa_paged(q, other, seqs.table, seqs.lengths, window_size=60, rotary=Rotary(D)))
+
+
+def test_in_inference_mode():
+    with torch.inference_mode():
+        seqs = R.Sequences([20], 16)
+        cache = PagedCache.allocate(seqs.pages, 1, 16, 64)
+        x = _heads((1, 1, 20, 64), torch.bfloat16, 1)
+        q, k = apply_rotary(x, x, Rotary(64))
+        append_kv(x, x, cache, seqs.table, seqs.lengths, rotary=Rotary(64))
+        assert torch.equal(read_kv(cache, seqs.table, seqs.lengths, 20)[0], k)
+    append_kv(x.clone(), x.clone(), cache, seqs.table, seqs.lengths, rotary=Rotary(64))
+    with torch.no_grad():
+        out = sdpa_paged(x.clone(), cache, seqs.table, seqs.lengths, rotary=Rotary(64))
+    want, bound = R.attention(x, cache, seqs, rotary=Rotary(64))
+    R.close(out, want, bound, 0)
+
+
 def test_pages_shared_between_sequences():
     """Two sequences with a common prefix read the same pages."""
     seqs = R.Sequences([100, 100, 60], 16)
@@ -372,8 +416,9 @@ def test_generation_step_by_step_equals_one_attention_over_the_whole():
 
 
 @pytest.mark.parametrize("bits", [16, 4])
-def test_a_captured_step_follows_lengths_and_pages_and_repeats_bits(bits):
-    B, Hq, Hkv, D, dtype = 4, 8, 2, 128, torch.bfloat16
+@pytest.mark.parametrize("Hq", [8, 64])                     # a few rows of a KV head, and enough for tiles
+def test_a_captured_step_follows_lengths_and_pages_and_repeats_bits(bits, Hq):
+    B, Hkv, D, dtype = 4, 2, 128, torch.bfloat16
     seqs = R.Sequences([900, 30, 64, 1], 32, room=40)
     cache = _cache(seqs, Hkv, D, dtype, bits, garbage=False)
     rotary = Rotary(D)

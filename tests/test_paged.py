@@ -88,6 +88,7 @@ def test_invalid_caches():
         ((z(3, 2, 16, 48).bfloat16(),) * 2, {}, ValueError), ((good.clone().requires_grad_(), good), {}, ValueError),
         ((z(3, 2, 16, 36).bfloat16()[..., :32],) * 2, {}, ValueError), ((z(3, 2, 16, 64).bfloat16()[..., ::2],) * 2, {}, ValueError),
         ((good[:1].expand(3, 2, 16, 32), good), {}, ValueError), ((good, good), dict(k_scales=scales), ValueError),
+        ((good, good), {}, ValueError), ((codes, codes.clone()), dict(k_scales=scales, v_scales=scales, dtype=torch.float16), ValueError),
         ((good, good), dict(k_scales=scales, v_scales=scales), TypeError), ((codes, codes), {}, TypeError),
         ((codes, codes), dict(k_scales=scales, v_scales=scales), TypeError),
         ((codes, codes), dict(k_scales=scales.half(), v_scales=scales.half(), dtype=torch.float16), TypeError),
