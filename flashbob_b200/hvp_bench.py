@@ -10,6 +10,9 @@ its flags, benchmarks/models/language_model_benchmark.py:625-646 for the step in
 benchmark).
 
     python -m flashbob_b200.hvp_bench --seq-lens 1024 4096 --dim 768 --heads 12 --layers 4
+
+With `--rotary` the layers turn queries and keys to their positions, through `apply_rotary` (`bob`) and in plain tensor
+operations (`math`).
 """
 
 from __future__ import annotations
@@ -24,6 +27,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .interface import sdpa_bob
+from .rotary import Rotary, apply_rotary, turn
 
 
 def math_attention(q, k, v, *, is_causal=False, scale=None):
@@ -40,11 +44,18 @@ def math_attention(q, k, v, *, is_causal=False, scale=None):
     return torch.softmax(s.float(), dim=-1).to(q.dtype) @ v
 
 
-class Layer(nn.Module):
-    """Pre-norm attention + MLP block; `kv_heads < heads` gives grouped-query attention."""
+def turned(x, rotary):
+    """x [B, H, N, D] at positions 0 ... N - 1, in plain tensor operations."""
+    return turn(x, torch.arange(x.shape[2], device=x.device), rotary)
 
-    def __init__(self, dim: int, heads: int, kv_heads: int, attention):
+
+class Layer(nn.Module):
+    """Pre-norm attention + MLP block; `kv_heads < heads` gives grouped-query attention.  `rotate` turns (q, k) to their
+    positions (None: as they are)."""
+
+    def __init__(self, dim: int, heads: int, kv_heads: int, attention, rotate=None):
         super().__init__()
+        self.rotate = rotate
         if dim % heads or heads % kv_heads:
             raise ValueError("dim must be a multiple of heads, heads a multiple of kv_heads")
         self.heads, self.kv_heads, self.hd, self.attention = heads, kv_heads, dim // heads, attention
@@ -59,6 +70,8 @@ class Layer(nn.Module):
         h = self.norm1(x)
         q = self.q(h).view(b, n, self.heads, self.hd).transpose(1, 2)
         k, v = (t.view(b, n, self.kv_heads, self.hd).transpose(1, 2) for t in self.kv(h).chunk(2, dim=-1))
+        if self.rotate is not None:
+            q, k = self.rotate(q, k)
         y = self.attention(q, k, v, is_causal=True)
         x = x + self.o(y.transpose(1, 2).reshape(b, n, -1))
         return x + self.down(F.gelu(self.up(self.norm2(x))))
@@ -78,7 +91,11 @@ BACKENDS = {"math": math_attention, "bob": sdpa_bob}
 
 def measure(backend: str, seq_len: int, args, device, dtype):
     torch.manual_seed(0)
-    model = nn.Sequential(*[Layer(args.dim, args.heads, args.kv_heads or args.heads, BACKENDS[backend])
+    rotate = None
+    if args.rotary:
+        rotary = Rotary(args.dim // args.heads)
+        rotate = (lambda q, k: apply_rotary(q, k, rotary)) if backend == "bob" else (lambda q, k: (turned(q, rotary), turned(k, rotary)))
+    model = nn.Sequential(*[Layer(args.dim, args.heads, args.kv_heads or args.heads, BACKENDS[backend], rotate)
                             for _ in range(args.layers)]).to(device=device, dtype=dtype)
     x = torch.randn(args.batch, seq_len, args.dim, device=device, dtype=dtype)
     directions = [torch.randn_like(p, dtype=torch.float32) for p in model.parameters()]
@@ -141,6 +158,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--heads", type=int, default=8)
     ap.add_argument("--kv-heads", type=int, default=0, help="fewer than --heads: grouped-query attention")
     ap.add_argument("--layers", type=int, default=2)
+    ap.add_argument("--rotary", action="store_true", help="queries and keys turned to their positions")
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--dtype", default="bf16", choices=["bf16", "fp16", "fp32"])
