@@ -43,6 +43,35 @@ class Rotary(ctypes.Structure):
     _fields_ = [("pairs", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("factor", ctypes.c_double), ("turns", ctypes.c_uint64 * 64)]
 
 
+class RotateArgs(ctypes.Structure):
+    """Mirror of `bob_sm100_rotate_args`."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "N", "D", "dtype", "device")] + \
+               [("heads", ctypes.c_int32 * 2), ("inverse", ctypes.c_int32), ("in_", _vp * 2), ("in_strides", ctypes.c_int64 * 3 * 2), ("out", _vp * 2),
+                ("positions", _vp), ("position_strides", ctypes.c_int64 * 2), ("first", ctypes.c_int64), ("position_bits", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("rotary", Rotary)]
+
+
+class Cache(ctypes.Structure):
+    """Mirror of `bob_sm100_cache`."""
+
+    _fields_ = [(n, ctypes.c_int32) for n in ("pages", "heads", "page_size", "D", "dtype", "bits", "device", "reserved")] + \
+               [("data", _vp * 2), ("strides", ctypes.c_int64 * 3 * 2), ("scales", _vp * 2), ("scale_strides", ctypes.c_int64 * 3 * 2)]
+
+
+class Sequences(ctypes.Structure):
+    """Mirror of `bob_sm100_sequences`."""
+
+    _fields_ = [("B", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("table", _vp), ("table_stride", ctypes.c_int64), ("lengths", _vp), ("counts", _vp)]
+
+
+class PagedArgs(ctypes.Structure):
+    """Mirror of `bob_sm100_paged_args`."""
+
+    _fields_ = [("cache", Cache), ("seq", Sequences), ("rotary", Rotary)] + [(n, ctypes.c_int32) for n in ("Hq", "N", "is_causal", "window")] + \
+               [("q", _vp), ("q_strides", ctypes.c_int64 * 3), ("out", _vp), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
 # every symbol include/bob_sm100.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "bob_sm100_version": (ctypes.c_int, []),

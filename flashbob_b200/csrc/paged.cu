@@ -99,7 +99,7 @@ template <class F> static void with_type(int dtype, F f) {
 
 // Rows x 16 elements from which on a thread turns four heads and shares its sines between them: with fewer, one each is as
 // fast or faster (measured, one head / four, us: 40 rows 2.2 / 2.7, 2,560 rows 2.5 / 3.3, 10,240 rows 3.4 / 3.4, 98,304 rows of 64
-// elements 7.1 / 5.4, 163,840 rows 21.1 / 15.4; eight 18.4). 
+// elements 7.1 / 5.4, 163,840 rows 21.1 / 15.4; eight 18.4).
 constexpr int64_t kSharedTurns = (int64_t)kPagedSms * 512;
 
 static int run_rotate(const bob_sm100_rotate_args* a, cudaStream_t stream, const int* lengths = nullptr, const int* counts = nullptr, int pack = 1) {
@@ -258,13 +258,17 @@ static int check_paged(const bob_sm100_paged_args* a) {
     if (a->Hq <= 0 || a->Hq % a->cache.heads || a->N <= 0 || a->N > (1 << 28)) return kBadGeom;
     if (a->window < 0 || (a->window > 0 && !a->is_causal)) return kBadGeom;
     if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return kBadGeom;
-    const int64_t R = (int64_t)a->N * (a->Hq / a->cache.heads);
-    const int64_t blocks = ((int64_t)a->seq.max_pages * a->cache.page_size + 15) / 16 + 1;
-    // a sequence's part of the line, and the grid of the second kernel, are counted in 32 bits
-    if (R > (1 << 28) || blocks * a->cache.heads * ((R + 15) / 16) > 0x7fffffffLL || (int64_t)a->seq.B * a->cache.heads * ((R + 15) / 16) > 0x7fffffffLL) return kBadGeom;
     if (int rc = check_tokens(a->q, a->q_strides)) return rc;
     if (!a->out) return kBadNull;
-    return reinterpret_cast<uintptr_t>(a->out) % 16 ? kBadAlign : 0;
+    if (reinterpret_cast<uintptr_t>(a->out) % 16) return kBadAlign;
+    if ((int64_t)a->N * (a->Hq / a->cache.heads) > (1 << 28)) return kBadGeom;
+    const PagedPlan d = paged_plan(a);
+    if (!d.sweep) {
+        // a sequence's part of the line, and the grid of the second kernel, are counted in 32 bits
+        const int64_t kb = block_keys(a->cache.D, a->cache.bits), blocks = ((int64_t)a->seq.max_pages * a->cache.page_size + kb - 1) / kb;
+        if (blocks * a->cache.heads * d.groups > 0x7fffffffLL || (int64_t)a->seq.B * a->cache.heads * d.groups > 0x7fffffffLL) return kBadGeom;
+    }
+    return 0;
 }
 
 template <int D, int ROWS, bool BF16, int BITS>

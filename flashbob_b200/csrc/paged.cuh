@@ -197,7 +197,6 @@ struct Cursor {
     int kv_head, group, blk, last, lo, hi;
     bool whole, begins;           // the segment is the whole item; ... has its first block
 
-
     // Finds the sequence that a stretch begins in.
     __device__ __forceinline__ void start(const PagedParams& p, const Line& line, int part, int lane) {
         pos = line.cut(part); end = line.cut(part + 1); base = 0; b = 0; first = 0; n = 0;
