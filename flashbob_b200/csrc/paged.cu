@@ -197,7 +197,7 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 struct PagedPlan { bool sweep; int pack, splits, rows, groups, ctas; size_t q_offset, ml_offset, acc_offset, kv_offset, kv_bytes, bytes; };
 
 // Most rows of a KV head's queries that paged_kernel takes: 32 in 16 bits (16 but for fewer than 4 heads in all), 64 in 4 bits.
-// Measured, paged_kernel / tiles of 128 rows, us: 40 rows of 8 heads in 16 bits 300 keys 20.0 / 20.8, 3000 25.2 / 22.7, of 64
+// Measured, paged_kernel / tiles of 128 rows, us: 20 rows of 8 heads in 16 bits 300 keys 20.0 / 20.8, 3000 25.2 / 22.7, of 64
 // heads 25.1 / 20.5 and 49.8 / 37.4; 32 rows of one head 14.2 / 20.9 and 15.9 / 21.0.  In 4 bits unpacking costs what tiles
 // gain: 20 rows of 64 heads 1000 keys 29.7 / 33.1, 8192 97.9 / 139.5 (8 heads 45.3 / 35.6), 64 rows of 32 heads 4096 keys 52 / 49;
 // 100 rows of 48 heads 2500 keys 41 / 33, 1024 rows of 16 heads 4096 keys 259 / 63.
@@ -293,7 +293,8 @@ static int launch_paged(PagedParams& p, int device, cudaStream_t stream) {
     cfg.stream = stream;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    // a CTA to a row while all of them run at once (512 rows in 37 parts each 31 us with a warp, 29 with four)
+    // a CTA to a row while all of them run at once (the whole call, a warp / four to a row,
+    // us: 512 rows in 9 parts each 29.3 / 28.8, 128 rows in 74 parts 31.1 / 30.2)
     if (items * rows <= kPagedSms * 8) {
         cfg.gridDim = dim3((unsigned)items, (unsigned)rows);
         return cudaLaunchKernelEx(&cfg, combine_kernel<D, ROWS, BF16, BITS, 4>, p) == cudaSuccess ? 0 : kBadLaunch;

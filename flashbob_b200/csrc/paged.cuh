@@ -418,8 +418,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
         const uint32_t q_rows = smem_u32(paged_smem) + CFG::OFF_Q, q_frags = smem_u32(paged_smem) + CFG::OFF_QF + 16 * lane;
         if constexpr (BITS == 4) {
             // the elements in the order in which a word of codes yields them: thread t holds words NWD t ... of a
-            // key row, and a word's pairs are (e, e + 4).  Kept in shared memory: in registers they leave room for 12
-            // warps per SM instead of 16.
+            // key row, and a word's pairs are (e, e + 4).  Kept in shared memory: the 32 to 64 registers that they
+            // would take are those of the third CTA per SM.
             #pragma unroll
             for (int k = 0; k < LR; ++k) q_sum[k] = 0.f;
             constexpr int NWD = D / 32;

@@ -9,8 +9,8 @@
 //
 // What bounds it: one read and one write of every element.  A thread turns the same 16 elements (8 pairs) of HPT heads of
 // a token, so its 8 sines and cosines are shared by them and their loads are in flight together.  They are the special-
-// function unit's: off by 2^-20.9 at most, a thousandth of the result's rounding in fp16 (with sincospif, four times the
-// instructions, the kernel spent 31 us on 84 MB with one head a thread, 18 with four).
+// function unit's: off by 2^-20.9 at most, a thousandth of the result's rounding in fp16 (sincospif, with four times the
+// instructions, took 31 us for 29.5 on 84 MB with one head a thread, 18 for 17.1 with four).
 #pragma once
 
 #include "ptx.cuh"
@@ -76,8 +76,8 @@ __device__ __forceinline__ void turn_factors(int64_t position, uint64_t turn, do
 }
 
 // Frequencies 2 i and 2 i + 1 of a rotation that is a kernel parameter, by its address: read as constants, which a warp takes
-// one address at a time, the eight frequencies of every thread took most of the kernel's time (29 us, with them as ordinary
-// loads 15, on 84 MB with one head a thread).
+// one address at a time, the eight frequencies of every thread took most of the kernel's time (84 MB with one head a
+// thread 29.5 us, with them as ordinary loads 21.1; with four heads a thread 17.1 and 15.4).
 __device__ __forceinline__ ulonglong2 turn_pair(const bob_sm100_rotary& r, int i) {
     ulonglong2 x;
     asm("ld.v2.u64 {%0, %1}, [%2];" : "=l"(x.x), "=l"(x.y) : "l"(r.turns + 2 * i));
