@@ -112,19 +112,20 @@ __device__ __forceinline__ float exp2_ftz(float x) {
 template <int BITS>
 __device__ __forceinline__ float whole(float first, float rest) { return BITS == 4 || fabsf(rest) < INFINITY ? first + rest : first; }
 
-// Pairs of codes as pairs of 16-bit numbers 16 + c: a shift and one logic operation, if mask and exponent come from
-// registers (with both as constants the compiler takes two operations).
-template <bool BF16>
+// Pairs of codes (nibbles i and i + 4 of a word) as pairs of fp16 numbers: one logic operation, and a shift for two of them.
+// The bits of c alone are the subnormal number c 2^-24 (i even) or c 2^-20 (i odd).
+__device__ __forceinline__ uint32_t subnormal_codes(uint32_t w, int i) { return (i & 2 ? w >> 8 : w) & (i & 1 ? 0x00f000f0u : 0x000f000fu); }
+
+// ... as pairs of bf16 numbers 16 + c: a shift and one logic operation, if mask and exponent come from registers (with both as
+// constants the compiler takes two operations).
 struct CodePairs {
-    static constexpr int AT = BF16 ? 3 : 6;              // where the code goes: the mantissa's upper four bits
     uint32_t mask, one;
     __device__ __forceinline__ CodePairs() {
-        asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(0x000f000fu << AT));
-        asm volatile("mov.b32 %0, %1;" : "=r"(one) : "n"(BF16 ? 0x41804180u : 0x4c004c00u));
+        asm volatile("mov.b32 %0, %1;" : "=r"(mask) : "n"(0x000f000fu << 3));       // the mantissa's upper four bits
+        asm volatile("mov.b32 %0, %1;" : "=r"(one) : "n"(0x41804180u));
     }
-    // nibbles i and i + 4 of a word
     __device__ __forceinline__ uint32_t operator()(uint32_t w, int i) const {
-        const int by = 4 * i - AT;
+        const int by = 4 * i - 3;
         const uint32_t x = by < 0 ? w << -by : w >> by;
         uint32_t r;
         asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(one));       // (x & mask) | one
@@ -310,9 +311,10 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     int fill = 0;                                        // ring slot that is free
     bool more = true;
     src.blk = src.last = 0;
-    // Lane i: where the block's keys 16 i ... lie, from the start of the cache's tensors.
-    long long row_k = 0, row_v = 0, scale_k = 0, scale_v = 0;
-    uint32_t pages = 0;                                  // bit i: ... if they do
+    // Lane i: the page of the block's keys 16 i ... if the item reads any of them.  It is asked for a block ahead, and looked
+    // at when the block is copied.
+    int entry = 0;
+    bool asked = false;
     constexpr int RPC = 32 / CFG::CHUNKS;                // rows of a warp-wide copy
     const int copy_row = lane / CFG::CHUNKS, chunk = lane % CFG::CHUNKS;
     auto seek = [&]() {                                  // to this warp's next block, and ask for its pages
@@ -321,44 +323,42 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             src.blk += warp;
         }
         if (!more) return;
-        bool there = false;
         const int key = src.blk * KB + 16 * lane;
-        if (lane < KB / 16 && key + 15 >= src.lo && key < src.hi) {
-            const int page = page_of(p.seq, src.b, key);
-            if (page < 0) {
-                report(p.seq.sticky, kStatusBadPage);
-            } else {
-                there = true;
-                const int row = key & ((1 << p.seq.page_shift) - 1);
-                auto at = [&](const CacheTensor& c) { return page * c.sp + src.kv_head * c.sh + row * c.sr; };
-                auto scale_at = [&](const CacheTensor& c) { return page * c.ssp + src.kv_head * c.ssh + row * c.ssr; };
-                row_k = row_v = at(p.cache[0]);
-                if constexpr (BITS == 4) scale_k = scale_v = scale_at(p.cache[0]);
-                if (!p.alike) {
-                    row_v = at(p.cache[1]);
-                    if constexpr (BITS == 4) scale_v = scale_at(p.cache[1]);
-                }
-            }
-        }
-        pages = __ballot_sync(0xffffffffu, there);
+        asked = lane < KB / 16 && key + 15 >= src.lo && key < src.hi;
+        if (asked) entry = page_entry(p.seq, src.b, key);
     };
     auto swizzled = [](int r, int ch) { return BITS == 4 ? ch : ch ^ (CFG::CHUNKS >= 8 ? r & 7 : (r >> 1) & 3); };
     auto copy_block = [&]() {
         if (more) {
             const uint32_t dst = ring + fill * STAGE;
             const int from_lo = src.blk * KB - src.lo, reach = src.hi - src.lo;
+            const bool found = asked && static_cast<unsigned>(entry) < static_cast<unsigned>(p.seq.pages);
+            if (asked && !found) report(p.seq.sticky, kStatusBadPage);
+            const uint32_t pages = __ballot_sync(0xffffffffu, found);
+            const int page = found ? entry : 0, row = (src.blk * KB + 16 * lane) & ((1 << p.seq.page_shift) - 1);
             // rows of 16 keys lie in one page, one after another
             auto there = [&](int r) { return static_cast<unsigned>(from_lo + r) < static_cast<unsigned>(reach) && (pages >> (r / 16) & 1); };
+            constexpr int STEP = RPC > 16 ? RPC / 16 : 1, GROUPS = KB / 16 / STEP;
+            long long at[GROUPS], scale_at[KB / 32 + 1];
             #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const CacheTensor& c = p.cache[w];
+                if (w == 0 || !p.alike) {
+                    const long long mine = page * c.sp + src.kv_head * c.sh + row * c.sr;
+                    #pragma unroll
+                    for (int i = 0; i < GROUPS; ++i) at[i] = __shfl_sync(0xffffffffu, mine, i * STEP + copy_row / 16);
+                    if constexpr (BITS == 4) {
+                        const long long scale = page * c.ssp + src.kv_head * c.ssh + row * c.ssr;
+                        #pragma unroll
+                        for (int i = 0; i < KB / 32; ++i) scale_at[i] = __shfl_sync(0xffffffffu, scale, 2 * i + lane / 16);
+                    }
+                }
                 #pragma unroll
-                for (int sub = 0; sub < KB / 16; sub += RPC > 16 ? RPC / 16 : 1) {
-                    const long long at = __shfl_sync(0xffffffffu, w ? row_v : row_k, sub + copy_row / 16);
-                    const uint8_t* from = c.data + at + (copy_row % 16) * c.sr + 16 * chunk;
+                for (int i = 0; i < GROUPS; ++i) {
+                    const uint8_t* from = c.data + at[i] + (copy_row % 16) * c.sr + 16 * chunk;
                     #pragma unroll
                     for (int k = 0; k < (RPC > 16 ? 1 : 16 / RPC); ++k) {
-                        const int r = 16 * sub + copy_row + k * RPC;
+                        const int r = 16 * i * STEP + copy_row + k * RPC;
                         copy16(dst + (w ? CFG::OFF_V + r * CFG::V_STRIDE : r * CFG::ROW_BYTES) + 16 * swizzled(r, chunk), from + k * RPC * c.sr, there(r));
                     }
                 }
@@ -366,8 +366,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     #pragma unroll
                     for (int k = 0; k < KB / 32; ++k) {
                         const int r = k * 32 + lane;
-                        const long long at = __shfl_sync(0xffffffffu, w ? scale_v : scale_k, r / 16);
-                        copy8(dst + (w ? CFG::OFF_SV : CFG::OFF_SK) + 8 * r, c.scales + at + (r % 16) * c.ssr, there(r));
+                        copy8(dst + (w ? CFG::OFF_SV : CFG::OFF_SK) + 8 * r, c.scales + scale_at[k] + (r % 16) * c.ssr, there(r));
                     }
                 }
             }
@@ -384,8 +383,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
 
     const float c_exp = p.scale * kLog2e;
     const int R = p.N * p.G;
-    const CodePairs<BF16> key_codes;
-    const CodePairs<true> value_codes;
+    const CodePairs value_codes;
     #pragma unroll 1
     while (seg.template next<ROWS>(p)) {
         const Sequence s = sequence_of(p.seq, seg.b, p.N);
@@ -411,40 +409,64 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             }
         }
         __syncthreads();
-        float q_sum[LR];                                 // 4 bits: sum of a row's elements
-        (void)q_sum;
+        float q_sum[LR], c_row[LR];                      // 4 bits: sum of a row's elements, what its scores are in
+        (void)q_sum; (void)c_row;
         // row of mine (LR of them) that half hr of product mt has, or a part of
         auto my_row = [](int mt, int hr) { return ROWS == 8 ? 0 : ROWS == 16 ? hr : 2 * mt + hr; };
         const uint32_t q_rows = smem_u32(paged_smem) + CFG::OFF_Q, q_frags = smem_u32(paged_smem) + CFG::OFF_QF + 16 * lane;
         if constexpr (BITS == 4) {
             // the elements in the order in which a word of codes yields them: thread t holds words NWD t ... of a
-            // key row, and a word's pairs are (e, e + 4).  Kept in shared memory: the 32 to 64 registers that they
-            // would take are those of the third CTA per SM.
-            #pragma unroll
-            for (int k = 0; k < LR; ++k) q_sum[k] = 0.f;
+            // key row, and a word's pairs are (e, e + 4).  In fp16, as the codes are, times a power of two that
+            // brings the row's largest to 2^14 (a part loses nothing but what is below 2^-38 of it), and those that meet
+            // c 2^-20 times 1/16.  Kept in shared memory: the registers that they would take are those of the third CTA per SM.
             constexpr int NWD = D / 32;
+            float up[LR];
             #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 uint32_t frag[KS][4];
                 #pragma unroll
                 for (int hr = 0; hr < 2; ++hr) {
-                    float sum = 0.f;
+                    const int k = my_row(mt, hr);
+                    const bool rest = PARTS && (ROWS == 8 ? hr : mt) == 1;
+                    float f[NWD][8];
                     #pragma unroll
                     for (int j = 0; j < NWD; ++j) {
                         uint32_t w[4];
                         lds_words<4>(q_rows + (mt * 16 + g + 8 * hr) * CFG::Q_STRIDE + 16 * (NWD * t + j), w);
-                        float f[8];
-                        widen8<BF16>(make_uint4(w[0], w[1], w[2], w[3]), f);
+                        widen8<BF16>(make_uint4(w[0], w[1], w[2], w[3]), f[j]);
+                    }
+                    if (!rest) {
+                        float largest = 0.f;
                         #pragma unroll
-                        for (int e = 0; e < 8; ++e) sum += f[e];
+                        for (int j = 0; j < NWD; ++j) {
+                            #pragma unroll
+                            for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(f[j][e]));
+                        }
+                        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                        // (from 2^-100 to 2^117, so that neither power leaves fp32's range: elements above 2^118 may be infinite)
+                        const int exponent = min(max(static_cast<int>(__float_as_uint(largest) >> 23), 127 - 100), 127 + 117);
+                        up[k] = __uint_as_float(static_cast<uint32_t>(2 * 127 + 14 - exponent) << 23);
+                        c_row[k] = c_exp * __uint_as_float(static_cast<uint32_t>(exponent - 14 + 24) << 23);
+                        q_sum[k] = 0.f;
+                    }
+                    float sum = 0.f;
+                    #pragma unroll
+                    for (int j = 0; j < NWD; ++j) {
+                        #pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            f[j][e] *= up[k];
+                            sum += f[j][e];
+                            if (e & 1) f[j][e] *= 0.0625f;
+                        }
                         #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            frag[2 * j + half][hr] = __byte_perm(w[half], w[2 + half], 0x5410);
-                            frag[2 * j + half][2 + hr] = __byte_perm(w[half], w[2 + half], 0x7632);
+                            frag[2 * j + half][hr] = pack2<false>(f[j][2 * half], f[j][2 * half + 4]);
+                            frag[2 * j + half][2 + hr] = pack2<false>(f[j][2 * half + 1], f[j][2 * half + 5]);
                         }
                     }
                     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                    q_sum[my_row(mt, hr)] += sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+                    q_sum[k] = fmaf(sum + __shfl_xor_sync(0xffffffffu, sum, 2), 0x1p-24f, q_sum[k]);
                 }
                 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
@@ -515,16 +537,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     }
                 }
             } else {
-                // codes as 16-bit numbers b = 16 + c, exactly: a shift and one operation on a pair.  A score is
-                // scale q . c + zero sum q, with q . c = q . b - 16 sum q: the accumulators begin at that.
-                #pragma unroll
-                for (int mt = 0; mt < (ROWS == 16 ? 1 : MT); ++mt) {
-                    #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        #pragma unroll
-                        for (int e = 0; e < (ROWS == 8 ? 2 : 4); ++e) sc[mt][i][e] = -16.f * q_sum[my_row(mt, e >> 1)];
-                    }
-                }
+                // a score is scale q . c + zero sum q, in multiples of c_row / c_exp
                 constexpr int NWD = D / 32;
                 uint32_t w[NT][NWD];
                 #pragma unroll
@@ -538,9 +551,9 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         for (int mt = 0; mt < MT; ++mt) query(mt, 2 * j + half, qa[mt]);
                         #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const uint32_t b0 = key_codes(w[nt][j], 2 * half), b1 = key_codes(w[nt][j], 2 * half + 1);
+                            const uint32_t b0 = subnormal_codes(w[nt][j], 2 * half), b1 = subnormal_codes(w[nt][j], 2 * half + 1);
                             #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) mma16816<BF16>(sc[mt][nt], qa[mt], b0, b1);
+                            for (int mt = 0; mt < MT; ++mt) mma16816<false>(sc[mt][nt], qa[mt], b0, b1);
                         }
                     }
                 }
@@ -590,7 +603,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                 for (int i = 1; i < NT; ++i) v = fmaxf(v, fmaxf(x[k][i][0], x[k][i][1]));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-                top[k] = fmaxf(v * c_exp, kNone);        // (the scale is positive)
+                top[k] = fmaxf(v * (BITS == 4 ? c_row[k] : c_exp), kNone);        // (the scale is positive)
                 grow = grow || top[k] > m[k] + 8.f;
             }
             // the reference moves only when the maximum has outgrown it by 2^8
@@ -623,7 +636,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     constexpr bool PB = BITS == 4 || BF16;
                     #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        pr[e] = exp2_ftz(fmaf(x[k][i][e], c_exp, -m[k]));
+                        pr[e] = exp2_ftz(fmaf(x[k][i][e], BITS == 4 ? c_row[k] : c_exp, -m[k]));
                         l[k] += pr[e];
                         if constexpr (BITS == 4) {
                             // value = scale b + (zero - 16 scale): the first part goes through the product, with the scale

@@ -32,10 +32,15 @@ __device__ __forceinline__ Sequence sequence_of(const SequenceParams& p, int b, 
     return s;
 }
 
-// The page of a position below its sequence's length; -1 if the table's entry is no page.
-__device__ __forceinline__ int page_of(const SequenceParams& p, int b, int position) {
+// The table's entry for a position below its sequence's length, as it stands there.
+__device__ __forceinline__ int page_entry(const SequenceParams& p, int b, int position) {
     if (!p.table) return b * p.max_pages + (position >> p.page_shift);
-    const int page = __ldg(p.table + b * p.table_stride + (position >> p.page_shift));
+    return __ldg(p.table + b * p.table_stride + (position >> p.page_shift));
+}
+
+// ... -1 if it is no page.
+__device__ __forceinline__ int page_of(const SequenceParams& p, int b, int position) {
+    const int page = page_entry(p, b, position);
     return static_cast<unsigned>(page) < static_cast<unsigned>(p.pages) ? page : -1;
 }
 
