@@ -199,8 +199,8 @@ struct PagedPlan { bool sweep; int pack, splits, rows, groups, ctas; size_t q_of
 // Most rows of a KV head's queries that paged_kernel takes: 32 in 16 bits (16 but for fewer than 4 heads in all), 64 in 4 bits.
 // Measured, paged_kernel / tiles of 128 rows, us: 20 rows of 8 heads in 16 bits 300 keys 20.0 / 20.8, 3000 25.2 / 22.7, of 64
 // heads 25.1 / 20.5 and 49.8 / 37.4; 32 rows of one head 14.2 / 20.9 and 15.9 / 21.0.  In 4 bits unpacking costs what tiles
-// gain: 20 rows of 64 heads 1000 keys 29.7 / 33.1, 8192 97.9 / 139.5 (8 heads 45.3 / 35.6), 64 rows of 32 heads 4096 keys 52 / 49;
-// 100 rows of 48 heads 2500 keys 41 / 33, 1024 rows of 16 heads 4096 keys 259 / 63.
+// gain, us: 8 sequences x 64 heads x 20 rows, 1000 keys 107 / 143, 8192 354 / 355 (one sequence of 8 heads 39 / 35); 4 sequences x 8 heads x
+// 64 rows, 4096 keys 42 / 50; 3 sequences x 16 heads x 100 rows, 2500 keys 77 / 51, 500 45 / 29.
 constexpr int kPagedRows = 32, kPagedRows4 = 64;
 // ... in 4 bits, while the unpacked cache (as much as the page table has room for) takes no more than this.
 constexpr int64_t kMostUnpacked = (int64_t)1 << 30;

@@ -40,6 +40,7 @@ struct alignas(16) PagedParams {
     int ctas;                     // CTAs of paged_kernel
 };
 
+constexpr float kLog2e = 1.4426950408889634f, kNone = -3e38f;         // (kNone: the reference of a row without keys)
 constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedMinBlocks = 4;          // blocks that are worth a CTA of their own
 
@@ -105,6 +106,9 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// A factor that neither infinities nor zeros are lost on.
+__device__ __forceinline__ float in_range(float x) { return fminf(fmaxf(x, 0x1p-126f), 3e38f); }
 
 // A product with a value's first part, and with the rest of it.  An infinite element makes the second one infinite of
 // either sign or NaN, and decides the first alone.
@@ -284,8 +288,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     using CFG = PagedConfig<D, ROWS, BITS>;
     constexpr int KB = CFG::KB, SUB = CFG::SUB, NT = SUB / 8, KS = D / 16, NST = CFG::NST, STAGE = CFG::STAGE, MT = CFG::MT, LR = CFG::LR;
     constexpr bool PARTS = CFG::PARTS;
-    constexpr float kLog2e = 1.4426950408889634f, kNone = -1e30f;
-    extern __shared__ __align__(128) uint8_t paged_smem[];
+        extern __shared__ __align__(128) uint8_t paged_smem[];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
     const uint32_t ring = smem_u32(paged_smem) + warp * NST * STAGE;
     constexpr int EXR = CFG::EX_ROWS, EXC = CFG::EX_COLS;
@@ -381,7 +384,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
     for (int i = 0; i < NST - 1; ++i) copy_block();
     int slot = 0;                                        // ring slot of the next block to use
 
-    const float c_exp = p.scale * kLog2e;
+    const float c_exp = in_range(p.scale * kLog2e);
     const int R = p.N * p.G;
     const CodePairs value_codes;
     #pragma unroll 1
@@ -409,8 +412,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             }
         }
         __syncthreads();
-        float q_sum[LR], c_row[LR];                      // 4 bits: sum of a row's elements, what its scores are in
-        (void)q_sum; (void)c_row;
+        float q_sum[LR], unit[LR];                       // 4 bits: sum of a row's elements, what its scores are multiples of
+        (void)q_sum; (void)unit;
         // row of mine (LR of them) that half hr of product mt has, or a part of
         auto my_row = [](int mt, int hr) { return ROWS == 8 ? 0 : ROWS == 16 ? hr : 2 * mt + hr; };
         const uint32_t q_rows = smem_u32(paged_smem) + CFG::OFF_Q, q_frags = smem_u32(paged_smem) + CFG::OFF_QF + 16 * lane;
@@ -444,10 +447,10 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         }
                         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
                         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                        // (from 2^-100 to 2^117, so that neither power leaves fp32's range: elements above 2^118 may be infinite)
-                        const int exponent = min(max(static_cast<int>(__float_as_uint(largest) >> 23), 127 - 100), 127 + 117);
+                        // (neither power leaves fp32's range: scores of queries above 2^117 become 2^10 times smaller at most)
+                        const int exponent = min(max(static_cast<int>(__float_as_uint(largest) >> 23), 127 - 100), 254);
                         up[k] = __uint_as_float(static_cast<uint32_t>(2 * 127 + 14 - exponent) << 23);
-                        c_row[k] = c_exp * __uint_as_float(static_cast<uint32_t>(exponent - 14 + 24) << 23);
+                        unit[k] = __uint_as_float(static_cast<uint32_t>(min(exponent - 14 + 24, 254)) << 23);
                         q_sum[k] = 0.f;
                     }
                     float sum = 0.f;
@@ -488,6 +491,11 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
         // ... that every row of the item does
         const int all_hi = p.causal ? min(s.length, s.start + i0 + 1) : s.length;
         const int all_lo = p.window > 0 ? s.start + i0 + token_of(ROWS - 1) - p.window + 1 : 0;
+        // a probability is 2^((x - m) c): the reference m is a score as it is, so that the largest one's difference from it is
+        // zero however large both are
+        float c[LR];
+        #pragma unroll
+        for (int k = 0; k < LR; ++k) c[k] = BITS == 4 ? in_range(c_exp * unit[k]) : c_exp;
         float acc[MT][D / 8][4], m[LR], l[LR], z[LR];    // z: 4 bits, what every column gains
         #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -537,7 +545,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     }
                 }
             } else {
-                // a score is scale q . c + zero sum q, in multiples of c_row / c_exp
+                // a score is scale q . c + zero sum q, in multiples of the row's unit
                 constexpr int NWD = D / 32;
                 uint32_t w[NT][NWD];
                 #pragma unroll
@@ -603,8 +611,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                 for (int i = 1; i < NT; ++i) v = fmaxf(v, fmaxf(x[k][i][0], x[k][i][1]));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
                 v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-                top[k] = fmaxf(v * (BITS == 4 ? c_row[k] : c_exp), kNone);        // (the scale is positive)
-                grow = grow || top[k] > m[k] + 8.f;
+                top[k] = fmaxf(v, kNone);
+                grow = grow || (top[k] - m[k]) * c[k] > 8.f;         // (the scale is positive)
             }
             // the reference moves only when the maximum has outgrown it by 2^8
             if (__any_sync(0xffffffffu, grow)) {
@@ -612,7 +620,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                 #pragma unroll
                 for (int k = 0; k < LR; ++k) {
                     const float ref = fmaxf(m[k], top[k]);
-                    f[k] = exp2_ftz(m[k] - ref);
+                    f[k] = exp2_ftz((m[k] - ref) * c[k]);
                     m[k] = ref;
                     l[k] *= f[k];
                     if constexpr (BITS == 4) z[k] *= f[k];
@@ -636,7 +644,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     constexpr bool PB = BITS == 4 || BF16;
                     #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        pr[e] = exp2_ftz(fmaf(x[k][i][e], BITS == 4 ? c_row[k] : c_exp, -m[k]));
+                        pr[e] = exp2_ftz((x[k][i][e] - m[k]) * c[k]);
                         l[k] += pr[e];
                         if constexpr (BITS == 4) {
                             // value = scale b + (zero - 16 scale): the first part goes through the product, with the scale
@@ -733,7 +741,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     zs += __shfl_xor_sync(0xffffffffu, zs, 1);
                     z[k] = zs + __shfl_xor_sync(0xffffffffu, zs, 2);
                 }
-                if (t == 0) { sm_m[warp * EXR + j * 8 + g] = m[k]; sm_l[warp * EXR + j * 8 + g] = sum; }
+                if (t == 0) { sm_m[warp * EXR + j * 8 + g] = BITS == 4 && m[k] > kNone ? m[k] * unit[k] : m[k]; sm_l[warp * EXR + j * 8 + g] = sum; }
             }
             if (lane == 0) sm_slot[warp] = (warp * NST + fill) * STAGE;
             #pragma unroll
@@ -769,7 +777,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     #pragma unroll
                     for (int w = 0; w < kPagedWarps; ++w) {
-                        const float f = exp2_ftz(sm_m[w * EXR + r] - ref);
+                        const float f = exp2_ftz((sm_m[w * EXR + r] - ref) * c_exp);
                         const float4 x = *reinterpret_cast<const float4*>(paged_smem + sm_slot[w] + 4 * (r * EXC + (col ^ ((r & 3) << 3))));
                         sum = fmaf(f, sm_l[w * EXR + r], sum);
                         v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
@@ -855,7 +863,8 @@ __global__ void __launch_bounds__(kPagedThreads) combine_kernel(const __grid_con
         if (row_ok && mine == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
         return;
     }
-    float ref = -1e30f, sum = 0.f;
+    const float c_exp = in_range(p.scale * kLog2e);
+    float ref = kNone, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = c0 + mine; row_ok && c <= c1; c += BATCH * STEP) {
         float2 ml[BATCH];
@@ -863,7 +872,7 @@ __global__ void __launch_bounds__(kPagedThreads) combine_kernel(const __grid_con
         #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
             const int part = c + k * STEP;
-            ml[k] = make_float2(-1e30f, 0.f);
+            ml[k] = make_float2(kNone, 0.f);
             x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (part <= c1) {
                 // slot 1 of the CTA where the item begins, slot 0 of those where it goes on
@@ -875,13 +884,13 @@ __global__ void __launch_bounds__(kPagedThreads) combine_kernel(const __grid_con
         float top = ref;
         #pragma unroll
         for (int k = 0; k < BATCH; ++k) top = fmaxf(top, ml[k].x);
-        const float back = exp2_ftz(ref - top);
+        const float back = exp2_ftz((ref - top) * c_exp);
         ref = top;
         sum *= back;
         v.x *= back; v.y *= back; v.z *= back; v.w *= back;
         #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
-            const float f = exp2_ftz(ml[k].x - top);
+            const float f = exp2_ftz((ml[k].x - top) * c_exp);
             sum = fmaf(f, ml[k].y, sum);
             v.x = fmaf(f, x[k].x, v.x); v.y = fmaf(f, x[k].y, v.y); v.z = fmaf(f, x[k].z, v.z); v.w = fmaf(f, x[k].w, v.w);
         }
@@ -897,7 +906,7 @@ __global__ void __launch_bounds__(kPagedThreads) combine_kernel(const __grid_con
     v = make_float4(0.f, 0.f, 0.f, 0.f);
     #pragma unroll
     for (int k = 0; k < STEP; ++k) {
-        const float f = exp2_ftz(sm_ml[group + k].x - top);
+        const float f = exp2_ftz((sm_ml[group + k].x - top) * c_exp);
         const float4 x = sm_acc[group + k][lane % LPR];
         sum = fmaf(f, sm_ml[group + k].y, sum);
         v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
