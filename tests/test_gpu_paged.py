@@ -300,6 +300,28 @@ def test_many_rows_over_other_layouts_and_freed_pages(bits):
     assert torch.equal(a, sdpa_paged(q, other, seqs.table, seqs.lengths, window_size=60, rotary=Rotary(D)))
 
 
+@pytest.mark.parametrize("bits,pages", [(16, 64000), (4, 256000)])
+def test_offsets_of_more_than_32_bits(bits, pages):
+    """Keys and values of 8.4 GB each: rows written, read and attended to at both ends."""
+    D, H, page, lengths = 128, 8, 64, [3000, 65, 700]
+    seqs = R.Sequences(lengths, page, extra_pages=pages)
+    cache = PagedCache.allocate(seqs.pages, H, page, D, dtype=torch.bfloat16, bits=bits)
+    page_bytes = cache.k.stride(0) * cache.k.element_size()
+    assert int(seqs.table.max()) * page_bytes > 2 ** 32 > int(seqs.table.clamp(min=0).min()) * page_bytes
+    k, v = (_heads((3, H, 3000, D), torch.bfloat16, seed) for seed in (1, 2))
+    append_kv(k, v, cache, seqs.table, seqs.lengths, counts=seqs.lengths)
+    got = read_kv(cache, seqs.table, seqs.lengths, 3000)
+    for which, x, y in (("k", k, got[0]), ("v", v, got[1])):
+        for b, n in enumerate(lengths):
+            rows, _ = R.values(cache, which, seqs, b, n)
+            assert torch.equal(y[b, :, :n], rows.to(y.dtype)) if bits == 4 else torch.equal(y[b, :, :n], x[b, :, :n])
+    for N, counts in ((1, [1, 1, 1]), (40, [40, 40, 33])):
+        q = _heads((3, 2 * H, N, D), torch.bfloat16, 5)
+        counts = torch.tensor(counts, dtype=torch.int32, device="cuda")
+        want, bound = R.attention(q, cache, seqs, counts)
+        R.close(sdpa_paged(q, cache, seqs.table, seqs.lengths, counts=counts), want, bound, TINY[torch.bfloat16])
+
+
 def test_in_inference_mode():
     with torch.inference_mode():
         seqs = R.Sequences([20], 16)
