@@ -340,7 +340,7 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
         if (d.splits == 1 && d.pack == 1) return 0;
         const int64_t rows = (int64_t)a->seq.B * a->Hq * a->N, blocks = (rows * (a->cache.D / 4) + 255) / 256;
         with_type(a->cache.dtype, [&](auto bf16) {
-            add_splits_kernel<decltype(bf16)::value><<<(unsigned)blocks, 256, 0, stream>>>(ml, acc, static_cast<uint16_t*>(a->out), d.splits, rows, a->cache.D, a->N, d.pack);
+            add_splits_kernel<decltype(bf16)::value><<<(unsigned)blocks, 256, 0, stream>>>(ml, acc, static_cast<uint16_t*>(a->out), d.splits, rows, a->cache.D, a->N, d.pack, a->scale);
         });
         return launched();
     }

@@ -802,11 +802,12 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
 
 // Adds the parts of a forward whose tiles were divided (SweepParams::splits, pack): one thread per four columns of a row.
 template <bool BF16>
-__global__ void __launch_bounds__(256) add_splits_kernel(const float* part_ml, const float* part_acc, uint16_t* out, int splits, long long rows, int D, int N, int pack) {
+__global__ void __launch_bounds__(256) add_splits_kernel(const float* part_ml, const float* part_acc, uint16_t* out, int splits, long long rows, int D, int N, int pack, float scale) {
     const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / (D / 4);
     const int col = static_cast<int>(id % (D / 4)) * 4;
     if (row >= rows) return;
-    float ref = -1e30f;
+    const float c_exp = in_range(scale * kLog2e);
+    float ref = kNone;
     for (int s = 0; s < splits; ++s) ref = fmaxf(ref, __ldcg(part_ml + 2 * (s * rows + row)));
     float sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -814,7 +815,7 @@ __global__ void __launch_bounds__(256) add_splits_kernel(const float* part_ml, c
     for (int s = 0; s < splits; ++s) {
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml + 2 * (s * rows + row)));
         const float4 x = __ldcg(reinterpret_cast<const float4*>(part_acc + (s * rows + row) * D + col));
-        const float f = exp2_ftz(ml.x - ref);
+        const float f = exp2_ftz((ml.x - ref) * c_exp);
         sum = fmaf(f, ml.y, sum);
         v.x = fmaf(f, x.x, v.x); v.y = fmaf(f, x.y, v.y); v.z = fmaf(f, x.z, v.z); v.w = fmaf(f, x.w, v.w);
     }

@@ -930,7 +930,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         const uint32_t tlane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);   // my lane, column 0
         const uint32_t tsc = tlane + grp * CFG::SC_COLS;                                  // my group's scores
         const uint32_t tout = tlane + NG * (CFG::SC_COLS + CFG::OPER_COLS);               // output accumulators
-        const float c_exp = p.scale * kLog2e;
+        const float c_exp = PAGED ? fminf(fmaxf(p.scale * kLog2e, 0x1p-126f), 3e38f) : p.scale * kLog2e;
         // 16 columns of a tile in one round (RW): eight packed words per operand
         constexpr int RW = 16, R = CW / RW;
         // where operand k of my columns' round r goes in tensor memory: next to the other operands, or (ALIAS)
@@ -976,8 +976,12 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
         float2 acc_a = make_float2(0.f, 0.f), acc_b = make_float2(0.f, 0.f);   // row sums alpha, ecirc
         // forward: my group's online softmax over the tiles it takes.  m_ref is the exponent reference
         // (log2 units): it follows the running maximum only when that has grown by more than 8, so
-        // that the output accumulator rarely needs rescaling; probabilities stay below 2^8.
-        float m_ref = -1e30f, l_run = 0.f;
+        // that the output accumulator rarely needs rescaling; probabilities stay below 2^8.  (PAGED: a score as it is, so that
+        // the largest one's difference from it is zero however large both are; one packed addition more per two scores.)
+        constexpr float kNoKeys = PAGED ? -3e38f : -1e30f;
+        float m_ref = kNoKeys, l_run = 0.f;
+        auto log2_apart = [&](float a, float b) { return PAGED ? (a - b) * c_exp : a - b; };     // of two references
+        (void)log2_apart;
         bool first_tile = true;                  // forward: my group has no accumulator yet
         (void)m_ref; (void)l_run; (void)first_tile;
 
@@ -1127,13 +1131,13 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                 for (int c = 0; c < CW; c += 2)
                     mr4[(c >> 1) & 3] = fmaxf(fmaxf(mr4[(c >> 1) & 3], s_[c]), s_[c + 1]);
                 const float mr = fmaxf(fmaxf(mr4[0], mr4[1]), fmaxf(mr4[2], mr4[3]));
-                const float mt = fmaxf(mr * c_exp, -1e30f);
+                const float mt = fmaxf(PAGED ? mr : mr * c_exp, kNoKeys);
                 // move the reference only when the maximum has outgrown it; the whole warp then
                 // rescales its rows of the output accumulator (factor 1 where nothing changed)
-                const bool grow = mt > m_ref + 8.f;
+                const bool grow = PAGED ? log2_apart(mt, m_ref) > 8.f : mt > m_ref + 8.f;
                 const bool rescale = __any_sync(0xffffffffu, grow) && !first_tile;
                 float factor = 1.f;
-                if (grow) { factor = fast_exp2(m_ref - mt); m_ref = mt; }
+                if (grow) { factor = fast_exp2(log2_apart(m_ref, mt)); m_ref = mt; }
                 l_run *= factor;
                 // My group's previous product must have consumed its operand and finished with the
                 // accumulator before I touch either.
@@ -1169,7 +1173,8 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
                     #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int c = 16 * h + 2 * k;
-                        const float2 x = __ffma2_rn(make_float2(s_[c], s_[c + 1]), cexp2, nm2);
+                        const float2 sc = make_float2(s_[c], s_[c + 1]);
+                        const float2 x = PAGED ? __fmul2_rn(__fadd2_rn(sc, nm2), cexp2) : __ffma2_rn(sc, cexp2, nm2);
                         const float2 pr = make_float2(fast_exp2(x.x), fast_exp2(x.y));
                         sum4[k & 3] = __fadd2_rn(sum4[k & 3], pr);
                         w0[k] = pack2<BF16>(pr.x, pr.y);
@@ -1401,7 +1406,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
             all_sync();
             const float m0 = xb[row], m1 = xb[128 + row];
             const float m = fmaxf(m0, m1);
-            const float a0 = fast_exp2(m0 - m), a1 = fast_exp2(m1 - m);
+            const float a0 = fast_exp2(log2_apart(m0, m)), a1 = fast_exp2(log2_apart(m1, m));
             const float l = a0 * xb[2 * 128 + row] + a1 * xb[3 * 128 + row];
             float inv = (l > 0.f) ? 1.f / l : 0.f;
             if constexpr (PAGED) {

@@ -56,12 +56,14 @@ def values(cache, which, seqs, b, n):
     return y * sc[..., :1] + sc[..., 1:], sc[..., :1]
 
 
-def attention(q, cache, seqs, counts=None, *, is_causal=True, scale=None, window_size=0, rotary=None):
+def attention(q, cache, seqs, counts=None, *, is_causal=True, scale=None, window_size=0, rotary=None, unpacked=False):
     """(out, bound): attention over the cache in 64 bits, and how far the kernels may be from it.
 
     Roundings to u = half a step of the type: the result, u |out|; every probability (relative to the row's sum), u sum p |v|,
     in 4 bits u(bf16) sum p 8 step on the part of the values that goes through the product; a query turned on the way,
     which moves a score by at most d = u scale |q| . |k| and the result by (e^(2 d) - 1) (sum p |v| + |out|).
+    unpacked: 4-bit rows that are rounded to 16 bits first.  An element is off by u of it at most, thus a score by u scale |q| . |k|,
+    as a turned query's, and the result by u sum p |v| more.
     Sums in fp32: scores of D products (in 4 bits with an offset of 128 or 1024 on every code) and the result's sums, 2^-23
     of the sum of magnitudes for each of the D / 16 + 1 steps; the exponential 2^-21.
     """
@@ -95,7 +97,7 @@ def attention(q, cache, seqs, counts=None, *, is_causal=True, scale=None, window
             out[b, h, :c] = p @ vh
             mag = p @ vh.abs()
             size = (x[h].abs() @ kh.abs().T * tau).masked_fill(~keep, 0).amax(-1, keepdim=True)
-            d = size * ((u if rotary is not None else 0) + 2.0 ** -23 * (D / 16 + 1))
+            d = size * ((u if rotary is not None else 0) + (u if unpacked else 0) + 2.0 ** -23 * (D / 16 + 1))
             if cache.bits == 4:
                 off = 128 if q.dtype == torch.bfloat16 else 1024
                 d = d + tau * x[h].abs().sum(-1, keepdim=True) * kstep[h // G].max() * (off + 16) * 2.0 ** -23 * (D / 16 + 1)
@@ -104,7 +106,7 @@ def attention(q, cache, seqs, counts=None, *, is_causal=True, scale=None, window
             else:
                 up = u
             d = d + 2.0 ** -21
-            bound[b, h, :c] = u * out[b, h, :c].abs() + (up + 2.0 ** -20) * mag + torch.expm1(2 * d) * (mag + out[b, h, :c].abs())
+            bound[b, h, :c] = u * out[b, h, :c].abs() + (up + (u if unpacked else 0) + 2.0 ** -20) * mag + torch.expm1(2 * d) * (mag + out[b, h, :c].abs())
     return out, bound
 
 

@@ -383,7 +383,7 @@ def test_scores_of_any_size(bits):
 
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("size", [2.0 ** 18, 2.0 ** 40, 2.0 ** 120])
-@pytest.mark.parametrize("N", [1, 3, 8])                      # 4 heads share keys: products of 8, 16 and 32 rows
+@pytest.mark.parametrize("N", [1, 3, 8, 40, 300])             # 4 heads share keys: products of 8, 16 and 32 rows, tiles of 128
 def test_scores_of_any_size_give_the_largest_all_the_weight(bits, size, N):
     """fp32 scores of up to 2^123, whose products with log2 e are not to leave the largest anything but 2^0."""
     D, n, j = 64, 3000, 1234
@@ -401,20 +401,22 @@ def test_scores_of_any_size_give_the_largest_all_the_weight(bits, size, N):
     # a code of 16 to 31, and the sums' fp32 roundings, which are smaller; then one rounding of the result.
     # 32 rows of 4 bits: the probability times the scale is one part of 8 bits, off by 2^-9 of it, and meets the code less 8
     # (16 + c - 24, from -8 to 7), with the 8 added in fp32.
+    # Tiles: the values are unpacked to 16 bits first, another 2^-9 of theirs.
     parts = 8 * 2.0 ** -9 if N == 8 else 1.01 * 31 * 2.0 ** -17
-    bound = 0 if bits == 16 else R.half_step(out.dtype) * want.abs() + (parts + 2.0 ** -18) * step[0, j]
+    more = R.half_step(out.dtype) * want.abs() if N > 16 else 0
+    bound = 0 if bits == 16 else R.half_step(out.dtype) * want.abs() + (parts + 2.0 ** -18) * step[0, j] + 1.01 * more
     assert ((out.double() - want).abs() <= bound).all()
 
 
 @pytest.mark.parametrize("bits", [16, 4])
-@pytest.mark.parametrize("N", [1, 3, 8])
+@pytest.mark.parametrize("N", [1, 3, 8, 40])
 @pytest.mark.parametrize("size,scale", [(2.0 ** -120, 1.0), (1.0, 2.0 ** -120), (2.0 ** -60, 2.0 ** -80), (2.0 ** 100, 2.0 ** -100)])
 def test_small_queries_and_scales(bits, N, size, scale):
     D = 64
     seqs = R.Sequences([700, 40], 32)
     cache = _cache(seqs, 2, D, torch.bfloat16, bits)
     q = _heads((2, 8, N, D), torch.bfloat16, 5) * size
-    want, bound = R.attention(q, cache, seqs, scale=scale)
+    want, bound = R.attention(q, cache, seqs, scale=scale, unpacked=bits == 4 and N == 40)     # (160 rows of 4 bits)
     R.close(sdpa_paged(q, cache, seqs.table, seqs.lengths, scale=scale), want, bound, TINY[torch.bfloat16])
 
 
