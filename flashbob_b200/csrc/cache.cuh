@@ -35,7 +35,9 @@ struct ReadParams {
     CacheTensor cache[2];
     uint16_t* out[2];                                            // contiguous [B, H, N, D]
     int H, N, D;
-    int unpack, window;           // out is [B * max_pages, H, page_size, D], only rows that a paged call looks at are written
+    // unpacking: out is [B * out_pages, H, 1 << out_shift, D], page i of sequence b at b * out_pages + i, and only rows that a paged
+    // call of `unpack` rows per sequence looks at are written
+    int unpack, window, out_pages, out_shift, chunks;
 };
 
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
@@ -163,19 +165,9 @@ __global__ void __launch_bounds__(kCacheThreads) append_kernel(const __grid_cons
     }
 }
 
-// One thread: 16 elements of a cached row of a head (blockIdx.y), of keys and values.  Rows behind a sequence become zero.
-template <bool BF16, int BITS>
-__global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_constant__ ReadParams p) {
-    const int per_row = p.D / 16, h = blockIdx.y;
-    const long long id = (long long)blockIdx.x * kCacheThreads + threadIdx.x, token = id / per_row;
-    if (token >= (long long)p.seq.B * p.N) return;
-    const int c = static_cast<int>(id % per_row), b = static_cast<int>(token / p.N), n = static_cast<int>(token % p.N);
-    const Sequence s = sequence_of(p.seq, b, p.unpack);
-    if (n == 0 && c == 0 && h == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
-    if (p.unpack) {
-        const int first = p.window > 0 ? s.length - (p.seq.counts ? __ldg(p.seq.counts + b) : p.unpack) - p.window + 1 : 0;
-        if (n >= s.length || n < first) return;
-    }
+// 16 elements of row n of sequence b and head h.
+template <bool BF16, int BITS, bool UNPACK>
+__device__ __forceinline__ void read_piece(const ReadParams& p, const Sequence& s, int b, int h, int n, int c) {
     int page = -1;
     if (n < s.length) {
         page = page_of(p.seq, b, n);
@@ -208,12 +200,34 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_consta
             x[w].a = narrow8<BF16>(v);
             x[w].b = narrow8<BF16>(v + 8);
         }
-        const long long at = p.unpack ? (((long long)b * p.seq.max_pages + (n >> p.seq.page_shift)) * p.H + h << p.seq.page_shift) + row
+        const long long at = UNPACK ? (((long long)b * p.out_pages + (n >> p.out_shift)) * p.H + h << p.out_shift) + (n & ((1 << p.out_shift) - 1))
                                       : ((long long)b * p.H + h) * p.N + n;
         uint4* dst = reinterpret_cast<uint4*>(p.out[w] + at * p.D) + 2 * c;
         dst[0] = x[w].a;
         dst[1] = x[w].b;
     }
+}
+
+// One thread: 16 elements of a cached row of a head (blockIdx.y), of keys and values.  Rows behind a sequence become zero.
+// Unpacking, `chunks` CTAs to a sequence take its rows in turn: a page table has room for more than a sequence holds.
+template <bool BF16, int BITS, bool UNPACK>
+__global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_constant__ ReadParams p) {
+    const int per_row = p.D / 16, h = blockIdx.y;
+    if constexpr (UNPACK) {
+        const int b = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks, c = threadIdx.x % per_row;
+        const Sequence s = sequence_of(p.seq, b, p.unpack);
+        if (blockIdx.x % p.chunks == 0 && threadIdx.x == 0 && h == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
+        const int first = p.window > 0 ? max(0, s.length - (p.seq.counts ? __ldg(p.seq.counts + b) : p.unpack) - p.window + 1) : 0;
+        for (long long n = first + (chunk * kCacheThreads + threadIdx.x) / per_row; n < s.length; n += p.chunks * (kCacheThreads / per_row))
+            read_piece<BF16, BITS, UNPACK>(p, s, b, h, static_cast<int>(n), c);
+        return;
+    }
+    const long long id = (long long)blockIdx.x * kCacheThreads + threadIdx.x, token = id / per_row;
+    if (token >= (long long)p.seq.B * p.N) return;
+    const int c = static_cast<int>(id % per_row), b = static_cast<int>(token / p.N), n = static_cast<int>(token % p.N);
+    const Sequence s = sequence_of(p.seq, b, 0);
+    if (n == 0 && c == 0 && h == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
+    read_piece<BF16, BITS, UNPACK>(p, s, b, h, n, c);
 }
 
 }  // namespace bob

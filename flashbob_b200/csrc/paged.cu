@@ -72,6 +72,7 @@ static SequenceParams sequences(const bob_sm100_cache* c, const bob_sm100_sequen
     p.lengths = s->lengths; p.counts = s->counts;
     p.B = s->B; p.max_pages = s->max_pages; p.pages = c->pages;
     while ((1 << p.page_shift) < c->page_size) ++p.page_shift;
+    p.room = s->max_pages << p.page_shift;
     p.sticky = sticky_word(c->device, true);
     return p;
 }
@@ -170,21 +171,28 @@ static int run_append(const bob_sm100_cache* c, const bob_sm100_sequences* s, co
 }
 
 // unpack > 0: for a paged call of that many rows per sequence (ReadParams::unpack).
-static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int n, void* const* out, cudaStream_t stream, int unpack = 0, int window = 0) {
+static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int n, void* const* out, cudaStream_t stream, int unpack = 0, int window = 0, int out_pages = 0, int out_shift = 0) {
     ReadParams p = {};
     p.seq = sequences(c, s);
     if (!unpack) p.seq.counts = nullptr;
     p.unpack = unpack;
     p.window = window;
+    p.out_pages = out_pages; p.out_shift = out_shift;
     for (int w = 0; w < 2; ++w) { p.cache[w] = cache_tensor(c, w); p.out[w] = static_cast<uint16_t*>(out[w]); }
     p.H = c->heads; p.N = n; p.D = c->D;
-    const int64_t threads = (int64_t)s->B * n * (c->D / 16), blocks = (threads + kCacheThreads - 1) / kCacheThreads;
+    int64_t blocks = ((int64_t)s->B * n * (c->D / 16) + kCacheThreads - 1) / kCacheThreads;
+    if (unpack) {                                        // as many CTAs as run at once, or whole sequences' worth
+        const int64_t most = ((int64_t)n * (c->D / 16) + kCacheThreads - 1) / kCacheThreads;
+        p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, kPagedSms * 2048 / kCacheThreads / ((int64_t)s->B * c->heads)));
+        blocks = (int64_t)p.chunks * s->B;
+    }
     if (blocks > 0x7fffffffLL) return kBadGeom;
     with_type(c->dtype, [&](auto bf16) {
         constexpr bool BF = decltype(bf16)::value;
         const dim3 grid((unsigned)blocks, c->heads);
-        if (c->bits == 16) read_kernel<BF, 16><<<grid, kCacheThreads, 0, stream>>>(p);
-        else read_kernel<BF, 4><<<grid, kCacheThreads, 0, stream>>>(p);
+        auto run = [&](auto kernel) { kernel<<<grid, kCacheThreads, 0, stream>>>(p); };
+        if (c->bits == 16) run(unpack ? read_kernel<BF, 16, true> : read_kernel<BF, 16, false>);
+        else run(unpack ? read_kernel<BF, 4, true> : read_kernel<BF, 4, false>);
     });
     return launched();
 }
@@ -193,8 +201,8 @@ static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int 
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // sweep: through the kernel for many rows, after a kernel that turns the queries into the workspace (and, in 4 bits, one that
-// unpacks the cache there), and with splits > 1 before one that adds the parts.
-struct PagedPlan { bool sweep; int pack, splits, rows, groups, ctas; size_t q_offset, ml_offset, acc_offset, kv_offset, kv_bytes, bytes; };
+// unpacks the cache there, or brings it into larger pages: kv_bytes > 0), and with splits > 1 before one that adds the parts.
+struct PagedPlan { bool sweep; int pack, splits, rows, groups, ctas; int out_pages, out_shift; size_t q_offset, ml_offset, acc_offset, kv_offset, kv_bytes, bytes; };
 
 // Most rows of a KV head's queries that paged_kernel takes: 32 in 16 bits (16 but for fewer than 4 heads in all), 64 in 4 bits.
 // Measured, paged_kernel / tiles of 128 rows, us: 20 rows of 8 heads in 16 bits 300 keys 20.0 / 20.8, 3000 25.2 / 22.7, of 64
@@ -202,8 +210,12 @@ struct PagedPlan { bool sweep; int pack, splits, rows, groups, ctas; size_t q_of
 // gain, us: 8 sequences x 64 heads x 20 rows, 1000 keys 107 / 143, 8192 354 / 355 (one sequence of 8 heads 39 / 35); 4 sequences x 8 heads x
 // 64 rows, 4096 keys 42 / 50; 3 sequences x 16 heads x 100 rows, 2500 keys 77 / 51, 500 45 / 29.
 constexpr int kPagedRows = 32, kPagedRows4 = 64;
-// ... in 4 bits, while the unpacked cache (as much as the page table has room for) takes no more than this.
+// ... while the unpacked cache (as much as the page table has room for) takes no more than this.
 constexpr int64_t kMostUnpacked = (int64_t)1 << 30;
+// Tiles of a KV head from which on 16-bit pages of 16 rows, whose copies of 2 KB hold a tile up, are brought into larger ones first (of up
+// to 8192 keys in pages of 16, as they are / in larger pages, us: 4 tiles 138 / 142, 8 tiles 257 / 222, 32 tiles 793 / 590; pages of 32 rows
+// 198 / 216 and 597 / 594).
+constexpr int kRepagedTiles = 8;
 constexpr int kMostSplits = 16;
 
 static int block_keys(int D, int bits) { return bits == 16 ? 2048 / D : (D == 128 ? 32 : 64); }
@@ -222,7 +234,11 @@ static bool copies_queries(const bob_sm100_paged_args* a) {
 static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
     PagedPlan d = {};
     const int64_t R = (int64_t)a->N * (a->Hq / a->cache.heads);
-    const int64_t rows = (int64_t)a->seq.B * a->Hq * a->N, unpacked = (int64_t)a->seq.B * a->seq.max_pages * a->cache.page_size * a->cache.heads * a->cache.D * 2;
+    const int64_t rows = (int64_t)a->seq.B * a->Hq * a->N;
+    // the cache unpacked, in pages of a tile's 128 rows or more
+    for (d.out_shift = 7; (1 << d.out_shift) < a->cache.page_size;) ++d.out_shift;
+    d.out_pages = (int)(((int64_t)a->seq.max_pages * a->cache.page_size + (1 << d.out_shift) - 1) >> d.out_shift);
+    const int64_t unpacked = ((int64_t)a->seq.B * d.out_pages << d.out_shift) * a->cache.heads * a->cache.D * 2;
     d.sweep = a->cache.bits == 16 ? R > kPagedRows || (R > 16 && (int64_t)a->seq.B * a->cache.heads >= 4) : R > kPagedRows4 && 2 * unpacked <= kMostUnpacked;
     if (d.sweep) {
         // with a tile for fewer than half of the SMs, the keys are divided too (whatever the lengths are)
@@ -234,7 +250,9 @@ static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
         d.ml_offset = d.q_offset + (copies_queries(a) ? up256(rows * a->cache.D * 2) : 0);
         d.acc_offset = d.ml_offset + (parted ? up256(d.splits * rows * 2 * sizeof(float)) : 0);
         d.kv_offset = d.acc_offset + (parted ? up256(d.splits * rows * a->cache.D * sizeof(float)) : 0);
-        d.kv_bytes = a->cache.bits == 4 ? up256(unpacked) : 0;
+        const int64_t tiles = ((int64_t)a->N * d.pack + 127) / 128 * (a->Hq / a->cache.heads / d.pack);       // of a KV head
+        const bool repaged = a->cache.page_size == 16 && tiles >= kRepagedTiles && 2 * unpacked <= kMostUnpacked;
+        d.kv_bytes = a->cache.bits == 4 || repaged ? up256(unpacked) : 0;
         d.bytes = d.kv_offset + 2 * d.kv_bytes;
         return d;
     }
@@ -323,14 +341,16 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
             q = r.out[0];
             strides[2] = a->cache.D; strides[1] = strides[2] * a->N * d.pack; strides[0] = strides[1] * (a->Hq / d.pack);
         }
-        if (a->cache.bits == 4) {
+        if (d.kv_bytes) {
             bob_sm100_cache& c = b.cache;
+            c.page_size = 1 << d.out_shift;
             for (int w = 0; w < 2; ++w) {
                 c.data[w] = ws + d.kv_offset + w * d.kv_bytes;
                 c.strides[w][2] = 2 * c.D; c.strides[w][1] = c.strides[w][2] * c.page_size; c.strides[w][0] = c.strides[w][1] * c.heads;
             }
-            if (int rc = run_read(&a->cache, &a->seq, a->seq.max_pages * c.page_size, c.data, stream, a->N, std::min(a->window, 1 << 28))) return rc;
+            if (int rc = run_read(&a->cache, &a->seq, seq.room, c.data, stream, a->N, std::min(a->window, 1 << 28), d.out_pages, d.out_shift)) return rc;
             c.bits = 16;
+            seq.max_pages = d.out_pages; seq.page_shift = d.out_shift;
             c.pages = seq.pages = seq.B * seq.max_pages;
             seq.table = nullptr;
         }

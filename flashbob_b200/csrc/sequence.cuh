@@ -11,7 +11,7 @@ struct SequenceParams {
     const int* table; long long table_stride;      // null: page i of sequence b is page b * max_pages + i
     const int* lengths;
     const int* counts;            // null: every row of the call
-    int B, max_pages, pages, page_shift;
+    int B, max_pages, pages, page_shift, room;       // room: rows that a sequence has pages for
     int* sticky;                  // host-visible status word (may be null)
 };
 
@@ -24,8 +24,7 @@ struct Sequence { int length, count, start; bool ok; };          // start: posit
 __device__ __forceinline__ Sequence sequence_of(const SequenceParams& p, int b, int N) {
     Sequence s;
     const int length = __ldg(p.lengths + b), count = p.counts ? __ldg(p.counts + b) : N;
-    const long long room = (long long)p.max_pages << p.page_shift;
-    s.length = static_cast<int>(min(max((long long)length, 0LL), room));
+    s.length = min(max(length, 0), p.room);
     s.count = min(max(count, 0), N);
     s.start = s.length - s.count;
     s.ok = length == s.length && count == s.count && s.start >= 0;

@@ -322,6 +322,21 @@ def test_offsets_of_more_than_32_bits(bits, pages):
         R.close(sdpa_paged(q, cache, seqs.table, seqs.lengths, counts=counts), want, bound, TINY[torch.bfloat16])
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("N,Hq,Hkv,counts,D,dtype", [(1030, 2, 2, [1030, 7, 0, 900], 64, torch.float16), (300, 8, 2, [300, 1, 0, 257], 128, torch.bfloat16), (1100, 1, 1, None, 32, torch.bfloat16)])
+@pytest.mark.parametrize("kw", [dict(), dict(window_size=100), dict(is_causal=False)])
+@pytest.mark.parametrize("room", [200, 1000])                 # pages that the table has room for: more than are in use
+def test_many_rows_over_pages_of_16(bits, N, Hq, Hkv, counts, D, dtype, kw, room):
+    lengths = [1500, 40, 0, 1203] if counts else [2000, 1100]
+    seqs = R.Sequences(lengths, 16, room=room, seed=3)
+    cache = _cache(seqs, Hkv, D, dtype, bits)
+    q = _heads((len(lengths), Hq, N, D), dtype, 5)
+    counts = None if counts is None else torch.tensor(counts, dtype=torch.int32, device="cuda")
+    out = sdpa_paged(q, cache, seqs.table, seqs.lengths, counts=counts, **kw)
+    want, bound = R.attention(q, cache, seqs, counts, unpacked=bits == 4, **kw)
+    R.close(out, want, bound, TINY[dtype])
+
+
 def test_in_inference_mode():
     with torch.inference_mode():
         seqs = R.Sequences([20], 16)
