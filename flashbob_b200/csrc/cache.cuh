@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kCacheThreads) append_kernel(const __grid_cons
         const Sequence s = sequence_of(p.seq, b, p.N);
         if (n == 0 && c == 0 && h0 == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
         position = s.start + n;
-        there = n < s.count && position >= 0;
+        there = n < s.count;
         if (there) {
             page = page_of(p.seq, b, position);
             if (page < 0) { report(p.seq.sticky, kStatusBadPage); there = false; }
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kCacheThreads) read_kernel(const __grid_consta
         const int b = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks, c = threadIdx.x % per_row;
         const Sequence s = sequence_of(p.seq, b, p.unpack);
         if (blockIdx.x % p.chunks == 0 && threadIdx.x == 0 && h == 0 && !s.ok) report(p.seq.sticky, kStatusBadLength);
-        const int first = p.window > 0 ? max(0, s.length - (p.seq.counts ? __ldg(p.seq.counts + b) : p.unpack) - p.window + 1) : 0;
+        const int first = p.window > 0 ? max(0, s.start - p.window + 1) : 0;
         for (long long n = first + (chunk * kCacheThreads + threadIdx.x) / per_row; n < s.length; n += p.chunks * (kCacheThreads / per_row))
             read_piece<BF16, BITS, UNPACK>(p, s, b, h, static_cast<int>(n), c);
         return;

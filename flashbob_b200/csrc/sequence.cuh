@@ -19,7 +19,8 @@ __device__ __forceinline__ void report(int* sticky, int code) {
     if (sticky) { *reinterpret_cast<volatile int*>(sticky) = code; __threadfence_system(); }
 }
 
-struct Sequence { int length, count, start; bool ok; };          // start: position of row 0, negative only if not ok
+// start: position of row 0.  One that is not ok is empty: what its length and count would lead to belongs to nobody's call.
+struct Sequence { int length, count, start; bool ok; };
 
 __device__ __forceinline__ Sequence sequence_of(const SequenceParams& p, int b, int N) {
     Sequence s;
@@ -28,6 +29,7 @@ __device__ __forceinline__ Sequence sequence_of(const SequenceParams& p, int b, 
     s.count = min(max(count, 0), N);
     s.start = s.length - s.count;
     s.ok = length == s.length && count == s.count && s.start >= 0;
+    if (!s.ok) s.length = s.count = s.start = 0;
     return s;
 }
 

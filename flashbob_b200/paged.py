@@ -20,8 +20,8 @@ which `sdpa_bob` takes.
 
 What only the GPU knows is checked there.  A page table entry within a sequence's length that is no page of the cache, a
 length that the table has no room for, or a count that exceeds the length or the call's rows raises `BobSm100Error`
-at the next call on that device (`BOB_SM100_CHECK_STATUS=1`: at the call itself); what it concerns is neither read nor
-written.  On the CPU the call raises `ValueError`.  Entries outside the reach of a sequence's rows - behind its length, before
+at the next call on that device (`BOB_SM100_CHECK_STATUS=1`: at the call itself); what it concerns - of a page its rows, of
+a length or count the whole sequence, whose results are zero - is neither read nor written.  On the CPU the call raises `ValueError`.  Entries outside the reach of a sequence's rows - behind its length, before
 its window - are never looked at.
 """
 

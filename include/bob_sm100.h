@@ -160,8 +160,8 @@ int bob_sm100_noalloc_read_status(int device, void* stream);
  * Tensors of tokens are [B, H, N, D] as above (element strides of batch, head and row; unit stride along D; multiples of
  * 8; 16-byte aligned), with D = 32, 64 or 128.  These entry points allocate nothing, wait for nothing and can be
  * captured.  What only the GPU knows (page table, lengths, counts) is checked there: an entry outside the cache or a
- * length or count out of range sets the device's status word (bob_sm100_last_status), and the rows that it
- * concerns are neither read nor written. */
+ * length or count out of range sets the device's status word (bob_sm100_last_status), and the page's rows, or the whole
+ * sequence's (whose results are zero), are neither read nor written. */
 
 /* Rotary positions: pair i turns elements (i, i + pairs), interleaved (2 i, 2 i + 1), by position * turns[i] / 2^64
  * turns, and is multiplied by factor; elements from 2 * pairs on are left alone.  pairs = 0: no rotation. */
