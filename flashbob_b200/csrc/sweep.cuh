@@ -1411,6 +1411,7 @@ sweep_kernel(const __grid_constant__ SweepParams p) {
             const float l = a0 * xb[2 * 128 + row] + a1 * xb[3 * 128 + row];
             float inv = (l > 0.f) ? 1.f / l : 0.f;
             if constexpr (PAGED) {
+                inv = l == 0.f ? 0.f : 1.f / l;          // (a row without keys is zero; a NaN score makes the sum NaN, and it stays)
                 if (parted) {
                     inv = 1.f;
                     if (grp == 0 && own_idx < n_own) *reinterpret_cast<float2*>(p.part_ml + 2 * (w.split * part_rows + row_stat)) = make_float2(m, l);
