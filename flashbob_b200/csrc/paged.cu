@@ -217,6 +217,8 @@ constexpr int64_t kMostUnpacked = (int64_t)1 << 30;
 // 198 / 216 and 597 / 594).
 constexpr int kRepagedTiles = 8;
 constexpr int kMostSplits = 16;
+// Query heads that may share a KV head (PagedParams::g_part).
+constexpr int kMostGroup = 32;
 
 static int block_keys(int D, int bits) { return bits == 16 ? 2048 / D : (D == 128 ? 32 : 64); }
 
@@ -274,6 +276,7 @@ static int check_paged(const bob_sm100_paged_args* a) {
     if (int rc = check_sequences(&a->cache, &a->seq)) return rc;
     if (int rc = check_rotary(a->rotary, a->cache.D)) return rc;
     if (a->Hq <= 0 || a->Hq % a->cache.heads || a->N <= 0 || a->N > (1 << 28)) return kBadGeom;
+    if (a->Hq / a->cache.heads > kMostGroup) return kBadGeom;
     if (a->window < 0 || (a->window > 0 && !a->is_causal)) return kBadGeom;
     if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return kBadGeom;
     if (int rc = check_tokens(a->q, a->q_strides)) return rc;

@@ -34,7 +34,7 @@ struct alignas(16) PagedParams {
     const uint16_t* q; long long q_sb, q_sh, q_sn;
     uint16_t* out;                // contiguous [B, Hq, N, D]
     int Hq, Hkv, G, N, form;
-    int g_part;                   // 65536 / G + 1: x / G = x * g_part / 65536 for x < 2048
+    int g_part;                   // 65536 / G + 1: x / G = x * g_part / 65536 for the x of an item's rows, below 64, and G up to 32
     int groups;                   // row groups of ROWS query rows per KV head
     int causal, window;
     int alike;                    // keys and values (and their scales) have the same strides

@@ -214,6 +214,7 @@ typedef struct bob_sm100_sequences {
 } bob_sm100_sequences;
 
 /* Attention over a cache: query i of sequence b sits at lengths[b] - counts[b] + i and is turned to that position first.
+ * Hq is a multiple of the cache's heads, up to 32 times.
  * out is contiguous [B, Hq, N, D]; rows from counts[b] on, and rows without keys, are zero.  workspace_bytes is known
  * from these arguments alone (not from lengths). */
 typedef struct bob_sm100_paged_args {
