@@ -114,6 +114,10 @@ __device__ __forceinline__ float exp2_ftz(float x) {
 // A factor that neither infinities nor zeros are lost on.
 __device__ __forceinline__ float in_range(float x) { return fminf(fmaxf(x, 0x1p-126f), 3e38f); }
 
+// x 2^n for |n| up to 252, in two steps: 2^n alone may be no fp32 number.
+__device__ __forceinline__ float power_of_two(int n) { return __uint_as_float(static_cast<uint32_t>(127 + n) << 23); }
+__device__ __forceinline__ float times_power(float x, int n) { return x * power_of_two(n / 2) * power_of_two(n - n / 2); }
+
 // A product with a value's first part, and with the rest of it.  An infinite element makes the second one infinite of
 // either sign or NaN, and decides the first alone.
 // (Codes are finite.)
@@ -416,7 +420,8 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
             }
         }
         __syncthreads();
-        float q_sum[LR], unit[LR];                       // 4 bits: sum of a row's elements, what its scores are multiples of
+        float q_sum[LR];                                 // 4 bits: sum of a row's elements;
+        int unit[LR];                                    // its scores are multiples of 2^unit
         (void)q_sum; (void)unit;
         // row of mine (LR of them) that half hr of product mt has, or a part of
         auto my_row = [](int mt, int hr) { return ROWS == 8 ? 0 : ROWS == 16 ? hr : 2 * mt + hr; };
@@ -451,10 +456,9 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         }
                         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
                         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                        // (neither power leaves fp32's range: scores of queries above 2^117 become 2^10 times smaller at most)
                         const int exponent = min(max(static_cast<int>(__float_as_uint(largest) >> 23), 127 - 100), 254);
                         up[k] = __uint_as_float(static_cast<uint32_t>(2 * 127 + 14 - exponent) << 23);
-                        unit[k] = __uint_as_float(static_cast<uint32_t>(min(exponent - 14 + 24, 254)) << 23);
+                        unit[k] = exponent - 127 - 14 + 24;
                         q_sum[k] = 0.f;
                     }
                     float sum = 0.f;
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
         // zero however large both are
         float c[LR];
         #pragma unroll
-        for (int k = 0; k < LR; ++k) c[k] = BITS == 4 ? in_range(c_exp * unit[k]) : c_exp;
+        for (int k = 0; k < LR; ++k) c[k] = BITS == 4 ? in_range(times_power(c_exp, unit[k])) : c_exp;
         float acc[MT][D / 8][4], m[LR], l[LR], z[LR];    // z: 4 bits, what every column gains
         #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -745,7 +749,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     zs += __shfl_xor_sync(0xffffffffu, zs, 1);
                     z[k] = zs + __shfl_xor_sync(0xffffffffu, zs, 2);
                 }
-                if (t == 0) { sm_m[warp * EXR + j * 8 + g] = BITS == 4 && m[k] > kNone ? m[k] * unit[k] : m[k]; sm_l[warp * EXR + j * 8 + g] = sum; }
+                if (t == 0) { sm_m[warp * EXR + j * 8 + g] = BITS == 4 && m[k] > kNone ? times_power(m[k], unit[k]) : m[k]; sm_l[warp * EXR + j * 8 + g] = sum; }
             }
             if (lane == 0) sm_slot[warp] = (warp * NST + fill) * STAGE;
             #pragma unroll
