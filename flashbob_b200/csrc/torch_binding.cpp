@@ -262,11 +262,12 @@ Tensor sdpa(const Tensor& q, const Tensor& k, const Tensor& v, const Mask& m) {
 
 // ---- rotary positions -------------------------------------------------------------------------------
 // The kernels for positions and the paged cache read any layout with unit stride along the head dim, strides that are
-// multiples of 8 elements (zero for an expanded tensor) and a 16-byte aligned base.
+// multiples of 8 elements (zero for an expanded tensor) and a 16-byte aligned base.  Anything else is copied: contiguous()
+// would give back a tensor that is contiguous but starts elsewhere, or has an odd stride along a dimension of one entry.
 Tensor tokens_ready(const Tensor& t) {
     bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
     for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) % 8 == 0 && t.stride(i) >= 0;
-    return ok ? t : t.contiguous();
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 int32_t dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? BOB_SM100_BF16 : BOB_SM100_FP16; }
