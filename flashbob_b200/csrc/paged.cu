@@ -66,7 +66,7 @@ static int check_sequences(const bob_sm100_cache* c, const bob_sm100_sequences* 
     return 0;
 }
 
-static SequenceParams sequences(const bob_sm100_cache* c, const bob_sm100_sequences* s) {
+static SequenceParams sequences(const bob_sm100_cache* c, const bob_sm100_sequences* s, bool apart = false) {
     SequenceParams p = {};
     p.table = s->table; p.table_stride = s->table_stride;
     p.lengths = s->lengths; p.counts = s->counts;
@@ -74,6 +74,7 @@ static SequenceParams sequences(const bob_sm100_cache* c, const bob_sm100_sequen
     while ((1 << p.page_shift) < c->page_size) ++p.page_shift;
     p.room = s->max_pages << p.page_shift;
     p.sticky = sticky_word(c->device, true);
+    p.apart = apart;
     return p;
 }
 
@@ -171,9 +172,9 @@ static int run_append(const bob_sm100_cache* c, const bob_sm100_sequences* s, co
 }
 
 // unpack > 0: for a paged call of that many rows per sequence (ReadParams::unpack).
-static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int n, void* const* out, cudaStream_t stream, int unpack = 0, int window = 0, int out_pages = 0, int out_shift = 0) {
+static int run_read(const bob_sm100_cache* c, const bob_sm100_sequences* s, int n, void* const* out, cudaStream_t stream, bool apart = false, int unpack = 0, int window = 0, int out_pages = 0, int out_shift = 0) {
     ReadParams p = {};
-    p.seq = sequences(c, s);
+    p.seq = sequences(c, s, apart);
     if (!unpack) p.seq.counts = nullptr;
     p.unpack = unpack;
     p.window = window;
@@ -329,7 +330,7 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
     if (d.sweep) {
         char* ws = static_cast<char*>(workspace);
         bob_sm100_paged_args b = *a;
-        SequenceParams seq = sequences(&a->cache, &a->seq);
+        SequenceParams seq = sequences(&a->cache, &a->seq, !a->is_causal);
         const void* q = a->q;
         int64_t strides[3] = {a->q_strides[0], a->q_strides[1], a->q_strides[2]};
         if (copies_queries(a)) {
@@ -351,7 +352,7 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
                 c.data[w] = ws + d.kv_offset + w * d.kv_bytes;
                 c.strides[w][2] = 2 * c.D; c.strides[w][1] = c.strides[w][2] * c.page_size; c.strides[w][0] = c.strides[w][1] * c.heads;
             }
-            if (int rc = run_read(&a->cache, &a->seq, seq.room, c.data, stream, a->N, std::min(a->window, 1 << 28), d.out_pages, d.out_shift)) return rc;
+            if (int rc = run_read(&a->cache, &a->seq, seq.room, c.data, stream, !a->is_causal, a->N, std::min(a->window, 1 << 28), d.out_pages, d.out_shift)) return rc;
             c.bits = 16;
             seq.max_pages = d.out_pages; seq.page_shift = d.out_shift;
             c.pages = seq.pages = seq.B * seq.max_pages;
@@ -369,7 +370,7 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
     }
     PagedParams p = {};
     p.rotary = a->rotary;
-    p.seq = sequences(&a->cache, &a->seq);
+    p.seq = sequences(&a->cache, &a->seq, !a->is_causal);
     for (int w = 0; w < 2; ++w) p.cache[w] = cache_tensor(&a->cache, w);
     p.q = static_cast<const uint16_t*>(a->q); p.q_sb = a->q_strides[0]; p.q_sh = a->q_strides[1]; p.q_sn = a->q_strides[2];
     p.out = static_cast<uint16_t*>(a->out);

@@ -19,10 +19,11 @@ tensor operations.  Nothing here records gradients: `read_kv` brings a cached co
 which `sdpa_bob` takes.
 
 What only the GPU knows is checked there.  A page table entry within a sequence's length that is no page of the cache, a
-length that the table has no room for, or a count that exceeds the length or the call's rows raises `BobSm100Error`
-at the next call on that device (`BOB_SM100_CHECK_STATUS=1`: at the call itself); what it concerns - of a page its rows, of
-a length or count the whole sequence, whose results are zero - is neither read nor written.  On the CPU the call raises `ValueError`.  Entries outside the reach of a sequence's rows - behind its length, before
-its window - are never looked at.
+length that the table has no room for, or a count that exceeds the call's rows or (but for attention without `is_causal`)
+the length raises `BobSm100Error` at the next call on that device (`BOB_SM100_CHECK_STATUS=1`: at the call itself); what it
+concerns - of a page its rows, of a length or count the whole sequence, whose results are zero - is neither read nor written.
+On the CPU the call raises `ValueError`.  Entries outside the reach of a sequence's rows - behind its length, before its
+window - are never looked at.
 """
 
 from __future__ import annotations
@@ -205,12 +206,12 @@ def _cpu_rows(cache: PagedCache, which: str, pages, places):
     return torch.stack((x & 15, x >> 4), -1).flatten(-2).float() * scales[..., :1] + scales[..., 1:]
 
 
-def _cpu_sequences(cache: PagedCache, page_table, lengths, counts, n_rows: int):
-    """(sequence, length, count) one by one, checked."""
+def _cpu_sequences(cache: PagedCache, page_table, lengths, counts, n_rows: int, apart: bool = False):
+    """(sequence, length, count) one by one, checked.  apart: the rows have no positions in the sequence, and may be more."""
     room = page_table.shape[1] * cache.page_size
     for b, length in enumerate(lengths.tolist()):
         count = n_rows if counts is None else int(counts[b])
-        if not 0 <= length <= room or not 0 <= count <= min(n_rows, length):
+        if not 0 <= length <= room or not 0 <= count <= (n_rows if apart else min(n_rows, length)):
             raise ValueError(f"sequence {b}: length {length} (room for {room}) or count {count} (of {n_rows} rows) out of range")
         yield b, length, count
 
@@ -296,8 +297,8 @@ def sdpa_paged(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, len
 
     Query i < counts[b] of sequence b sits at position lengths[b] - counts[b] + i, to which `rotary` turns it.  `is_causal`
     keeps keys at positions up to the query's, `window_size` w > 0 further keeps only the last w of them; without
-    `is_causal` every query sees all lengths[b] keys, as in cross attention to cached encoder states (and `rotary` is
-    refused: such queries have no position among the keys).  Rows from counts[b] on, and rows without keys, are zero.
+    `is_causal` every query sees all lengths[b] keys, as in cross attention to cached encoder states (such queries have no
+    position among the keys: there may be more of them, and `rotary` is refused).  Rows from counts[b] on, and rows without keys, are zero.
     Key and value rows that no query of its sequence attends to have no part in the result, whatever they hold; a NaN or infinity
     among the values that some queries of a sequence attend to may reach its other queries of the same call, as in any
     product of probabilities and values.  H_Q is a multiple of H_KV, up to 32 times.
@@ -329,7 +330,7 @@ def sdpa_paged(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, len
     group, n_rows = q.shape[1] // cache.kv_heads, q.shape[2]
     tau = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)
     with torch.no_grad():
-        for b, length, count in _cpu_sequences(cache, *sequences, n_rows):
+        for b, length, count in _cpu_sequences(cache, *sequences, n_rows, not is_causal):
             first = max(0, length - count - window + 1) if window else 0
             if not count or first >= length:
                 continue

@@ -204,7 +204,8 @@ typedef struct bob_sm100_cache {
 } bob_sm100_cache;
 
 /* B sequences: position t of sequence b is row t % page_size of page table[b * table_stride + t / page_size];
- * lengths[b] positions are there with the new ones, the last counts[b] (NULL: all N rows of the call) are new. */
+ * lengths[b] positions are there with the new ones, the last counts[b] (NULL: all N rows of the call) are new.  (Attention
+ * without is_causal: counts[b] queries that have no positions, and may be more than lengths[b].) */
 typedef struct bob_sm100_sequences {
     int32_t B, max_pages;
     const int32_t* table;
