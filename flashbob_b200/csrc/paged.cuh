@@ -47,6 +47,7 @@ struct alignas(16) PagedParams {
 constexpr float kLog2e = 1.4426950408889634f, kNone = -3e38f;         // (kNone: the reference of a row without keys)
 constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedMinBlocks = 4;          // blocks that are worth a CTA of their own
+constexpr int kLevel = 8;                   // a warp's blocks between two takings of 4-bit values' offset from its sums (16 or 32 products' steps)
 
 template <int D_, int ROWS_, int BITS_>
 struct PagedConfig {
@@ -504,14 +505,39 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
         float c[LR];
         #pragma unroll
         for (int k = 0; k < LR; ++k) c[k] = BITS == 4 ? in_range(times_power(c_exp, unit[k])) : c_exp;
-        float acc[MT][D / 8][4], m[LR], l[LR], z[LR];    // z: 4 bits, what every column gains
+        // 4 bits: z: what every column gains; w_sum: the weights that the accumulators' codes have met since the last level()
+        float acc[MT][D / 8][4], m[LR], l[LR], z[LR], w_sum[LR];
         #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             #pragma unroll
             for (int i = 0; i < D / 8; ++i) acc[mt][i][0] = acc[mt][i][1] = acc[mt][i][2] = acc[mt][i][3] = 0.f;
         }
         #pragma unroll
-        for (int k = 0; k < LR; ++k) { m[k] = kNone; l[k] = z[k] = 0.f; }
+        for (int k = 0; k < LR; ++k) { m[k] = kNone; l[k] = z[k] = w_sum[k] = 0.f; }
+        // 4 bits: a code goes through the products as 16 + c, so that an accumulator grows by some 24 times the weights while its
+        // result, of values about zero, does not, and the products' sums, which are cut off and not rounded, drift with
+        // every step.  So 23.5 times the weights are taken off every kLevel blocks and at a segment's end, and what is left are
+        // sums of weight times c - 7.5.  (131,072 fp16 keys of like weight in one CTA: off by 4.9e-2 of the result without it,
+        // 2.3e-4 with it.  8 rows take as long as without; 16 and 32 rows of 128 elements 4 to 7 % more, for registers.)
+        auto level = [&]() {
+            #pragma unroll
+            for (int k = 0; k < LR; ++k) {
+                if constexpr (PARTS) z[k] = fmaf(7.5f, w_sum[k], z[k]);
+                float all = w_sum[k];
+                all += __shfl_xor_sync(0xffffffffu, all, 1);
+                all += __shfl_xor_sync(0xffffffffu, all, 2);
+                w_sum[k] = 0.f;
+                #pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    #pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& a = acc[PARTS ? 0 : k / 2][i][ROWS == 8 ? e : 2 * (k % 2) + e];
+                        a = fmaf(-23.5f, all, a);
+                    }
+                }
+            }
+        };
+        (void)level;
 
         #pragma unroll 1
         for (int blk = seg.blk + warp; blk < seg.last; blk += kPagedWarps) {
@@ -631,7 +657,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                     f[k] = exp2_ftz((m[k] - ref) * c[k]);
                     m[k] = ref;
                     l[k] *= f[k];
-                    if constexpr (BITS == 4) z[k] *= f[k];
+                    if constexpr (BITS == 4) { z[k] *= f[k]; w_sum[k] *= f[k]; }
                 }
                 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
@@ -655,20 +681,21 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         pr[e] = exp2_ftz((x[k][i][e] - m[k]) * c[k]);
                         l[k] += pr[e];
                         if constexpr (BITS == 4) {
-                            // value = scale b + (zero - 16 scale): the first part goes through the product, with the scale
-                            // in the probability, the second is the same for every column.  In bf16 for both
-                            // types: a scale may lie outside fp16.
-                            // (one part: about the middle, so that its rounding, 2^-9, meets b - 24 and not b)
-                            const float scale = __uint_as_float(raw[2 * e]);
-                            z[k] = fmaf(pr[e], fmaf(PARTS ? -16.f : 8.f, scale, __uint_as_float(raw[2 * e + 1])), z[k]);
+                            // value = scale (b - 23.5) + (zero + 7.5 scale), b = 16 + c: scale b goes through the product, with the scale
+                            // in the probability, the last part is the same for every column (with two parts its 7.5 scale is
+                            // added in level()).  In bf16 for both types: a scale may lie outside fp16.
+                            // (one part: the weights taken off are the rounded ones, so that the rounding, 2^-9, meets b - 23.5 and not b)
+                            const float scale = __uint_as_float(raw[2 * e]), zero = __uint_as_float(raw[2 * e + 1]);
+                            z[k] = fmaf(pr[e], PARTS ? zero : fmaf(7.5f, scale, zero), z[k]);
                             pr[e] *= scale;
+                            if constexpr (PARTS) w_sum[k] += pr[e];
                         }
                     }
                     const uint32_t first = pack2<PB>(pr[0], pr[1]);
                     float back[2];
                     if constexpr (PB) { back[0] = __uint_as_float(first << 16); back[1] = __uint_as_float(first & 0xffff0000u); }
                     else { const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&first)); back[0] = f2.x; back[1] = f2.y; }
-                    if constexpr (BITS == 4 && !PARTS) z[k] = fmaf(-24.f, back[0] + back[1], z[k]);
+                    if constexpr (BITS == 4 && !PARTS) w_sum[k] += back[0] + back[1];
                     if constexpr (PARTS) {
                         const uint32_t rest = pack2<PB>(pr[0] - back[0], pr[1] - back[1]);
                         if constexpr (ROWS == 8) { pa[0][i / 2][2 * (i % 2)] = first; pa[0][i / 2][2 * (i % 2) + 1] = rest; }
@@ -726,6 +753,7 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                 }
             }
             }   // sub
+            if (BITS == 4 && ((blk / kPagedWarps) % kLevel == kLevel - 1 || blk + kPagedWarps >= seg.last)) level();
         }
 
         // ---- the four warps' parts, through their free ring slots, EXR rows at a time ----------------------
