@@ -74,7 +74,7 @@ static SequenceParams sequences(const bob_sm100_cache* c, const bob_sm100_sequen
     while ((1 << p.page_shift) < c->page_size) ++p.page_shift;
     p.room = s->max_pages << p.page_shift;
     p.sticky = sticky_word(c->device, true);
-    p.apart = apart;
+    p.first = apart ? -(1 << 29) : 0;
     return p;
 }
 

@@ -13,25 +13,26 @@ struct SequenceParams {
     const int* counts;            // null: every row of the call
     int B, max_pages, pages, page_shift, room;       // room: rows that a sequence has pages for
     int* sticky;                  // host-visible status word (may be null)
-    bool apart;                   // the call's rows have no positions in the sequence (attention without a causal mask): there may be
-                                  // more of them than the sequence has
+    int first;                    // least position of row 0: 0, or any negative number where the call's rows have no positions in the
+                                  // sequence (attention without a causal mask) and may be more than it has
 };
 
 __device__ __forceinline__ void report(int* sticky, int code) {
     if (sticky) { *reinterpret_cast<volatile int*>(sticky) = code; __threadfence_system(); }
 }
 
-// start: position of row 0 (negative only where rows are apart).  One that is not ok is empty: what its length and count would lead to belongs to nobody's call.
+// start: position of row 0 (negative only where rows have none).  One that is not ok is empty: what its length and count would
+// lead to belongs to nobody's call.
 struct Sequence { int length, count, start; bool ok; };
 
 __device__ __forceinline__ Sequence sequence_of(const SequenceParams& p, int b, int N) {
     Sequence s;
     const int length = __ldg(p.lengths + b), count = p.counts ? __ldg(p.counts + b) : N;
-    s.length = min(max(length, 0), p.room);
-    s.count = min(max(count, 0), N);
+    s.ok = static_cast<unsigned>(length) <= static_cast<unsigned>(p.room) && static_cast<unsigned>(count) <= static_cast<unsigned>(N) &&
+           length - count >= p.first;                        // (neither is above 2^28 here)
+    s.length = s.ok ? length : 0;
+    s.count = s.ok ? count : 0;
     s.start = s.length - s.count;
-    s.ok = length == s.length && count == s.count && (s.start >= 0 || p.apart);
-    if (!s.ok) s.length = s.count = s.start = 0;
     return s;
 }
 
