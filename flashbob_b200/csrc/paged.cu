@@ -208,8 +208,9 @@ struct PagedPlan { bool sweep; int pack, splits, rows, groups, ctas; int out_pag
 // Most rows of a KV head's queries that paged_kernel takes: 32 in 16 bits (16 but for fewer than 4 heads in all), 64 in 4 bits.
 // Measured, paged_kernel / tiles of 128 rows, us: 20 rows of 8 heads in 16 bits 300 keys 20.0 / 20.8, 3000 25.2 / 22.7, of 64
 // heads 25.1 / 20.5 and 49.8 / 37.4; 32 rows of one head 14.2 / 20.9 and 15.9 / 21.0.  In 4 bits unpacking costs what tiles
-// gain, us: 8 sequences x 64 heads x 20 rows, 1000 keys 107 / 143, 8192 354 / 355 (one sequence of 8 heads 39 / 35); 4 sequences x 8 heads x
-// 64 rows, 4096 keys 42 / 50; 3 sequences x 16 heads x 100 rows, 2500 keys 77 / 51, 500 45 / 29.
+// gain, us: 8 sequences x 64 heads x 20 rows, 1000 keys 121 / 147 (fp16, in which rows are taken 16 at a time, 128 / 147), one sequence of
+// 8 heads, 8192 keys 43 / 35 (30 / 35); 4 sequences x 8 heads x 64 rows, 4096 keys 45 / 50 (56 / 49); 3 sequences x 16 heads x 100
+// rows, 2500 keys 87 / 50 (83 / 51), 500 49 / 28.
 constexpr int kPagedRows = 32, kPagedRows4 = 64;
 // ... while the unpacked cache (as much as the page table has room for) takes no more than this.
 constexpr int64_t kMostUnpacked = (int64_t)1 << 30;
@@ -259,7 +260,12 @@ static PagedPlan paged_plan(const bob_sm100_paged_args* a) {
         d.bytes = d.kv_offset + 2 * d.kv_bytes;
         return d;
     }
-    d.rows = R <= 8 ? 8 : (R <= 16 ? 16 : 32);
+    // fp16 over 4 bits: 16 at a time, since one part of a probability times its scale is a bf16 number, which has 3 bits fewer
+    // than the rest of the call (error against 64 bits 1.8e-3 with 32 rows at a time, 2.1e-4 with 16; us, 32 / 16 at a time: 8 sequences x
+    // 64 heads x 20 rows of 64 elements, 1000 keys 56 / 75, 8192 keys 217 / 338; 4 x 8 heads x 64 rows, 4096 keys 26 / 33; 8 x 8 heads x 20
+    // rows of 128 elements, 3000 keys 55 / 48)
+    const bool by16 = a->cache.bits == 4 && a->cache.dtype == BOB_SM100_FP16;
+    d.rows = R <= 8 ? 8 : (R <= 16 || by16 ? 16 : 32);
     d.groups = (int)((R + d.rows - 1) / d.rows);
     // no more CTAs than the longest possible sequences have work for
     const int64_t kb = block_keys(a->cache.D, a->cache.bits), most = ((int64_t)a->seq.max_pages * a->cache.page_size + kb - 1) / kb;
@@ -391,7 +397,8 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
         constexpr bool BF = decltype(bf16)::value;
         auto dim = [&](auto rows, auto bits) {
             constexpr int ROWS = decltype(rows)::value, BITS = decltype(bits)::value;
-            if (a->cache.D == 32) rc = launch_paged<32, ROWS, BF, BITS>(p, a->cache.device, stream);
+            if constexpr (ROWS == 32 && BITS == 4 && !BF) return;        // (paged_plan)
+            else if (a->cache.D == 32) rc = launch_paged<32, ROWS, BF, BITS>(p, a->cache.device, stream);
             else if (a->cache.D == 64) rc = launch_paged<64, ROWS, BF, BITS>(p, a->cache.device, stream);
             else rc = launch_paged<128, ROWS, BF, BITS>(p, a->cache.device, stream);
         };

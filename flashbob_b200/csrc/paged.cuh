@@ -4,7 +4,7 @@
 // share every row that is read, and the products run on mma.sync (m16n8k16): a step of generation needs a few rows of
 // a product, where tcgen05's 128 would be padding, and its operands come straight from the registers that decode 4 bits.
 //
-// Up to 16 rows, queries and probabilities go through the products in two 16-bit parts each (the value rounded, and what
+// Up to 16 rows at a time, queries and probabilities go through the products in two 16-bit parts each (the value rounded, and what
 // the rounding left), so that only the result is rounded to 16 bits.  With up to 8 rows the second parts are rows 8 ... 15 of
 // the same product, which would be padding, and cost nothing; with up to 16 they are a second product.
 //

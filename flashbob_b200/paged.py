@@ -303,8 +303,8 @@ def sdpa_paged(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, len
     among the values that some queries of a sequence attend to may reach its other queries of the same call, as in any
     product of probabilities and values.  H_Q is a multiple of H_KV, up to 32 times.
 
-    Up to 16 rows (tokens of the call x H_Q / H_KV) only the result is rounded to 16 bits; beyond, turned queries and
-    probabilities are too, as in `apply_rotary` followed by `sdpa_bob`.
+    Up to 16 rows (tokens of the call x H_Q / H_KV), in fp16 over 4 bits up to 64, only the result is rounded to 16 bits; beyond,
+    turned queries, probabilities and rows of 4 bits are too, as in `apply_rotary` and `read_kv` followed by `sdpa_bob`.
     """
     turn_args = _plain_rotary(rotary)
     if _native_call(cache, turn_args):
