@@ -47,7 +47,7 @@ struct alignas(16) PagedParams {
 constexpr float kLog2e = 1.4426950408889634f, kNone = -3e38f;         // (kNone: the reference of a row without keys)
 constexpr int kPagedWarps = 4, kPagedThreads = 32 * kPagedWarps;
 constexpr int kPagedMinBlocks = 4;          // blocks that are worth a CTA of their own
-constexpr int kLevel = 8;                   // a warp's blocks between two takings of 4-bit values' offset from its sums (16 or 32 products' steps)
+constexpr int kLevel = 8;                   // a warp's blocks between two levellings of 4-bit values' sums (16 or 32 products' steps)
 
 template <int D_, int ROWS_, int BITS_>
 struct PagedConfig {
@@ -516,25 +516,29 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
         for (int k = 0; k < LR; ++k) { m[k] = kNone; l[k] = z[k] = w_sum[k] = 0.f; }
         // 4 bits: a code goes through the products as 16 + c, so that an accumulator grows by some 24 times the weights while its
         // result, of values about zero, does not, and the products' sums, which are cut off and not rounded, drift with
-        // every step.  So 23.5 times the weights are taken off every kLevel blocks and at a segment's end, and what is left are
-        // sums of weight times c - 7.5.  (131,072 fp16 keys of like weight in one CTA: off by 4.9e-2 of the result without it,
-        // 2.3e-4 with it.  8 rows take as long as without; 16 and 32 rows of 128 elements 4 to 7 % more, for registers.)
+        // every step.  So every kLevel blocks, and at a segment's end, what a row's columns have in common, their mean, moves to z
+        // together with the offset's share, which it all but cancels: what is left are the columns' differences.
+        // (131,072 fp16 keys of like weight in one CTA: off by 4.9e-2 of the result without it, 2.0e-4 with it, one rounding.  8 rows
+        // take 1 to 3 % more, 16 and 32 rows of 128 elements 5 to 9 %, for registers.)
         auto level = [&]() {
             #pragma unroll
             for (int k = 0; k < LR; ++k) {
-                if constexpr (PARTS) z[k] = fmaf(7.5f, w_sum[k], z[k]);
-                float all = w_sum[k];
-                all += __shfl_xor_sync(0xffffffffu, all, 1);
-                all += __shfl_xor_sync(0xffffffffu, all, 2);
-                w_sum[k] = 0.f;
+                auto column_sum = [&](int i, int e) -> float& { return acc[PARTS ? 0 : k / 2][i][ROWS == 8 ? e : 2 * (k % 2) + e]; };
+                float mean = 0.f, weights = w_sum[k];
+                #pragma unroll
+                for (int i = 0; i < D / 8; ++i) mean += column_sum(i, 0) + column_sum(i, 1);
+                mean += __shfl_xor_sync(0xffffffffu, mean, 1);
+                weights += __shfl_xor_sync(0xffffffffu, weights, 1);
+                mean += __shfl_xor_sync(0xffffffffu, mean, 2);
+                weights += __shfl_xor_sync(0xffffffffu, weights, 2);
+                mean *= 1.f / D;
                 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
-                    #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& a = acc[PARTS ? 0 : k / 2][i][ROWS == 8 ? e : 2 * (k % 2) + e];
-                        a = fmaf(-23.5f, all, a);
-                    }
+                    column_sum(i, 0) -= mean;
+                    column_sum(i, 1) -= mean;
                 }
+                z[k] = fmaf(0.25f, fmaf(PARTS ? -16.f : -24.f, weights, mean), z[k]);        // (a row's z is the sum of its four threads')
+                w_sum[k] = 0.f;
             }
         };
         (void)level;
@@ -681,12 +685,13 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                         pr[e] = exp2_ftz((x[k][i][e] - m[k]) * c[k]);
                         l[k] += pr[e];
                         if constexpr (BITS == 4) {
-                            // value = scale (b - 23.5) + (zero + 7.5 scale), b = 16 + c: scale b goes through the product, with the scale
-                            // in the probability, the last part is the same for every column (with two parts its 7.5 scale is
-                            // added in level()).  In bf16 for both types: a scale may lie outside fp16.
-                            // (one part: the weights taken off are the rounded ones, so that the rounding, 2^-9, meets b - 23.5 and not b)
+                            // value = scale b + zero - 16 scale, b = 16 + c: scale b goes through the product, with the scale in
+                            // the probability, the rest is the same for every column: the zero goes to z, -16 scale by level().
+                            // In bf16 for both types: a scale may lie outside fp16.
+                            // (one part: value = scale (b - 24) + zero + 8 scale, where the 24 goes with the rounded weights, so
+                            // that their rounding, 2^-9, meets b - 24 and not b)
                             const float scale = __uint_as_float(raw[2 * e]), zero = __uint_as_float(raw[2 * e + 1]);
-                            z[k] = fmaf(pr[e], PARTS ? zero : fmaf(7.5f, scale, zero), z[k]);
+                            z[k] = fmaf(pr[e], PARTS ? zero : fmaf(8.f, scale, zero), z[k]);
                             pr[e] *= scale;
                             if constexpr (PARTS) w_sum[k] += pr[e];
                         }

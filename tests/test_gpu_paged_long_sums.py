@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import paged_reference as R
-from flashbob_b200.paged import sdpa_paged
+from flashbob_b200.paged import PagedCache, _quantise, sdpa_paged
 from test_gpu_paged import TINY, _cache, _heads
 
 pytestmark = pytest.mark.gpu
@@ -36,4 +36,33 @@ def test_sums_over_long_contexts(D, dtype, n, N):
             want = torch.softmax(q[b, h, i].double() @ k[0, :seen].T * D ** -0.5, -1) @ v[0, :seen]
             bound = R.half_step(dtype) * want.abs() + 2.0 ** -23 * ((32 if D == 64 else 16) * 31 * top + n / 64 * 6 / root) \
                 + 6 / root * (weight + 2.0 ** -17) + 6 * (n / 8) ** 0.5 * 2.0 ** -24 / root
+            R.close(out[b, h, i], want, 1.01 * bound, TINY[dtype])
+
+
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("N", [1, 4])
+def test_sums_of_rows_with_one_large_element(D, dtype, N):
+    """Element 3 of every value row is about 20, so that the codes of the others are small ones: their sums are as far from the middle
+    as the offset.  The bound is as above, where a sum is of j values between -1/2 and 15 1/2 steps about the columns' mean: the
+    large element's column drifts by n / 64 steps of 2^-23 of its 20, and the others by as much of a step, their mean being off
+    the columns' mean by what the large one adds, 20 / D, and their own below 1."""
+    n = 131072
+    seqs = R.Sequences([n], 64)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(seqs.pages, 1, 64, D, device="cuda", generator=gen) for _ in range(2))
+    v[..., 3] = 20 + 0.1 * v[..., 3]
+    (k, ks), (v, vs) = (_quantise(t.to(dtype)) for t in (k, v))
+    cache = PagedCache(k, v, k_scales=ks, v_scales=vs, dtype=dtype)
+    q = 0.01 * _heads((512, 4, N, D), dtype, 3)
+    out = sdpa_paged(q, cache, seqs.table.expand(512, -1), seqs.lengths.expand(512))
+    k, _ = R.values(cache, "k", seqs, 0, n)
+    v, step = R.values(cache, "v", seqs, 0, n)
+    root, top = n ** 0.5, float(step.max())
+    for b, h in ((0, 0), (17, 3), (511, 2)):
+        for i in range(N):
+            seen = n - N + i + 1
+            want = torch.softmax(q[b, h, i].double() @ k[0, :seen].T * D ** -0.5, -1) @ v[0, :seen]
+            drift = n / 64 * (want.abs() + 20 / D + 1)
+            bound = R.half_step(dtype) * want.abs() + 2.0 ** -23 * ((32 if D == 64 else 16) * 31 * top + drift) \
+                + 6 / root * (2.0 ** -16 * 31 * top + 2.0 ** -15) + 6 * (n / 8) ** 0.5 * 2.0 ** -24 * 20 / root
             R.close(out[b, h, i], want, 1.01 * bound, TINY[dtype])
