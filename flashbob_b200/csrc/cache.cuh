@@ -11,8 +11,9 @@
 // What bounds these kernels: every row is read and written once.  Page entries and lengths are checked here, for they are
 // known on the GPU only: an entry outside the cache is reported and its rows are neither read nor written.
 //
-// Measured: ragged prompts up to 2048 tokens, 8 x 8 heads of 128 elements in 16 bits 22.7 us (92 MB, 4.0 TB/s); up to 4001 tokens, 2 x 16
-// heads of 64 elements into 4 bits 20 us (the exact rotation and the quotients: instructions), read back 10 to 12.
+// Measured (replayed in a graph): ragged prompts up to 2048 tokens, 8 x 8 heads of 128 elements in 16 bits 20.8 us (92 MB, 4.4 TB/s; 27.3 for
+// 134 MB without raggedness), read back 20.2 (113 MB, 5.6 TB/s); up to 4001 tokens, 2 x 16 heads of 64 elements into 4 bits 19.0 us (the
+// exact rotation and the quotients: instructions), read back 10.3; one token of 64 sequences x 8 heads of 128 elements 2.8, 4 bits 4.7.
 #pragma once
 
 #include "rotary.cuh"

@@ -18,9 +18,9 @@
 // An item inside one CTA is finished there; parts of a divided one are parked and added in the order of the CTAs by
 // combine_kernel, so results do not depend on which CTA finishes first.  The host needs no lengths for any of this.
 //
-// Measured, heads 32/8 of 128 elements, one token: 64 sequences of up to 8192 keys in 16 bits 210 us (6.5 TB/s, what a copy reaches);
-// 16 of up to 16,384 in 4 bits 71 us (2.8 TB/s: 780 instructions a warp and 32 keys, at 12 warps per SM); one sequence of 500 keys 8.3 us
-// (latency).
+// Measured (replayed in a graph), heads 32/8 of 128 elements, one token: 64 sequences of up to 8192 keys in 16 bits 211 us (6.5 TB/s, what
+// a copy reaches); 16 of up to 16,384 in 4 bits 72 us (2.75 TB/s: 795 instructions a warp and 32 keys, at 12 warps per SM); one sequence
+// of 500 keys 8.5 us (latency).
 #pragma once
 
 #include "cache.cuh"

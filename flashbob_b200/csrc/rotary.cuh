@@ -4,13 +4,13 @@
 // same map with the angles negated, so one kernel serves forward and every order of backward.
 //
 // Angles: a frequency is kept as the 64-bit fraction of a turn per position.  position * fraction modulo 2^64 is then
-// the exact angle modulo a turn, for any position, in one integer product, and a sine needs no range reduction;
-// position * frequency in fp32 is off by 0.004 radians at position 100,000.
+// the angle modulo a turn in one integer product, off by 2^-64 turns per position (8e-10 radians at position 2^31), and a sine
+// needs no range reduction; position * frequency in fp32 is off by 0.004 radians at position 100,000.
 //
 // What bounds it: one read and one write of every element.  A thread turns the same 16 elements (8 pairs) of HPT heads of
 // a token, so its 8 sines and cosines are shared by them and their loads are in flight together.  They are the special-
-// function unit's: off by 2^-20.9 at most, a thousandth of the result's rounding in fp16 (sincospif, with four times the
-// instructions, took 31 us for 29.5 on 84 MB with one head a thread, 18 for 17.1 with four).  Measured now: 84 MB in 15.4 us, 5.4 TB/s.
+// function unit's, off by 2^-21.4 and 2^-21.2, of an fp32 angle that is off by 4e-7: 8e-7 together, a six-hundredth of the
+// result's rounding in fp16 (sincospif, with four times the instructions, took 31 us for 29.5 on 84 MB with one head a thread, 18 for 17.1 with four).  Measured now: 84 MB in 15.4 us, 5.4 TB/s.
 #pragma once
 
 #include "ptx.cuh"
@@ -31,7 +31,7 @@ __device__ __forceinline__ int64_t angle_of(int64_t position, uint64_t turn) {  
     return static_cast<int64_t>(static_cast<uint64_t>(position) * turn);
 }
 __device__ __forceinline__ void turn_factors(int64_t position, uint64_t turn, float& s, float& c) {
-    // the upper 32 bits: 2^-33 of a turn, 7e-10 radians
+    // the upper 32 bits, 7e-10 radians; in fp32 and times 2 pi / 2^32 off by up to 4e-7
     const float x = static_cast<float>(static_cast<int32_t>(angle_of(position, turn) >> 32)) * 1.4629180792671596e-9f;      // 2 pi / 2^32
     s = __sinf(x);
     c = __cosf(x);

@@ -12,7 +12,8 @@ read by the host, so a step can be captured in a CUDA graph (after one eager cal
 
 A cache of 4 bits keeps a row of a head as codes 0 ... 15 (element 2 j in the low half of byte j) and fp32 (scale, zero):
 value = code * scale + zero, with zero the row's minimum and scale 1/15 of its range (1 where that is nothing), fp32 throughout.  Keys
-are turned and rounded to the cache's 16-bit type before they are coded.  A row with a NaN or infinity reads as not finite.
+are turned and rounded to the cache's 16-bit type before they are coded.  A row with a NaN or infinity, or a range beyond fp32's,
+reads as not finite.
 
 CUDA tensors go through libbob_sm100.so (csrc/cache.cuh, csrc/paged.cuh); there is no fallback.  CPU tensors take plain
 tensor operations.  Nothing here records gradients: `read_kv` brings a cached context back to contiguous keys and values,
@@ -233,7 +234,7 @@ def append_kv(k: torch.Tensor, v: torch.Tensor, cache: PagedCache, page_table: t
 
     Row i < counts[b] of sequence b goes to position lengths[b] - counts[b] + i; the rows from counts[b] on are padding and not
     looked at, and no other row of the cache changes.  Pages may be shared between sequences as long as nothing is
-    written to them: two new rows for one place leave either there.
+    written to them: of two new rows for one place, parts of both may be left there.
     """
     # The usual valid CUDA call is recognised natively; everything else takes the checks below.
     turn_args = _plain_rotary(rotary)
@@ -299,9 +300,9 @@ def sdpa_paged(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor, len
     keeps keys at positions up to the query's, `window_size` w > 0 further keeps only the last w of them; without
     `is_causal` every query sees all lengths[b] keys, as in cross attention to cached encoder states (such queries have no
     position among the keys: there may be more of them, and `rotary` is refused).  Rows from counts[b] on, and rows without keys, are zero.
-    Key and value rows that no query of its sequence attends to have no part in the result, whatever they hold; a NaN or infinity
-    among the values that some queries of a sequence attend to may reach its other queries of the same call, as in any
-    product of probabilities and values.  H_Q is a multiple of H_KV, up to 32 times.
+    Key and value rows that no query of its sequence attends to have no part in the result, whatever they hold; a NaN in a query or
+    in a key that it attends to makes its result NaN and no other; a NaN or infinity among the values that some queries of a
+    sequence attend to may reach its other queries of the same call, as in any product of probabilities and values.  H_Q is a multiple of H_KV, up to 32 times.
 
     Up to 16 rows (tokens of the call x H_Q / H_KV), in fp16 over 4 bits up to 64, only the result is rounded to 16 bits; beyond,
     turned queries, probabilities and rows of 4 bits are too, as in `apply_rotary` and `read_kv` followed by `sdpa_bob`.

@@ -8,9 +8,10 @@ A pair of elements at position t is turned by t * frequency; the gradient turns 
 differentiated any number of times, as second-order steps need.  The same `Rotary` goes to `append_kv` and `sdpa_paged`
 (flashbob_b200/paged.py), which turn keys and queries on their way.
 
-CUDA tensors go through libbob_sm100.so (csrc/rotary.cuh); CPU tensors take plain tensor operations.  Angles are exact to
-a few 1e-10 radians at any position: a frequency is kept as a 64-bit fraction of a turn, and position * fraction is taken
-modulo a turn in integers.
+CUDA tensors go through libbob_sm100.so (csrc/rotary.cuh); CPU tensors take plain tensor operations, angles in 64 bits.  On the
+GPU a frequency is kept as a 64-bit fraction of a turn, and position * fraction is taken modulo a turn in integers: off by
+2^-64 of a turn per position, 8e-10 radians at position 2^31 and 4e-7 at 2^40.  16-bit results take the angle and its sines in
+fp32, off by 8e-7 together; keys for a 4-bit cache are turned in 64 bits.
 """
 
 from __future__ import annotations
