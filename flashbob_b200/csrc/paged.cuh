@@ -526,12 +526,11 @@ __global__ void __launch_bounds__(kPagedThreads, (PagedConfig<D, ROWS, BITS>::CT
                 auto column_sum = [&](int i, int e) -> float& { return acc[PARTS ? 0 : k / 2][i][ROWS == 8 ? e : 2 * (k % 2) + e]; };
                 float mean = 0.f, weights = w_sum[k];
                 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) mean += column_sum(i, 0) + column_sum(i, 1);
+                for (int i = 0; i < D / 8; ++i) mean = fmaf(column_sum(i, 0) + column_sum(i, 1), 1.f / D, mean);     // (no sum of columns overflows)
                 mean += __shfl_xor_sync(0xffffffffu, mean, 1);
                 weights += __shfl_xor_sync(0xffffffffu, weights, 1);
                 mean += __shfl_xor_sync(0xffffffffu, mean, 2);
                 weights += __shfl_xor_sync(0xffffffffu, weights, 2);
-                mean *= 1.f / D;
                 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
                     column_sum(i, 0) -= mean;
