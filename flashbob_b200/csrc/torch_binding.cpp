@@ -13,6 +13,7 @@
 #include "../../include/bob_sm100.h"
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -276,9 +277,15 @@ int32_t dtype_of(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? BO
 void finish_reported(int rc, const char* what, int device, bool check_status) {
     if (rc) fail(what, rc);
     if (check_status) c10::cuda::getCurrentCUDAStream(device).synchronize();
-    if ((rc = lib.last_status(device)))
+    if ((rc = lib.last_status(device))) {
+        // a call's kernels, and their threads, report one after another: what is still to come is part of this error
+        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) {
+            c10::cuda::getCurrentCUDAStream(device).synchronize();
+            lib.last_status(device);
+        }
         fail((check_status ? std::string(what) + " (device status)" : "an earlier libbob_sm100 kernel on cuda:" + std::to_string(device) +
               " (seen after " + what + "; its results are undefined)"), rc);
+    }
 }
 
 struct Rotation {
