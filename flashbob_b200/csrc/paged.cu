@@ -397,7 +397,7 @@ static int run_paged(const bob_sm100_paged_args* a, void* workspace, cudaStream_
         constexpr bool BF = decltype(bf16)::value;
         auto dim = [&](auto rows, auto bits) {
             constexpr int ROWS = decltype(rows)::value, BITS = decltype(bits)::value;
-            if constexpr (ROWS == 32 && BITS == 4 && !BF) return;        // (paged_plan)
+            if constexpr (ROWS == 32 && BITS == 4 && !BF) rc = kBadGeom;      // (paged_plan takes 16 at a time)
             else if (a->cache.D == 32) rc = launch_paged<32, ROWS, BF, BITS>(p, a->cache.device, stream);
             else if (a->cache.D == 64) rc = launch_paged<64, ROWS, BF, BITS>(p, a->cache.device, stream);
             else rc = launch_paged<128, ROWS, BF, BITS>(p, a->cache.device, stream);
